@@ -1,0 +1,438 @@
+"""The feed-forward operators that a program built on ``hstu_amd`` calls around
+its HSTU layers, as cases to time.
+
+A case is one pass: the RMS norm with the residual's addition (serving, with an
+e4m3 output and its row scales; training, with its backward), the gated
+feed-forward projection (bf16 serving and training, e4m3 serving), and the
+microscaled 4-bit format (quantisation, and a linear layer of 4-bit weights
+that quantises its activations on the way).  ``own`` False computes a pass in
+plain torch operations, True by the package's entry points; ``exact`` is the
+operators' definition in 64 bits.
+"""
+
+import math
+import os
+import sys
+
+import torch
+
+sys.path.insert(1, os.path.join(os.getcwd(), "mlperf-training_amd"))
+
+own = False
+
+E4M3 = torch.float8_e4m3fn
+E4M3_MAX = 448.0
+EPS = 1e-6
+WIDTH = 512          # embedding width of the HSTU layer
+FULL_TOKENS = 162251   # tokens of the full training batch
+MEDIUM_TOKENS = 37429  # tokens of the medium batch
+TYPES = {"bf16": torch.bfloat16, "f32": torch.float32}
+MAX_NORM = FULL_TOKENS * WIDTH               # values of the largest norm / quantisation case
+MAX_GATED = 8192 * 10240 * 4096              # rows x hidden x features of the largest gated case
+MAX_MX = 8192 * 8192 * 8192                  # rows x outputs x inputs of the largest 4-bit product
+
+
+# ---------------------------------------------------------------------------
+# the cases
+# ---------------------------------------------------------------------------
+def listed():
+    return [
+        # the norm of one new token, quantised for an e4m3 product: one call of a decoding loop
+        dict(name="norm_fp8_token", path="norm_fp8", dtype="bf16", rows=1, width=2048, residual=True, strided=False),
+        # the norm before the feed-forward block of the full batch, scored in e4m3
+        dict(name="norm_fp8_full", path="norm_fp8", dtype="bf16", rows=FULL_TOKENS, width=WIDTH, residual=True,
+             strided=False),
+        # training on the medium batch: the residual sum, the norm and its backward
+        dict(name="norm_train_medium", path="norm_train", dtype="bf16", rows=MEDIUM_TOKENS, width=WIDTH,
+             residual=True, strided=False),
+        # training a wide model with its residual stream in fp32, an odd number of rows
+        dict(name="norm_train_wide", path="norm_train", dtype="f32", rows=4099, width=5120, residual=False,
+             strided=False),
+        # a handful of tokens through the gate and up projections: bound by the weights
+        dict(name="gated_decode", path="gated_fwd", rows=7, features=2048, hidden=5632, act="silu"),
+        # training on the medium batch at the layer's width
+        dict(name="gated_train_medium", path="gated_train", rows=MEDIUM_TOKENS, features=WIDTH, hidden=2048,
+             act="silu"),
+        # training a wide feed-forward block
+        dict(name="gated_train_wide", path="gated_train", rows=8192, features=4096, hidden=10240, act="gelu"),
+        # scoring the medium batch in e4m3, activations scaled by row, weights by column
+        dict(name="gated_fp8_medium", path="gated_fp8", rows=MEDIUM_TOKENS, features=1024, hidden=4096, act="silu"),
+        # the values that 4-bit activations stand for, as quantisation-aware evaluation takes them
+        dict(name="mx_values_full", path="mx_values", dtype="bf16", rows=FULL_TOKENS, width=WIDTH),
+        # packing a matrix of fp32 master weights
+        dict(name="mx_values_weight", path="mx_values", dtype="f32", rows=2048, width=5632),
+        # a decoding step's linear layer with 4-bit weights, residual added
+        dict(name="mx_linear_decode", path="mx_linear", rows=5, features=5632, outputs=2048, residual=True),
+        # a large batch through a linear layer with 4-bit weights
+        dict(name="mx_linear_large", path="mx_linear", rows=8192, features=8192, outputs=8192, residual=False),
+    ]
+
+
+def _log(rng, low, high):
+    return int(math.exp(rng.uniform(math.log(low), math.log(high + 1))))
+
+
+def _step(rng, low, high, step):
+    return min(high, max(low, round(_log(rng, low, high) / step) * step))
+
+
+def draw(rng):
+    path = rng.choice(["norm_fp8", "norm_train", "gated_fwd", "gated_train", "gated_fp8", "mx_values", "mx_linear"])
+    if path in ("norm_fp8", "norm_train"):
+        width = _step(rng, 64, 8192, rng.choice([8, 64, 1]))
+        return dict(path=path, dtype=rng.choice(["bf16", "bf16", "f32"]),
+                    rows=_log(rng, 1, min(FULL_TOKENS, MAX_NORM // width)), width=width,
+                    residual=rng.random() < 0.6, strided=rng.random() < 0.3)
+    if path == "mx_values":
+        width = _step(rng, 32, 8192, 32)
+        return dict(path=path, dtype=rng.choice(["bf16", "bf16", "f32"]),
+                    rows=_log(rng, 1, min(FULL_TOKENS, MAX_NORM // width)), width=width)
+    if path == "mx_linear":
+        features, outputs = _step(rng, 128, 8192, 128), _step(rng, 16, 8192, 16)
+        return dict(path=path, rows=_log(rng, 1, min(65536, MAX_MX // (features * outputs))), features=features,
+                    outputs=outputs, residual=rng.random() < 0.5)
+    features, hidden = _step(rng, 256, 4096, 256), _step(rng, 128, 10240, 128)
+    return dict(path=path, rows=_log(rng, 1, min(FULL_TOKENS, MAX_GATED // (3 * features * hidden))),
+                features=features, hidden=hidden, act=rng.choice(["silu", "silu", "gelu", "sigmoid"]))
+
+
+# ---------------------------------------------------------------------------
+# what a pass cannot do without
+# ---------------------------------------------------------------------------
+def work(case):
+    path = case["path"]
+    if path in ("norm_fp8", "norm_train"):
+        n, es = case["rows"] * case["width"], 2 if case["dtype"] == "bf16" else 4
+        res = 2 if case["residual"] else 0  # the residual in, the new one out
+        if path == "norm_fp8":
+            return {"bytes": n * (es * (1 + res) + 1) + 4 * case["rows"] + 4 * case["width"], "flops": 6 * n}
+        # forward: x (and the residual) in, y (and the new residual) out; backward: dy, h (and its gradient) in, dx out
+        return {"bytes": n * es * (2 + res + 3 + res // 2) + 8 * case["width"], "flops": 14 * n}
+    if path == "mx_values":
+        n, es = case["rows"] * case["width"], 2 if case["dtype"] == "bf16" else 4
+        return {"bytes": n * (es + 2 + 1 / 32), "flops": 4 * n}
+    if path == "mx_linear":
+        m, k, n = case["rows"], case["features"], case["outputs"]
+        out = 2 * m * n * (2 if case["residual"] else 1)
+        return {"bytes": 2 * m * k + n * k * 17 / 32 + out, "flops": 2 * m * n * k}
+    m, d, f = case["rows"], case["features"], case["hidden"]
+    if path == "gated_fp8":
+        return {"bytes": m * d + 2 * f * d + 4 * m + 8 * f + 2 * m * f, "flops": 4 * m * f * d}
+    if path == "gated_fwd":
+        return {"bytes": 2 * (m * d + 2 * f * d + m * f), "flops": 4 * m * f * d}
+    # training: x and the weights in and their gradients out, the output and its gradient
+    return {"bytes": 2 * (2 * m * d + 4 * f * d + 2 * m * f), "flops": 12 * m * f * d}
+
+
+# ---------------------------------------------------------------------------
+# the inputs
+# ---------------------------------------------------------------------------
+def _activations(gen, rows, width, dtype):
+    """Rows of a residual stream: unit normal, a few channels ten times as large."""
+    x = torch.randn(rows, width, generator=gen, device="cuda", dtype=torch.float32)
+    loud = torch.rand(width, generator=gen, device="cuda") < 0.01
+    return (x * (1.0 + 9.0 * loud)).to(dtype)
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+
+    def normal(*shape, std=1.0, dtype=torch.bfloat16):
+        return (torch.randn(*shape, generator=gen, device="cuda", dtype=torch.float32) * std).to(dtype)
+
+    path = case["path"]
+    s = dict(case=case)
+    if path in ("norm_fp8", "norm_train"):
+        rows, width, dt = case["rows"], case["width"], TYPES[case["dtype"]]
+        if case["strided"]:  # columns of a wider buffer
+            s["x"] = _activations(gen, rows, 2 * width + 8, dt)[:, 8:8 + width]
+        else:
+            s["x"] = _activations(gen, rows, width, dt)
+        s["residual"] = _activations(gen, rows, width, dt) if case["residual"] else None
+        s["weight"] = 1.0 + normal(width, std=0.2, dtype=torch.float32)
+        if path == "norm_train":
+            s["dy"] = normal(rows, width, std=0.1, dtype=dt)
+            s["dh"] = normal(rows, width, std=0.1, dtype=dt) if case["residual"] else None
+            for name in ("x", "residual", "weight"):
+                if s[name] is not None:
+                    s[name].requires_grad_(True)
+        return s
+    if path == "mx_values":
+        s["x"] = _activations(gen, case["rows"], case["width"], TYPES[case["dtype"]])
+        return s
+    if path == "mx_linear":
+        s["x"] = _activations(gen, case["rows"], case["features"], torch.bfloat16)
+        w = normal(case["outputs"], case["features"], std=case["features"] ** -0.5, dtype=torch.float32)
+        s["weight"] = _mx_pack(w)  # packed once, kept by the program
+        s["bias"] = normal(case["outputs"], std=0.1)
+        s["residual"] = normal(case["rows"], case["outputs"]) if case["residual"] else None
+        return s
+    m, d, f = case["rows"], case["features"], case["hidden"]
+    x = normal(m, d)
+    gate, up = normal(f, d, std=1.5 * d ** -0.5), normal(f, d, std=d ** -0.5)
+    if path == "gated_fp8":
+        s["x"], s["x_scale"] = _e4m3_rows(x.float())
+        s["gate"], s["up"] = _e4m3_rows(gate.float()), _e4m3_rows(up.float())  # (values, scale of each output)
+        return s
+    s["x"], s["gate"], s["up"] = x, gate, up
+    if path == "gated_train":
+        s["dh"] = normal(m, f, std=0.1)
+        for name in ("x", "gate", "up"):
+            s[name].requires_grad_(True)
+    return s
+
+
+# ---------------------------------------------------------------------------
+# the formats, in plain operations
+# ---------------------------------------------------------------------------
+def _e4m3_rows(v):
+    """(e4m3 values, fp32 scale of each row): the scale takes the row's largest magnitude to 448."""
+    amax = v.abs().amax(-1)
+    scale = torch.where(amax > 0, amax, torch.ones_like(amax)) / E4M3_MAX
+    return (v / scale[:, None]).clamp(-E4M3_MAX, E4M3_MAX).to(E4M3), scale
+
+
+def _mx_scale_exponent(blocks):
+    """E of each block of 32: floor(log2 amax) - 2, -127 at the least."""
+    amax = blocks.abs().amax(-1)
+    exponent = torch.frexp(amax)[1] - 3
+    return torch.where(amax > 0, exponent, torch.full_like(exponent, -127)).clamp(min=-127)
+
+
+def _mx_split(v):
+    """(e2m1 codes 0..15 [R, C], E [R, C / 32]) of fp32 or fp64 rows; nearest, ties to the even code."""
+    blocks = v.reshape(v.shape[0], -1, 32)
+    exponent = _mx_scale_exponent(blocks)
+    t = torch.ldexp(blocks.abs(), -exponent[..., None])
+    code = ((t > 0.25).int() + (t >= 0.75) + (t > 1.25) + (t >= 1.75) + (t > 2.5) + (t >= 3.5) + (t > 5.0))
+    code = code + 8 * torch.signbit(blocks)
+    return code.reshape(v.shape), exponent
+
+
+def _mx_pack(v):
+    """(codes uint8 [R, C / 2], two a byte, the even column in the low half; scales uint8 [R, C / 32] = E + 127)."""
+    code, exponent = _mx_split(v)
+    pairs = code.reshape(v.shape[0], -1, 2)
+    return (pairs[..., 0] + 16 * pairs[..., 1]).to(torch.uint8), (exponent + 127).to(torch.uint8)
+
+
+def _mx_values(code, exponent, dtype):
+    table = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -3.0, -4.0, -6.0],
+                         dtype=dtype, device=code.device)
+    v = table[code.long()].reshape(code.shape[0], -1, 32)
+    return torch.ldexp(v, exponent[..., None]).reshape(code.shape)
+
+
+def _mx_unpack(packed, dtype):
+    codes, scales = packed
+    code = torch.stack((codes & 15, codes >> 4), -1).reshape(codes.shape[0], -1)
+    return _mx_values(code, scales.int() - 127, dtype)
+
+
+# ---------------------------------------------------------------------------
+# one pass
+# ---------------------------------------------------------------------------
+def _act(name, g):
+    """(a(g), a'(g))"""
+    if name == "gelu":  # tanh form: g sigmoid(2 c (g + 0.044715 g^3)), c = sqrt(2 / pi)
+        c = 2.0 * math.sqrt(2.0 / math.pi)
+        sg = torch.sigmoid(c * (g + 0.044715 * g * g * g))
+        return g * sg, sg + g * sg * (1 - sg) * c * (1 + 3 * 0.044715 * g * g)
+    sg = torch.sigmoid(g)
+    if name == "sigmoid":
+        return sg, sg * (1 - sg)
+    return g * sg, sg + g * sg * (1 - sg)
+
+
+def _norm_plain(s, wide):
+    """(h, y, rstd) with h rounded as it is kept, the rest in `wide`."""
+    x = s["x"].detach()
+    h = x if s["residual"] is None else (x.to(wide) + s["residual"].detach().to(wide)).to(x.dtype)
+    hw = h.to(wide)
+    rstd = torch.rsqrt((hw * hw).mean(-1, keepdim=True) + EPS)
+    return h, hw * rstd * s["weight"].detach().to(wide), rstd
+
+
+def _norm_backward_plain(s, h, rstd, wide):
+    dy, hw = s["dy"].to(wide), h.to(wide)
+    c, xhat = dy * s["weight"].detach().to(wide), hw * rstd
+    dx = rstd * (c - xhat * (c * xhat).mean(-1, keepdim=True))
+    if s["dh"] is not None:
+        dx = dx + s["dh"].to(wide)
+    return dx, (dy * xhat).sum(0)
+
+
+def _gated_plain(case, x, gate, up):
+    g, u = x @ gate.t(), x @ up.t()
+    a, da = _act(case["act"], g)
+    return a * u, a, da, u
+
+
+def _run_plain(s):
+    case = s["case"]
+    path = case["path"]
+    f32 = torch.float32
+    if path == "norm_fp8":
+        h, y, _ = _norm_plain(s, f32)
+        y8, scale = _e4m3_rows(y)
+        out = {"y": y8, "scale": scale}
+        if s["residual"] is not None:
+            out["h"] = h
+        return out
+    if path == "norm_train":
+        h, y, rstd = _norm_plain(s, f32)
+        # the weight's gradient is a sum over every row: in 64 bits
+        dx, dw = _norm_backward_plain(s, h, rstd, f32)
+        dw = (s["dy"].double() * (h.double() * rstd.double())).sum(0)
+        dt = h.dtype
+        out = {"y": y.to(dt), "dx": dx.to(dt), "dweight": dw.to(f32)}
+        if s["residual"] is not None:
+            out["h"], out["dresidual"] = h, out["dx"]
+        return out
+    if path == "mx_values":
+        code, exponent = _mx_split(s["x"].float())
+        return {"values": _mx_values(code, exponent, f32).to(torch.bfloat16),
+                "scales": (exponent + 127).to(torch.uint8)}
+    if path == "mx_linear":
+        code, exponent = _mx_split(s["x"].float())
+        out = _mx_values(code, exponent, f32) @ _mx_unpack(s["weight"], f32).t() + s["bias"].float()
+        if s["residual"] is not None:
+            out = out + s["residual"].float()
+        return out.to(torch.bfloat16)
+    if path == "gated_fp8":
+        x = s["x"].float() * s["x_scale"][:, None]
+        gate, up = (w.float() * scale[:, None] for w, scale in (s["gate"], s["up"]))
+        return _gated_plain(case, x, gate, up)[0].to(torch.bfloat16)
+    x, gate, up = (s[n].detach().float() for n in ("x", "gate", "up"))
+    h, a, da, u = _gated_plain(case, x, gate, up)
+    bf = torch.bfloat16
+    if path == "gated_fwd":
+        return h.to(bf)
+    dh = s["dh"].float()
+    dg, du = dh * u * da, dh * a
+    return {"h": h.to(bf), "dx": (dg @ gate + du @ up).to(bf), "dgate": (dg.t() @ x).to(bf), "dup": (du.t() @ x).to(bf)}
+
+
+def _run_own(s):
+    import hstu_amd
+
+    case = s["case"]
+    path = case["path"]
+    if path == "norm_fp8":
+        if s["residual"] is None:
+            y8, scale = hstu_amd.rms_norm_fp8(s["x"], s["weight"], EPS)
+            return {"y": y8, "scale": scale}
+        y8, scale, h = hstu_amd.rms_norm_fp8(s["x"], s["weight"], EPS, residual=s["residual"])
+        return {"y": y8, "scale": scale, "h": h}
+    if path == "norm_train":
+        if s["residual"] is None:
+            y = hstu_amd.rms_norm(s["x"], s["weight"], EPS)
+            dx, dw = torch.autograd.grad(y, (s["x"], s["weight"]), s["dy"])
+            return {"y": y, "dx": dx, "dweight": dw}
+        y, h = hstu_amd.rms_norm(s["x"], s["weight"], EPS, residual=s["residual"])
+        dx, dres, dw = torch.autograd.grad((y, h), (s["x"], s["residual"], s["weight"]), (s["dy"], s["dh"]))
+        return {"y": y, "dx": dx, "dweight": dw, "h": h, "dresidual": dres}
+    if path == "mx_values":
+        codes, scales = hstu_amd.quantize_mxfp4(s["x"])
+        return {"values": hstu_amd.dequantize_mxfp4(codes, scales), "scales": scales}
+    if path == "mx_linear":
+        return hstu_amd.mxfp4_linear(s["x"], s["weight"], bias=s["bias"], residual=s["residual"])
+    if path == "gated_fp8":
+        return hstu_amd.gated_linear_fp8(s["x"], s["x_scale"], s["gate"], s["up"], activation=case["act"])
+    h = hstu_amd.gated_linear(s["x"], s["gate"], s["up"], activation=case["act"])
+    if path == "gated_fwd":
+        return h
+    dx, dgate, dup = torch.autograd.grad(h, (s["x"], s["gate"], s["up"]), s["dh"])
+    return {"h": h, "dx": dx, "dgate": dgate, "dup": dup}
+
+
+def run(state):
+    return _run_own(state) if own else _run_plain(state)
+
+
+# ---------------------------------------------------------------------------
+# the definitions in 64 bits
+# ---------------------------------------------------------------------------
+def _sigmoid64(z):
+    return torch.where(z >= 0, 1 / (1 + torch.exp(-z.abs())), torch.exp(-z.abs()) / (1 + torch.exp(-z.abs())))
+
+
+def _act64(name, g):
+    if name == "gelu":
+        z = math.sqrt(2.0 / math.pi) * (g + 0.044715 * g ** 3)
+        th = torch.tanh(z)
+        dz = math.sqrt(2.0 / math.pi) * (1 + 0.134145 * g ** 2)
+        return 0.5 * g * (1 + th), 0.5 * (1 + th) + 0.5 * g * (1 - th ** 2) * dz
+    sg = _sigmoid64(g)
+    return (sg, sg * (1 - sg)) if name == "sigmoid" else (g * sg, sg * (1 + g * (1 - sg)))
+
+
+_E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def _mx64(v):
+    """The values that rows of v stand for in the 4-bit format, and each block's exponent."""
+    b = v.double().reshape(v.shape[0], -1, 32)
+    top = b.abs().max(-1).values
+    # floor(log2) from the largest power of two that is no larger, without trusting log2's last bit
+    e = torch.floor(torch.log2(top.clamp(min=2.0 ** -130)))
+    e = torch.where(torch.exp2(e) > top, e - 1, e)
+    e = torch.where(torch.exp2(e + 1) <= top, e + 1, e)
+    e = torch.where(top > 0, (e - 2).clamp(min=-127), torch.full_like(e, -127))
+    unit = torch.exp2(e)[..., None]
+    t = (b.abs() / unit).clamp(max=6.0)
+    # steps of 0.5 up to 2, 1 up to 4, 2 beyond; torch.round takes ties to even
+    step = torch.where(t < 2, 0.5, torch.where(t < 4, 1.0, 2.0))
+    q = torch.round(t / step) * step
+    return (torch.sign(b) * q * unit).reshape(v.shape), e
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    path = case["path"]
+    if path in ("norm_fp8", "norm_train"):
+        x, w = s["x"].detach(), s["weight"].detach().double()
+        total = x.double() if s["residual"] is None else x.double() + s["residual"].detach().double()
+        h = total.to(x.dtype).double()  # the norm is of the residual stream as it is kept
+        r = (h.square().sum(-1, keepdim=True) / case["width"] + EPS) ** -0.5
+        y = h * r * w
+        if path == "norm_fp8":
+            top = y.abs().amax(-1)
+            scale = torch.where(top > 0, top, 1.0) / E4M3_MAX
+            out = {"y": y / scale[:, None], "scale": scale}
+            if s["residual"] is not None:
+                out["h"] = total
+            return out
+        dy = s["dy"].double()
+        inner = (dy * w * h).sum(-1, keepdim=True) / case["width"]
+        dx = r * dy * w - h * r ** 3 * inner
+        if s["dh"] is not None:
+            dx = dx + s["dh"].double()
+        out = {"y": y, "dx": dx, "dweight": (dy * h * r).sum(0)}
+        if s["residual"] is not None:
+            out["h"], out["dresidual"] = total, dx
+        return out
+    if path == "mx_values":
+        return {"values": _mx64(s["x"])[0], "scales": None}
+    if path == "mx_linear":
+        codes, scales = s["weight"]
+        nibbles = torch.stack((codes % 16, codes // 16), 2).flatten(1).long()
+        size = torch.tensor(_E2M1, dtype=torch.float64, device=codes.device)[nibbles % 8]
+        unit = torch.exp2(scales.double() - 127).repeat_interleave(32, 1)
+        w = torch.where(nibbles >= 8, -size, size) * unit
+        out = _mx64(s["x"])[0] @ w.t() + s["bias"].double()
+        return out if s["residual"] is None else out + s["residual"].double()
+    if path == "gated_fp8":
+        x = s["x"].double() * s["x_scale"].double()[:, None]
+        gate, up = (v.double() * scale.double()[:, None] for v, scale in (s["gate"], s["up"]))
+        return _act64(case["act"], x @ gate.t())[0] * (x @ up.t())
+    x, gate, up = (s[n].detach().double() for n in ("x", "gate", "up"))
+    g, u = x @ gate.t(), x @ up.t()
+    a, da = _act64(case["act"], g)
+    if path == "gated_fwd":
+        return a * u
+    dh = s["dh"].double()
+    h = a * u
+    dg, du = dh * u * da, dh * a
+    del g, u, a, da, dh
+    return {"h": h, "dx": dg @ gate + du @ up, "dgate": dg.t() @ x, "dup": du.t() @ x}
