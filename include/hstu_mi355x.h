@@ -605,6 +605,41 @@ int hstu_quantize_do_e4m3_blk(int dtype, const void* dout, int64_t dout_row_stri
 int hstu_dequantize_do_e4m3_blk(const void* dout_e4m3, const void* e8, int64_t T, int H, int D, void* out,
                                 int64_t out_row_stride, hipStream_t stream);
 
+/*
+ * RMS norm with the residual's addition.
+ *   h = round(x + residual) (h = x when residual is NULL; then the h argument
+ *   is ignored), rstd = 1 / sqrt(mean(h^2) + eps), y = h * rstd * weight.
+ * x, residual, h: [rows, D] of dtype (HSTU_DTYPE_BF16 or HSTU_DTYPE_FP32), row
+ * strides in elements; any D up to 32768, any alignment of whole elements
+ * (rows of 16-byte multiples at 16-byte addresses take 16-byte accesses).
+ * weight [D] bf16 or fp32 (param_dtype).  The norm is of the rounded h, the one
+ * a backward has.  out_dtype: dtype, or HSTU_DTYPE_FP8_E4M3: y = e4m3(clamp(y /
+ * s, +-448)) with s = scale_in[0] (one given fp32 on the device) or, with
+ * scale_in NULL, the row's own s = max|y| / 448 (1 / 448 for a row of zeros),
+ * written to scale_out [rows]; exactly one of the two is given.  NaN stays
+ * NaN.  rstd: fp32 [rows] for the backward, or NULL.  Statistics are fp32.
+ * h may be x or residual, and y may be x, in place (same pointer and stride).
+ * No counterpart in the reference's HSTU path, which norms with LayerNorm
+ * (ops/triton/triton_layer_norm.py:1668-1740).
+ */
+int hstu_rms_norm_fwd(int dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight,
+                      int param_dtype, float eps, int64_t rows, int D, void* h, int64_t ldh, void* y, int64_t ldy,
+                      int out_dtype, const float* scale_in, float* scale_out, float* rstd, hipStream_t stream);
+
+/*
+ * Backward: with c = weight * dy and xhat = h * rstd,
+ *   dx = rstd (c - xhat mean(c xhat)) [+ dh]   (the gradient of x and of residual),
+ *   dweight = sum over rows of dy * xhat (bf16 or fp32, dweight_dtype; zeros without rows).
+ * dh: the gradient of the returned h, or NULL.  Deterministic: the blocks'
+ * sums go to the workspace (hstu_rms_norm_bwd_workspace_bytes, 16-byte aligned)
+ * and are added in a fixed order.
+ */
+int64_t hstu_rms_norm_bwd_workspace_bytes(int64_t rows, int D);
+int hstu_rms_norm_bwd(int dtype, const void* dy, int64_t lddy, const void* h, int64_t ldh, const void* dh, int64_t lddh,
+                      const void* weight, int param_dtype, const float* rstd, int64_t rows, int D, void* dx,
+                      int64_t lddx, void* dweight, int dweight_dtype, void* workspace, int64_t workspace_bytes,
+                      hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -196,6 +196,16 @@ __device__ __forceinline__ uint32_t pack_fp8x4(float a, float b, float c, float 
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
 
+// v / s rounded to fp32 exactly as the division, from y = 1 / s (correctly
+// rounded): q0 = v y, r = v - q0 s (exact with the FMA), q = q0 + r y
+// (Markstein's correction, Handbook of Floating-Point Arithmetic sec. 4.7).
+// Non-finite q0 (v infinite or NaN, or v y overflowing) is kept as is.
+__device__ __forceinline__ float div_by(float v, float s, float y) {
+  const float q0 = v * y;
+  const float q = __builtin_fmaf(__builtin_fmaf(-q0, s, v), y, q0);
+  return __builtin_fabsf(q0) < __builtin_huge_valf() ? q : q0;
+}
+
 // two e4m3 bytes (low or high half of w) -> two bf16, exact (scale 1.0)
 template <bool HI>
 __device__ __forceinline__ uint32_t cvt_fp8x2_bf16(uint32_t w) {

@@ -521,16 +521,6 @@ __device__ __forceinline__ int wide_col(int g, int e) {
   else return e < 8 ? 8 * g + e : 32 + 8 * g + (e - 8);
 }
 
-// v / s rounded to fp32 exactly as the division, from y = 1 / s (correctly
-// rounded): q0 = v y, r = v - q0 s (exact with the FMA), q = q0 + r y
-// (Markstein's correction, Handbook of Floating-Point Arithmetic sec. 4.7).
-// Non-finite q0 (v infinite or NaN, or v y overflowing) is kept as is.
-__device__ __forceinline__ float div_by(float v, float s, float y) {
-  const float q0 = v * y;
-  const float q = __builtin_fmaf(__builtin_fmaf(-q0, s, v), y, q0);
-  return __builtin_fabsf(q0) < __builtin_huge_valf() ? q : q0;
-}
-
 // Barriers without a memory fence (a fence would make the MFMA waves wait
 // for their own stores): the MFMA waves wait for their LDS reads only, the
 // loader for its loads up to the last VM outstanding ones.

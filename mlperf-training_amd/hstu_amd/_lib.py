@@ -10,6 +10,7 @@ is missing or does not load, every entry point raises ``HstuUnavailableError``
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -66,6 +67,9 @@ EXPORTED_SYMBOLS = (
     "hstu_attn_bwd_fp8_workspace_bytes",
     "hstu_attn_bwd_fp8_dkdv",
     "hstu_attn_bwd_fp8_dq",
+    "hstu_rms_norm_fwd",
+    "hstu_rms_norm_bwd_workspace_bytes",
+    "hstu_rms_norm_bwd",
 )
 
 
@@ -178,6 +182,15 @@ _SIGNATURES = {
         [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _i32,
          _f32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp],
     ),
+    "hstu_rms_norm_fwd": (
+        _i32,
+        [_i32, _vp, _i64, _vp, _i64, _vp, _i32, _f32, _i64, _i32, _vp, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _vp],
+    ),
+    "hstu_rms_norm_bwd_workspace_bytes": (_i64, [_i64, _i32]),
+    "hstu_rms_norm_bwd": (
+        _i32,
+        [_i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _vp, _i64, _i32, _vp, _i64, _vp, _i32, _vp, _i64, _vp],
+    ),
 }
 
 
@@ -225,6 +238,22 @@ def check(status: int, what: str) -> None:
                HSTU_E_SCRATCH_TOO_SMALL: "needs more than the allocation-free entry point's scratch"}.get(
             status, f"hipError {status}")
         raise HstuKernelError(f"{what} failed: {msg}")
+
+
+def stream(t) -> int:
+    """The current stream of the tensor's device."""
+    import torch
+
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def on_device(t):
+    """A context in which the tensor's device is the current one, which a launch on its stream needs."""
+    import torch
+
+    if t.device.index is None or t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
 
 
 def ptr(t) -> Optional[int]:

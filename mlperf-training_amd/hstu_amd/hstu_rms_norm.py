@@ -1,0 +1,170 @@
+"""RMS norm with the residual's addition (``csrc/hstu_rms_norm.hip``):
+
+    h = round(x + residual)        (h = x without a residual)
+    y = h / sqrt(mean(h^2) + eps) * weight
+
+over the last dimension, for bf16 and fp32 activations and bf16 or fp32
+weights of any width up to 32768.  It stands beside the weighted LayerNorm
+(``triton_weighted_layer_norm_fwd``), which the reference norms with
+(``ops/triton/triton_layer_norm.py:1668-1740``); the reference's HSTU layer
+has no RMS norm.
+
+* ``rms_norm``: differentiable, ``y`` or ``(y, h)``;
+* ``rms_norm_fp8``: e4m3 output with the scale of each row (what
+  ``fp8.fp8_gemm`` and ``gated_linear_fp8`` take as ``a_scale``) or at one given
+  scale;
+* ``rms_norm_fwd`` / ``rms_norm_bwd``: the two kernels.
+
+The norm is of the rounded ``h`` that is returned, so that the gradients, for
+which only that ``h`` is kept, are those of the function that was computed.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+
+E4M3 = torch.float8_e4m3fn
+_TYPES = {torch.bfloat16: _lib.HSTU_DTYPE_BF16, torch.float32: _lib.HSTU_DTYPE_FP32}
+MAX_D = 32768
+
+
+def _rows2d(t: torch.Tensor) -> torch.Tensor:
+    """[rows, D] with unit column stride and disjoint rows (column slices of a wider buffer stay in place)."""
+    t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+
+
+def _ld(t: Optional[torch.Tensor]) -> int:
+    """Row stride; a single row may have any."""
+    return 0 if t is None else max(t.stride(0), t.shape[1])
+
+
+def _like(name: str, t: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
+    if t.shape != x.shape or t.dtype != x.dtype or t.device != x.device:
+        raise ValueError(f"{name} {tuple(t.shape)} {t.dtype} on {t.device} must match x {tuple(x.shape)} {x.dtype} "
+                         f"on {x.device}")
+    return _rows2d(t)
+
+
+def _weight(weight: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
+    if weight.dim() != 1 or weight.shape[0] != x.shape[-1] or weight.device != x.device:
+        raise ValueError(f"weight {tuple(weight.shape)} on {weight.device} must be [{x.shape[-1]}] on {x.device}")
+    if weight.dtype not in _TYPES:
+        raise NotImplementedError(f"weight: bf16 or fp32 (got {weight.dtype})")
+    return weight.contiguous()
+
+
+def _check(x: torch.Tensor) -> None:
+    if x.dtype not in _TYPES:
+        raise NotImplementedError(f"x: bf16 or fp32 (got {x.dtype})")
+    if x.dim() < 1 or not 0 < x.shape[-1] <= MAX_D:
+        raise NotImplementedError(f"x {tuple(x.shape)}: a last dimension of 1 .. {MAX_D}")
+    if not x.is_cuda:
+        raise NotImplementedError("x: device tensors only")
+
+
+def rms_norm_fwd(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None,
+                 output_fp8: bool = False, scale: Optional[torch.Tensor] = None, want_rstd: bool = True
+                 ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """(y, h, rstd, y_scale).  ``h`` is ``x`` itself without a residual; ``rstd``
+    fp32 [rows]; ``output_fp8``: y e4m3 and ``y_scale`` the fp32 scales of the
+    rows, or ``scale`` (one fp32 value on the device) where it is given."""
+    _check(x)
+    w = _weight(weight.detach(), x)
+    D = x.shape[-1]
+    x2 = _rows2d(x.detach())
+    rows = x2.shape[0]
+    r2 = None if residual is None else _like("residual", residual.detach(), x)
+    h2 = None if residual is None else torch.empty((rows, D), dtype=x.dtype, device=x.device)
+    y = torch.empty((rows, D), dtype=E4M3 if output_fp8 else x.dtype, device=x.device)
+    rstd = torch.empty((rows,), dtype=torch.float32, device=x.device) if want_rstd else None
+    given = y_scale = None
+    if output_fp8:
+        if scale is None:
+            y_scale = torch.empty((rows,), dtype=torch.float32, device=x.device)
+        else:
+            if scale.numel() != 1 or scale.device != x.device:
+                raise ValueError("scale must be one value on x's device")
+            given = scale.detach().to(torch.float32).reshape(1)
+    elif scale is not None:
+        raise ValueError("scale goes with output_fp8")
+    if rows > 0:
+        with _lib.on_device(x):
+            st = _lib.fn("hstu_rms_norm_fwd")(
+                _TYPES[x.dtype], x2.data_ptr(), _ld(x2), _lib.ptr(r2), _ld(r2), w.data_ptr(), _TYPES[w.dtype],
+                float(eps), rows, D, _lib.ptr(h2), D, y.data_ptr(), D,
+                _lib.HSTU_DTYPE_FP8_E4M3 if output_fp8 else _TYPES[x.dtype], _lib.ptr(given), _lib.ptr(y_scale),
+                _lib.ptr(rstd), _lib.stream(x))
+        _lib.check(st, "hstu_rms_norm_fwd")
+    h = x if residual is None else h2.view(x.shape)
+    return y.view(x.shape), h, rstd, given if given is not None else y_scale
+
+
+def rms_norm_bwd(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor,
+                 dh: Optional[torch.Tensor] = None, dweight_dtype: Optional[torch.dtype] = None
+                 ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(dx, dweight): dx is the gradient of x and of the residual; ``dh`` the
+    gradient of the returned h.  dweight in ``dweight_dtype`` (the weight's)."""
+    _check(h)
+    w = _weight(weight.detach(), h)
+    D = h.shape[-1]
+    dt = w.dtype if dweight_dtype is None else dweight_dtype
+    if dt not in _TYPES:
+        raise NotImplementedError(f"dweight: bf16 or fp32 (got {dt})")
+    h2, dy2 = _rows2d(h.detach()), _like("dy", dy.detach(), h)
+    d2 = None if dh is None else _like("dh", dh.detach(), h)
+    rows = h2.shape[0]
+    if rstd.dtype != torch.float32 or rstd.numel() != rows or rstd.device != h.device:
+        raise ValueError(f"rstd must be fp32 [{rows}] on {h.device}")
+    dx = torch.empty((rows, D), dtype=h.dtype, device=h.device)
+    dw = torch.empty((D,), dtype=dt, device=h.device)
+    nbytes = int(_lib.fn("hstu_rms_norm_bwd_workspace_bytes")(rows, D))
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=h.device)
+    with _lib.on_device(h):
+        st = _lib.fn("hstu_rms_norm_bwd")(
+            _TYPES[h.dtype], dy2.data_ptr(), _ld(dy2), h2.data_ptr(), _ld(h2), _lib.ptr(d2), _ld(d2), w.data_ptr(),
+            _TYPES[w.dtype], rstd.contiguous().data_ptr(), rows, D, dx.data_ptr(), D, dw.data_ptr(), _TYPES[dt],
+            ws.data_ptr(), nbytes, _lib.stream(h))
+    _lib.check(st, "hstu_rms_norm_bwd")
+    return dx.view(h.shape), dw
+
+
+class RMSNormFunction(torch.autograd.Function):
+    """Autograd of the norm: (y, h) from (x, residual, weight).  A gradient
+    that nothing asks for is None and costs nothing."""
+
+    @staticmethod
+    def forward(ctx, x, weight, eps, residual):
+        ctx.set_materialize_grads(False)
+        y, h, rstd, _ = rms_norm_fwd(x, weight, eps, residual)
+        ctx.save_for_backward(h, weight, rstd)
+        ctx.has_residual = residual is not None
+        return (y, h) if residual is not None else y
+
+    @staticmethod
+    def backward(ctx, dy, dh=None):
+        h, weight, rstd = ctx.saved_tensors
+        if dy is None:  # only h was used
+            return dh, None, None, dh
+        dx, dw = rms_norm_bwd(dy, h, weight, rstd, dh)
+        return dx, dw if ctx.needs_input_grad[1] else None, None, dx if ctx.has_residual else None
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None):
+    """``y``, or ``(y, h)`` with a residual: h = x + residual is the new residual
+    stream and y its norm times ``weight``.  Differentiable in x, residual and
+    weight, through y and h."""
+    return RMSNormFunction.apply(x, weight, eps, residual)
+
+
+def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None,
+                 scale: Optional[torch.Tensor] = None):
+    """``(y8, scale)`` or, with a residual, ``(y8, scale, h)``: the norm in e4m3,
+    y = y8 * scale with one fp32 scale a row ([rows], max|y| / 448) or the given
+    one (returned as [1])."""
+    y8, h, _, s = rms_norm_fwd(x, weight, eps, residual, output_fp8=True, scale=scale, want_rstd=False)
+    return (y8, s) if residual is None else (y8, s, h)
