@@ -640,6 +640,64 @@ int hstu_rms_norm_bwd(int dtype, const void* dy, int64_t lddy, const void* h, in
                       int64_t lddx, void* dweight, int dweight_dtype, void* workspace, int64_t workspace_bytes,
                       hipStream_t stream);
 
+/*
+ * Gated feed-forward projection: g = x Wg^T, u = x Wu^T, h = a(g) u, both
+ * products and the activation in one kernel; x [M, D], w_gate and w_up [F, D]
+ * (the contraction index contiguous), h [M, F], all bf16, fp32 accumulation,
+ * rounded once; ld* in elements.  activation: 0 silu, 1 gelu (tanh form),
+ * 2 sigmoid.  D % 256 == 0, F % 128 == 0, any M; rows 16-byte aligned.  Rows
+ * past M are not touched.
+ * Replaces: two projections of ops/triton/triton_addmm.py:1756-1767 and an
+ *           elementwise pass over both (the reference's UVQK projection has SiLU
+ *           on a column range, ops/hstu_compute.py:140, but no product).
+ */
+int hstu_gated_fwd(const void* x, int64_t ldx, const void* w_gate, int64_t ldg, const void* w_up, int64_t ldu, int M,
+                   int F, int D, int activation, void* h, int64_t ldh, hipStream_t stream);
+/*
+ * The same from e4m3 x and weights (D % 128 == 0): g and u are multiplied by
+ * x_scale (mode 0: one fp32 on the device, 1: [M]) and by their weight's scale
+ * (mode 0: one, 1: [F]).  ld* of e4m3 operands in bytes.
+ */
+int hstu_gated_fwd_fp8(const void* x, int64_t ldx, const float* x_scale, int x_scale_mode, const void* w_gate,
+                       int64_t ldg, const float* gate_scale, int gate_scale_mode, const void* w_up, int64_t ldu,
+                       const float* up_scale, int up_scale_mode, int M, int F, int D, int activation, void* h,
+                       int64_t ldh, hipStream_t stream);
+/*
+ * The elementwise part of its backward: from dh [M, F] and g, u computed again
+ * in fp32, dgu [M, 2F] = [dh u a'(g) | dh a(g)] in bf16 -- the gradients of g and
+ * u, from which dx = dgu [Wg; Wu] (hstu_bf16_gemm) and [dWg; dWu] = dgu^T x
+ * (hstu_wgrad) follow.  dgu may not overlap the inputs.
+ */
+int hstu_gated_bwd(const void* dh, int64_t lddh, const void* x, int64_t ldx, const void* w_gate, int64_t ldg,
+                   const void* w_up, int64_t ldu, int M, int F, int D, int activation, void* dgu, int64_t lddgu,
+                   hipStream_t stream);
+
+/*
+ * Microscaled 4-bit floating point (OCP MX, e2m1 values with one E8M0 scale for
+ * 32 consecutive values of a row).  x [rows, cols] bf16 or fp32 (dtype; ldx in
+ * elements, any alignment of whole elements), cols % 32 == 0 -> codes
+ * [rows, cols / 2] (two a byte, the even column in the low half) and scales
+ * [rows, cols / 32] = E + 127, both contiguous: E = max(floor(log2 max|x|) - 2,
+ * -127), codes the nearest of x 2^-E (ties to even), at most 6.  A block of
+ * zeros has scale byte 0, one with an infinity or NaN 255 (NaN).
+ * The reference's microscaled format for its projections is a 6-bit one
+ * (ops/hip/k512_mx6_gemm.cu:1-45).
+ */
+int hstu_mxfp4_quantize(int dtype, const void* x, int64_t ldx, int64_t rows, int cols, void* codes, void* scales,
+                        hipStream_t stream);
+/* The values that contiguous codes and scales stand for, in bf16 (exact) or fp32. */
+int hstu_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, int cols, int out_dtype, void* out,
+                          int64_t ldo, hipStream_t stream);
+/*
+ * C[m][n] = sum_k A[m][k] W[n][k] [+ bias[n]] [+ residual[m][n]]: A [M, K] and W
+ * [N, K] in the format above (ld of codes and scales in bytes, codes' rows
+ * 16-byte and scales' rows 4-byte aligned), bias [N], residual and C bf16, fp32
+ * accumulation.  N % 16 == 0, K % 128 == 0, any M.
+ */
+int hstu_mxfp4_gemm(const void* A, int64_t lda, const void* a_scale, int64_t ldas, const void* W, int64_t ldw,
+                    const void* w_scale, int64_t ldws, const void* bias, const void* residual, int64_t ldr, void* C,
+                    int64_t ldc, int M, int N, int K, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -22,7 +22,8 @@ CSRC = PKG_ROOT / "csrc"
 OBJ_DIR = PKG_ROOT / "_build"
 OUT = PKG_ROOT / "hstu_amd" / "libhstu_mi355x.so"
 SOURCES = ["hstu_attention.hip", "hstu_fp8_gemm.hip", "hstu_layernorm.hip", "hstu_delta.hip", "hstu_do_fp8.hip",
-           "hstu_wgrad.hip", "hstu_rms_norm.hip"]
+           "hstu_wgrad.hip", "hstu_rms_norm.hip", "hstu_gated.hip",
+           "hstu_mxfp4.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

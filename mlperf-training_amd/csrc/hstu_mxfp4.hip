@@ -1,0 +1,258 @@
+// Microscaled 4-bit floating point (OCP MX: e2m1 values, one E8M0 scale for 32
+// consecutive values of a row): quantisation, its inverse, and the product of
+// two quantised matrices, for MI355X (gfx950).
+//
+//   E = max(floor(log2 max|v|) - 2, -127) of a block (2 is e2m1's largest
+//   exponent), scale byte E + 127; code = nearest e2m1 (0, .5, 1, 1.5, 2, 3, 4,
+//   6) of v 2^-E, ties to the even code, at most 6.  A block of zeros has byte 0,
+//   one with an infinity or NaN byte 255 and stands for NaN.  Codes lie two a
+//   byte, the even column in the low half.
+//   C[m][n] = sum_k A[m][k] W[n][k] [+ bias[n]] [+ residual[m][n]], A [M, K] and W
+//   [N, K] in this format: the matrix cores scale each block of the products'
+//   sum, which is kept in fp32.
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "hstu_common.h"
+#include "hstu_mi355x.h"
+
+namespace {
+using namespace hstu;
+
+__device__ __forceinline__ float bf16f(uint32_t b16) { return __builtin_bit_cast(float, b16 << 16); }
+
+// ---------------------------------------------------------------- quantisation
+// maximum over the four lanes of a quad
+__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true));  // quad_perm 1 0 3 2
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true));  // quad_perm 2 3 0 1
+}
+// Eight values (bits of fp32) of a lane, the block being those of its quad ->
+// codes and the scale byte.  Magnitudes compare as integers, NaN above infinity.
+__device__ __forceinline__ uint32_t mx_encode8(const float (&v)[8], uint32_t& byte) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top = max(top, __builtin_bit_cast(uint32_t, v[e]) & 0x7fffffffu);
+  const uint32_t ex = quad_max(top) >> 23;
+  byte = ex == 255u ? 255u : ex >= 2u ? ex - 2u : 0u;
+  const float up = ex == 255u ? 0.f : __builtin_bit_cast(float, (254u - byte) << 23);  // 2^-E
+  uint32_t w = 0;
+  float t[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) t[e] = ex == 255u ? 0.f : v[e] * up;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[0], t[1], 1.f, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[2], t[3], 1.f, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[4], t[5], 1.f, 2);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[6], t[7], 1.f, 3);
+  return w;
+}
+
+struct QuantArgs {
+  const uint8_t* x;
+  int64_t ldx;  // bytes
+  int64_t rows;
+  int chunks;  // chunks of 8 values in a row
+  uint8_t* codes;
+  uint8_t* scales;
+};
+
+// A lane takes 8 consecutive values; a quad is a block.  VEC: 16-byte aligned rows.
+template <bool F32, bool VEC>
+__global__ void __launch_bounds__(256) mx_quantize_kernel(QuantArgs a) {
+  const int64_t total = a.rows * a.chunks;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / a.chunks;
+    const int c = (int)(i - row * a.chunks);
+    const uint8_t* src = a.x + row * a.ldx + (int64_t)c * (F32 ? 32 : 16);
+    float v[8];
+    if constexpr (VEC && F32) {
+      const f32x4 p = *(const f32x4*)src, q = *(const f32x4*)(src + 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = p[e], v[4 + e] = q[e];
+    } else if constexpr (VEC) {
+      const u32x4 p = *(const u32x4*)src;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[2 * e] = bf16f(p[e] & 0xffffu), v[2 * e + 1] = bf16f(p[e] >> 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = F32 ? ((const float*)src)[e] : bf16f(((const uint16_t*)src)[e]);
+    }
+    uint32_t byte;
+    const uint32_t w = mx_encode8(v, byte);
+    ((uint32_t*)a.codes)[i] = w;
+    if ((i & 3) == 0) a.scales[i >> 2] = (uint8_t)byte;
+  }
+}
+
+// 2^(byte - 127); NaN for 255
+__device__ __forceinline__ float mx_unit(uint32_t byte) {
+  return __builtin_bit_cast(float, byte == 255u ? 0x7fc00000u : byte == 0u ? 0x00400000u : byte << 23);
+}
+template <bool F32>
+__global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint32_t* __restrict__ codes,
+                                                            const uint8_t* __restrict__ scales, int64_t total,
+                                                            int chunks, uint8_t* out, int64_t ldo) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / chunks;
+    const int c = (int)(i - row * chunks);
+    const uint32_t w = codes[i];
+    const float s = mx_unit(scales[i >> 2]);
+    const f32x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 0), p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 1);
+    const f32x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 2), p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 3);
+    const float v[8] = {p0[0] * s, p0[1] * s, p1[0] * s, p1[1] * s, p2[0] * s, p2[1] * s, p3[0] * s, p3[1] * s};
+    uint8_t* dst = out + row * ldo + (int64_t)c * (F32 ? 32 : 16);
+    if constexpr (F32) {
+      *(f32x4*)dst = f32x4{v[0], v[1], v[2], v[3]};
+      *(f32x4*)(dst + 16) = f32x4{v[4], v[5], v[6], v[7]};
+    } else {
+      *(u32x4*)dst = u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
+    }
+  }
+}
+
+// ---------------------------------------------------------------- product
+struct MxParams {
+  const uint8_t* A;
+  const uint8_t* W;
+  const uint8_t* as;
+  const uint8_t* ws;
+  int64_t lda, ldw, ldas, ldws;  // bytes
+  const uint16_t* bias;          // bf16 [N] or null
+  const uint16_t* resid;         // bf16 or null
+  uint16_t* C;
+  int64_t ldr, ldc;  // elements
+  int M, N, K;
+};
+
+// e2m1 x e2m1 (16x16x128) with E8M0 scales: lane (li, q) holds values 32 q .. 32 q
+// + 31 of row li of each operand and, in byte 0 of its scale register, the
+// scale of that block.
+__device__ __forceinline__ f32x4 mfma_mx4(u32x4 a, u32x4 b, f32x4 c, int sa, int sb) {
+  const u32x4 z = {0u, 0u, 0u, 0u};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(cat8(a, z), cat8(b, z), c, 4, 4, 0, sa, 0, sb);
+}
+
+// Four consecutive outputs of row m from column n on.
+__device__ __forceinline__ void mx_store4(const MxParams& p, int m, int n, f32x4 v) {
+  if (p.bias) {
+    const u32x2 b = *(const u32x2*)(p.bias + n);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += bf16f(e & 1 ? b[e >> 1] >> 16 : b[e >> 1] & 0xffffu);
+  }
+  if (p.resid) {
+    const u32x2 r = *(const u32x2*)(p.resid + (int64_t)m * p.ldr + n);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += bf16f(e & 1 ? r[e >> 1] >> 16 : r[e >> 1] & 0xffffu);
+  }
+  *(u32x2*)(p.C + (int64_t)m * p.ldc + n) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+}
+
+// Row form: 16 columns and 16 MB rows a workgroup, its four waves split the
+// contraction and meet in LDS in wave order.
+template <int MB>
+__global__ void __launch_bounds__(kThreads) mx_rows_kernel(MxParams p) {
+  __shared__ f32x4 part[3][MB][64];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, li = lane & 15, q = lane >> 4;
+  const int nt = p.N / 16, mt = blockIdx.x / nt, n0 = (blockIdx.x - mt * nt) * 16, m0 = mt * 16 * MB;
+  const uint8_t* wp = p.W + (int64_t)(n0 + li) * p.ldw + 16 * q;
+  const uint8_t* wsp = p.ws + (int64_t)(n0 + li) * p.ldws + q;
+  const uint8_t* ap[MB];
+  const uint8_t* asp[MB];
+#pragma unroll
+  for (int b = 0; b < MB; ++b) {
+    const int m = min(m0 + 16 * b + li, p.M - 1);
+    ap[b] = p.A + (int64_t)m * p.lda + 16 * q;
+    asp[b] = p.as + (int64_t)m * p.ldas + q;
+  }
+  f32x4 acc[MB];
+#pragma unroll
+  for (int b = 0; b < MB; ++b) acc[b] = zero4();
+  const int steps = p.K / 128;
+#pragma unroll 4
+  for (int s = wave; s < steps; s += 4) {
+    const u32x4 w = *(const u32x4*)(wp + 64 * s);
+    const int ws = wsp[4 * s];
+#pragma unroll
+    for (int b = 0; b < MB; ++b) acc[b] = mfma_mx4(w, *(const u32x4*)(ap[b] + 64 * s), acc[b], ws, asp[b][4 * s]);
+  }
+  if (wave > 0) {
+#pragma unroll
+    for (int b = 0; b < MB; ++b) part[wave - 1][b][lane] = acc[b];
+  }
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int b = 0; b < MB; ++b) {
+#pragma unroll
+    for (int w = 0; w < 3; ++w) acc[b] += part[w][b][lane];
+    const int m = m0 + 16 * b + li;
+    if (m < p.M) mx_store4(p, m, n0 + 4 * q, acc[b]);
+  }
+}
+
+}  // namespace
+
+extern "C" int hstu_mxfp4_quantize(int dtype, const void* x, int64_t ldx, int64_t rows, int cols, void* codes,
+                                   void* scales, hipStream_t stream) {
+  const bool f32 = dtype == HSTU_DTYPE_FP32;
+  if ((!f32 && dtype != HSTU_DTYPE_BF16) || rows < 0 || cols <= 0 || ldx < cols) return HSTU_E_BAD_ARG;
+  if (rows > 0 && (!x || !codes || !scales)) return HSTU_E_BAD_ARG;
+  const int es = f32 ? 4 : 2;
+  if (cols % 32 || (uintptr_t)x % es || (uintptr_t)codes % 4) return HSTU_E_UNSUPPORTED;
+  if (rows == 0) return 0;
+  QuantArgs a{(const uint8_t*)x, ldx * es, rows, cols / 8, (uint8_t*)codes, (uint8_t*)scales};
+  const bool vec = (uintptr_t)x % 16 == 0 && a.ldx % 16 == 0;
+  const dim3 grid((unsigned)std::min<int64_t>((rows * a.chunks + 255) / 256, 4096)), block(256);
+  if (f32 && vec) hipLaunchKernelGGL((mx_quantize_kernel<true, true>), grid, block, 0, stream, a);
+  else if (f32) hipLaunchKernelGGL((mx_quantize_kernel<true, false>), grid, block, 0, stream, a);
+  else if (vec) hipLaunchKernelGGL((mx_quantize_kernel<false, true>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((mx_quantize_kernel<false, false>), grid, block, 0, stream, a);
+  return (int)hipGetLastError();
+}
+
+extern "C" int hstu_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, int cols, int out_dtype,
+                                     void* out, int64_t ldo, hipStream_t stream) {
+  const bool f32 = out_dtype == HSTU_DTYPE_FP32;
+  if ((!f32 && out_dtype != HSTU_DTYPE_BF16) || rows < 0 || cols <= 0 || ldo < cols) return HSTU_E_BAD_ARG;
+  if (rows > 0 && (!codes || !scales || !out)) return HSTU_E_BAD_ARG;
+  const int es = f32 ? 4 : 2;
+  if (cols % 32 || (uintptr_t)codes % 4 || (uintptr_t)out % 16 || (ldo * es) % 16) return HSTU_E_UNSUPPORTED;
+  if (rows == 0) return 0;
+  const int64_t total = rows * (cols / 8);
+  const dim3 grid((unsigned)std::min<int64_t>((total + 255) / 256, 4096)), block(256);
+  if (f32)
+    hipLaunchKernelGGL((mx_dequantize_kernel<true>), grid, block, 0, stream, (const uint32_t*)codes,
+                       (const uint8_t*)scales, total, cols / 8, (uint8_t*)out, ldo * es);
+  else
+    hipLaunchKernelGGL((mx_dequantize_kernel<false>), grid, block, 0, stream, (const uint32_t*)codes,
+                       (const uint8_t*)scales, total, cols / 8, (uint8_t*)out, ldo * es);
+  return (int)hipGetLastError();
+}
+
+extern "C" int hstu_mxfp4_gemm(const void* A, int64_t lda, const void* a_scale, int64_t ldas, const void* W,
+                               int64_t ldw, const void* w_scale, int64_t ldws, const void* bias, const void* residual,
+                               int64_t ldr, void* C, int64_t ldc, int M, int N, int K, hipStream_t stream) {
+  if (M < 0 || N <= 0 || K <= 0 || lda < K / 2 || ldw < K / 2 || ldas < K / 32 || ldws < K / 32 || ldc < N ||
+      (residual && ldr < N))
+    return HSTU_E_BAD_ARG;
+  if (M > 0 && (!A || !a_scale || !W || !w_scale || !C)) return HSTU_E_BAD_ARG;
+  if (N % 16 || K % 128) return HSTU_E_UNSUPPORTED;
+  if (((uintptr_t)A | (uintptr_t)W | (uintptr_t)C | (uintptr_t)residual) % 16 || (lda | ldw) % 16 ||
+      ((uintptr_t)a_scale | (uintptr_t)w_scale) % 4 || (ldas | ldws) % 4 || ldc % 8 || (residual && ldr % 8) ||
+      (uintptr_t)bias % 16)
+    return HSTU_E_UNSUPPORTED;
+  if (M == 0) return 0;
+  MxParams p{(const uint8_t*)A, (const uint8_t*)W, (const uint8_t*)a_scale, (const uint8_t*)w_scale, lda, ldw, ldas,
+             ldws, (const uint16_t*)bias, (const uint16_t*)residual, (uint16_t*)C, ldr, ldc, M, N, K};
+  const int mb = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+  const int64_t tiles = ((int64_t)M + 16 * mb - 1) / (16 * mb) * (N / 16);
+  if (tiles >= ((int64_t)1 << 31)) return HSTU_E_UNSUPPORTED;
+  const dim3 grid((unsigned)tiles);
+  if (mb == 1) hipLaunchKernelGGL((mx_rows_kernel<1>), grid, dim3(kThreads), 0, stream, p);
+  else if (mb == 2) hipLaunchKernelGGL((mx_rows_kernel<2>), grid, dim3(kThreads), 0, stream, p);
+  else hipLaunchKernelGGL((mx_rows_kernel<4>), grid, dim3(kThreads), 0, stream, p);
+  return (int)hipGetLastError();
+}

@@ -34,4 +34,6 @@ from .hstu_preprocess import (  # noqa: F401
 from .hstu_delta import delta_hstu_mha, triton_cached_hstu_mha, triton_hstu_attention_delta_bwd  # noqa: F401
 from .hstu_do_fp8 import dequantize_do_e4m3_blk, quantize_do_e4m3_blk  # noqa: F401
 from .hstu_rms_norm import RMSNormFunction, rms_norm, rms_norm_bwd, rms_norm_fp8, rms_norm_fwd  # noqa: F401
+from .hstu_gated import GatedLinearFunction, gated_linear, gated_linear_bwd, gated_linear_fp8, gated_linear_fwd  # noqa: F401
+from .mxfp4 import dequantize_mxfp4, mxfp4_linear, mxfp4_mm, quantize_mxfp4  # noqa: F401
 from . import reference_ops  # noqa: F401,E402  (registers generative_recommenders::triton_hstu_attention_*)

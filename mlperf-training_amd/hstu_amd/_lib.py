@@ -70,6 +70,12 @@ EXPORTED_SYMBOLS = (
     "hstu_rms_norm_fwd",
     "hstu_rms_norm_bwd_workspace_bytes",
     "hstu_rms_norm_bwd",
+    "hstu_gated_fwd",
+    "hstu_gated_fwd_fp8",
+    "hstu_gated_bwd",
+    "hstu_mxfp4_quantize",
+    "hstu_mxfp4_dequantize",
+    "hstu_mxfp4_gemm",
 )
 
 
@@ -190,6 +196,18 @@ _SIGNATURES = {
     "hstu_rms_norm_bwd": (
         _i32,
         [_i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _vp, _i64, _i32, _vp, _i64, _vp, _i32, _vp, _i64, _vp],
+    ),
+    "hstu_gated_fwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp]),
+    "hstu_gated_fwd_fp8": (
+        _i32,
+        [_vp, _i64, _vp, _i32, _vp, _i64, _vp, _i32, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _vp],
+    ),
+    "hstu_gated_bwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp]),
+    "hstu_mxfp4_quantize": (_i32, [_i32, _vp, _i64, _i64, _i32, _vp, _vp, _vp]),
+    "hstu_mxfp4_dequantize": (_i32, [_vp, _vp, _i64, _i32, _i32, _vp, _i64, _vp]),
+    "hstu_mxfp4_gemm": (
+        _i32,
+        [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _vp],
     ),
 }
 

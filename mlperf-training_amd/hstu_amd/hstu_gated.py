@@ -1,0 +1,176 @@
+"""Gated feed-forward projection (``csrc/hstu_gated.hip``):
+
+    g = x @ w_gate^T,  u = x @ w_up^T,  h = a(g) * u
+
+with a = silu, gelu (the tanh form) or sigmoid; both products and the
+activation are one kernel, and h is the only [.., F] tensor written.  Weights
+are [F, D] with the contraction index contiguous, as ``fp8.bf16_gemm`` takes
+them.  The UVQK projection (``hstu_compute_uqvk``) has SiLU on a column range
+of one product, not the product of two.
+
+* ``gated_linear``: differentiable, bf16, D a multiple of 256 and F of 128;
+* ``gated_linear_fp8``: forward from e4m3 (``rms_norm_fp8``'s or
+  ``fp8.quantize_e4m3_rows``' output), D a multiple of 128;
+* ``gated_linear_fwd`` / ``gated_linear_bwd``: the two directions.
+
+The backward keeps x and the weights only: it computes g and u again, in fp32,
+and writes [dg | du], whose products with the weights and with x are the bf16
+projection GEMM and the token-axis weight gradient.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from .fp8 import bf16_gemm
+from .wgrad import wgrad
+
+ACTIVATIONS = {"silu": 0, "gelu": 1, "sigmoid": 2}
+E4M3 = torch.float8_e4m3fn
+Scaled = Tuple[torch.Tensor, torch.Tensor]
+
+
+def _act(activation: str) -> int:
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation {activation!r} (one of {sorted(ACTIVATIONS)})")
+    return ACTIVATIONS[activation]
+
+
+def _rows2d(t: torch.Tensor) -> torch.Tensor:
+    """[rows, width] with unit column stride and 16-byte aligned rows."""
+    t = t.reshape(-1, t.shape[-1])
+    ok = (t.stride(1) == 1 and t.data_ptr() % 16 == 0
+          and (t.shape[0] <= 1 or (t.stride(0) >= t.shape[1] and t.stride(0) * t.element_size() % 16 == 0)))
+    if ok:
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _check(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, dtype: torch.dtype, multiple: int) -> None:
+    for name, t in (("x", x), ("w_gate", w_gate), ("w_up", w_up)):
+        if t.dtype != dtype:
+            raise NotImplementedError(f"{name}: {dtype} (got {t.dtype})")
+        if t.device != x.device or not t.is_cuda:
+            raise NotImplementedError(f"{name}: on one device (got {t.device}, x on {x.device})")
+    if x.dim() < 1 or w_gate.dim() != 2 or w_up.shape != w_gate.shape or w_gate.shape[1] != x.shape[-1]:
+        raise ValueError(f"x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)}: expected "
+                         "[.., D], [F, D], [F, D]")
+    F, D = w_gate.shape
+    if D == 0 or F == 0 or D % multiple or F % 128:
+        raise NotImplementedError(f"D = {D}, F = {F}: D a multiple of {multiple} and F of 128")
+    if x.numel() // D >= 2 ** 31 - 256:
+        raise NotImplementedError("x: fewer than 2^31 rows")
+
+
+def gated_linear_fwd(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = "silu"
+                     ) -> torch.Tensor:
+    """h [.., F] in bf16."""
+    act = _act(activation)
+    x, w_gate, w_up = x.detach(), w_gate.detach(), w_up.detach()
+    _check(x, w_gate, w_up, torch.bfloat16, 256)
+    F, D = w_gate.shape
+    x2, g, u = _rows2d(x), _rows2d(w_gate), _rows2d(w_up)
+    M = x2.shape[0]
+    h = torch.empty((M, F), dtype=torch.bfloat16, device=x.device)
+    if M > 0:
+        with _lib.on_device(x):
+            st = _lib.fn("hstu_gated_fwd")(x2.data_ptr(), _ld(x2), g.data_ptr(), _ld(g), u.data_ptr(), _ld(u), M, F, D,
+                                           act, h.data_ptr(), F, _lib.stream(x))
+        _lib.check(st, "hstu_gated_fwd")
+    return h.view(x.shape[:-1] + (F,))
+
+
+def gated_linear_bwd(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
+                     activation: str = "silu", need_dx: bool = True, need_dw: bool = True
+                     ) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """(dx, dw_gate, dw_up) in bf16; None for what is not needed."""
+    act = _act(activation)
+    dh, x, w_gate, w_up = dh.detach(), x.detach(), w_gate.detach(), w_up.detach()
+    _check(x, w_gate, w_up, torch.bfloat16, 256)
+    F, D = w_gate.shape
+    if dh.shape != x.shape[:-1] + (F,) or dh.dtype != torch.bfloat16 or dh.device != x.device:
+        raise ValueError(f"dh {tuple(dh.shape)} {dh.dtype}; expected {tuple(x.shape[:-1] + (F,))} bf16 on {x.device}")
+    x2, g, u, d2 = _rows2d(x), _rows2d(w_gate), _rows2d(w_up), _rows2d(dh)
+    M = x2.shape[0]
+    if M == 0:
+        dw = torch.zeros((2 * F, D), dtype=torch.bfloat16, device=x.device)
+        return torch.empty_like(x) if need_dx else None, dw[:F] if need_dw else None, dw[F:] if need_dw else None
+    dgu = torch.empty((M, 2 * F), dtype=torch.bfloat16, device=x.device)
+    with _lib.on_device(x):
+        st = _lib.fn("hstu_gated_bwd")(d2.data_ptr(), _ld(d2), x2.data_ptr(), _ld(x2), g.data_ptr(), _ld(g),
+                                       u.data_ptr(), _ld(u), M, F, D, act, dgu.data_ptr(), 2 * F, _lib.stream(x))
+        _lib.check(st, "hstu_gated_bwd")
+        dx = dg = du = None
+        if need_dx:  # the contraction runs over both halves of dgu: the weights side by side, transposed
+            dx = bf16_gemm(dgu, torch.cat((g, u)).t().contiguous()).view(x.shape)
+        if need_dw:
+            dw = wgrad(dgu, x2, split=_wgrad_split(M, 2 * F, D))
+            dg, du = dw[:F], dw[F:]
+    return dx, dg, du
+
+
+def _wgrad_split(T: int, n1: int, n2: int) -> Optional[int]:
+    """Token ranges for the weight gradient: the kernel's own choice, more where
+    a range's rows would pass its 32-bit offsets."""
+    most = (2 ** 31) // (2 * max(n1, n2)) - 256
+    return None if T <= most else -(-T // most)
+
+
+class GatedLinearFunction(torch.autograd.Function):
+    """Autograd of the gated projection: keeps x and the weights, not g, u or h."""
+
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, activation):
+        ctx.save_for_backward(x, w_gate, w_up)
+        ctx.activation = activation
+        return gated_linear_fwd(x, w_gate, w_up, activation)
+
+    @staticmethod
+    def backward(ctx, dh):
+        x, w_gate, w_up = ctx.saved_tensors
+        need_x, need_g, need_u, _ = ctx.needs_input_grad
+        dx, dg, du = gated_linear_bwd(dh, x, w_gate, w_up, ctx.activation, need_x, need_g or need_u)
+        return dx, dg if need_g else None, du if need_u else None, None
+
+
+def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = "silu") -> torch.Tensor:
+    """a(x @ w_gate^T) * (x @ w_up^T): x [.., D], weights [F, D], h [.., F], bf16.
+    Differentiable in x and both weights."""
+    return GatedLinearFunction.apply(x, w_gate, w_up, activation)
+
+
+def _scale(name: str, s: torch.Tensor, n: int, x: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    if s.device != x.device or s.numel() not in (1, n):
+        raise ValueError(f"{name}: 1 or {n} values on {x.device} (got {tuple(s.shape)} on {s.device})")
+    return s.detach().to(torch.float32).reshape(-1).contiguous(), 1 if s.numel() > 1 else 0
+
+
+def gated_linear_fp8(x8: torch.Tensor, x_scale: torch.Tensor, gate: Scaled, up: Scaled, activation: str = "silu"
+                     ) -> torch.Tensor:
+    """The forward from e4m3: x8 [.., D] with one fp32 scale or one a row, and
+    ``gate``, ``up`` as pairs (e4m3 [F, D], scale: one or [F]).  h [.., F] in bf16."""
+    act = _act(activation)
+    (g8, gs), (u8, us) = gate, up
+    _check(x8, g8, u8, E4M3, 128)
+    F, D = g8.shape
+    x2, g2, u2 = _rows2d(x8), _rows2d(g8), _rows2d(u8)
+    M = x2.shape[0]
+    xs, xm = _scale("x_scale", x_scale, M, x8)
+    gs, gm = _scale("gate scale", gs, F, x8)
+    us, um = _scale("up scale", us, F, x8)
+    h = torch.empty((M, F), dtype=torch.bfloat16, device=x8.device)
+    if M > 0:
+        with _lib.on_device(x8):
+            st = _lib.fn("hstu_gated_fwd_fp8")(
+                x2.data_ptr(), _ld(x2), xs.data_ptr(), xm, g2.data_ptr(), _ld(g2), gs.data_ptr(), gm, u2.data_ptr(),
+                _ld(u2), us.data_ptr(), um, M, F, D, act, h.data_ptr(), F, _lib.stream(x8))
+        _lib.check(st, "hstu_gated_fwd_fp8")
+    return h.view(x8.shape[:-1] + (F,))

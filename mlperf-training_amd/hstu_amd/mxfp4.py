@@ -1,0 +1,150 @@
+"""Microscaled 4-bit floating point (OCP MX: e2m1 values with one E8M0 scale
+for 32 consecutive values of a row) on the kernels of ``csrc/hstu_mxfp4.hip``.
+It stands beside the e4m3 quantizers and GEMMs (``fp8``); the reference's
+microscaled format for its projections is a 6-bit one
+(``ops/hip/k512_mx6_gemm.cu:1-45``).
+
+A quantized matrix is a pair ``(codes, scales)``: uint8 [R, C / 2], two values a
+byte, the even column in the low half, and uint8 [R, C / 32], E + 127 with
+E = max(floor(log2 max|v|) - 2, -127) of the block.  A value is the nearest of
+0, 0.5, 1, 1.5, 2, 3, 4, 6 times 2^E (ties to the even code, larger ones 6); a
+block with an infinity or NaN stands for NaN (scale byte 255).
+
+* ``quantize_mxfp4`` / ``dequantize_mxfp4``;
+* ``mxfp4_mm(a, w)``: the product of two quantized matrices;
+* ``mxfp4_linear(x, w)``: bf16 activations, quantized on the way.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+
+_TYPES = {torch.bfloat16: _lib.HSTU_DTYPE_BF16, torch.float32: _lib.HSTU_DTYPE_FP32}
+Packed = Tuple[torch.Tensor, torch.Tensor]
+
+
+def quantize_mxfp4(x: torch.Tensor) -> Packed:
+    """(codes [.., C / 2], scales [.., C / 32]) of bf16 or fp32 x [.., C], C a multiple of 32."""
+    if x.dtype not in _TYPES:
+        raise NotImplementedError(f"x: bf16 or fp32 (got {x.dtype})")
+    if x.dim() < 1 or x.shape[-1] == 0 or x.shape[-1] % 32:
+        raise NotImplementedError(f"x {tuple(x.shape)}: a last dimension that is a multiple of 32")
+    if not x.is_cuda:
+        raise NotImplementedError("x: device tensors only")
+    C = x.shape[-1]
+    x2 = x.detach().reshape(-1, C)
+    if x2.stride(1) != 1 or (x2.shape[0] > 1 and x2.stride(0) < C):
+        x2 = x2.contiguous()
+    R = x2.shape[0]
+    codes = torch.empty((R, C // 2), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((R, C // 32), dtype=torch.uint8, device=x.device)
+    if R > 0:
+        with _lib.on_device(x):
+            st = _lib.fn("hstu_mxfp4_quantize")(_TYPES[x.dtype], x2.data_ptr(), x2.stride(0) if R > 1 else C, R, C,
+                                                codes.data_ptr(), scales.data_ptr(), _lib.stream(x))
+        _lib.check(st, "hstu_mxfp4_quantize")
+    return codes.view(x.shape[:-1] + (C // 2,)), scales.view(x.shape[:-1] + (C // 32,))
+
+
+def _pair(name: str, codes: torch.Tensor, scales: torch.Tensor) -> None:
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise ValueError(f"{name}: uint8 codes and scales (got {codes.dtype}, {scales.dtype})")
+    if codes.device != scales.device or not codes.is_cuda:
+        raise NotImplementedError(f"{name}: codes and scales on one device")
+    if (codes.dim() < 1 or codes.shape[:-1] != scales.shape[:-1] or codes.shape[-1] != 16 * scales.shape[-1]
+            or codes.shape[-1] == 0):
+        raise ValueError(f"{name}: codes {tuple(codes.shape)} and scales {tuple(scales.shape)}; expected [.., C / 2] "
+                         "and [.., C / 32]")
+
+
+def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values [.., C] that the pair stands for, in bf16 (exact) or fp32."""
+    if dtype not in _TYPES:
+        raise NotImplementedError(f"dtype: bf16 or fp32 (got {dtype})")
+    _pair("dequantize_mxfp4", codes, scales)
+    lead, C = codes.shape[:-1], 2 * codes.shape[-1]
+    c2, s2 = codes.reshape(-1, C // 2).contiguous(), scales.reshape(-1, C // 32).contiguous()
+    c2 = c2 if c2.data_ptr() % 4 == 0 else c2.clone()
+    R = c2.shape[0]
+    out = torch.empty((R, C), dtype=dtype, device=codes.device)
+    if R > 0:
+        with _lib.on_device(codes):
+            st = _lib.fn("hstu_mxfp4_dequantize")(c2.data_ptr(), s2.data_ptr(), R, C, _TYPES[dtype], out.data_ptr(), C,
+                                                  _lib.stream(codes))
+        _lib.check(st, "hstu_mxfp4_dequantize")
+    return out.view(lead + (C,))
+
+
+def _aligned(t: torch.Tensor, n: int) -> torch.Tensor:
+    """A 2-D operand with unit column stride and rows at multiples of n bytes."""
+    if (t.stride(1) == 1 and t.data_ptr() % n == 0
+            and (t.shape[0] <= 1 or (t.stride(0) >= t.shape[1] and t.stride(0) * t.element_size() % n == 0))):
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % n == 0 else t.clone()
+
+
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _epilogue(bias: Optional[torch.Tensor], residual: Optional[torch.Tensor], shape, device):
+    if bias is not None:
+        if bias.shape != shape[-1:] or bias.device != device:
+            raise ValueError(f"bias {tuple(bias.shape)} on {bias.device}; expected [{shape[-1]}] on {device}")
+        bias = bias.detach().to(torch.bfloat16).contiguous()
+        bias = bias if bias.data_ptr() % 16 == 0 else bias.clone()
+    if residual is not None:
+        if residual.shape != shape or residual.device != device or residual.dtype != torch.bfloat16:
+            raise ValueError(f"residual {tuple(residual.shape)} {residual.dtype} on {residual.device}; expected "
+                             f"{tuple(shape)} bf16 on {device}")
+        residual = _aligned(residual.detach().reshape(-1, shape[-1]), 16)
+    return bias, residual
+
+
+def _weight(weight: Packed) -> Tuple[torch.Tensor, torch.Tensor, int, int]:
+    wc, ws = weight
+    _pair("weight", wc, ws)
+    if wc.dim() != 2:
+        raise ValueError(f"weight codes {tuple(wc.shape)}; expected [N, K / 2]")
+    N, K = wc.shape[0], 2 * wc.shape[1]
+    if N == 0 or N % 16 or K % 128:
+        raise NotImplementedError(f"weight [{N}, {K}]: N a multiple of 16 and K of 128")
+    return _aligned(wc, 16), _aligned(ws, 4), N, K
+
+
+def mxfp4_mm(a: Packed, weight: Packed, bias: Optional[torch.Tensor] = None,
+             residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """a @ weight^T (+ bias [N]) (+ residual [.., N]) in bf16, fp32 accumulation:
+    a a pair of [.., K], weight a pair of [N, K]; N a multiple of 16, K of 128."""
+    wc, ws, N, K = _weight(weight)
+    ac, as_ = a
+    _pair("a", ac, as_)
+    if ac.shape[-1] != K // 2 or ac.device != wc.device:
+        raise ValueError(f"a codes {tuple(ac.shape)} on {ac.device} against weight [{N}, {K}] on {wc.device}")
+    shape = ac.shape[:-1] + (N,)
+    bias, r2 = _epilogue(bias, residual, shape, wc.device)
+    a2, s2 = _aligned(ac.reshape(-1, K // 2), 16), _aligned(as_.reshape(-1, K // 32), 4)
+    M = a2.shape[0]
+    if M >= 2 ** 31 - 256:
+        raise NotImplementedError("a: fewer than 2^31 rows")
+    out = torch.empty((M, N), dtype=torch.bfloat16, device=wc.device)
+    if M > 0:
+        with _lib.on_device(wc):
+            st = _lib.fn("hstu_mxfp4_gemm")(
+                a2.data_ptr(), _ld(a2), s2.data_ptr(), _ld(s2), wc.data_ptr(), _ld(wc), ws.data_ptr(), _ld(ws),
+                _lib.ptr(bias), _lib.ptr(r2), 0 if r2 is None else _ld(r2), out.data_ptr(), N, M, N, K, _lib.stream(wc))
+        _lib.check(st, "hstu_mxfp4_gemm")
+    return out.view(shape)
+
+
+def mxfp4_linear(x: torch.Tensor, weight: Packed, bias: Optional[torch.Tensor] = None,
+                 residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """quantize(x) @ weight^T (+ bias) (+ residual) in bf16, for bf16 x [.., K]."""
+    if x.dtype != torch.bfloat16:
+        raise NotImplementedError(f"x: bf16 (got {x.dtype})")
+    return mxfp4_mm(quantize_mxfp4(x), weight, bias, residual)

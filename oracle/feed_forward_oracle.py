@@ -70,6 +70,11 @@ def gated_bwd_ref(dh, x, w_gate, w_up, name):
 E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
 
+def _pow2(e: torch.Tensor) -> torch.Tensor:
+    """2^e in float64 from its bits (a device's pow and ldexp may be an ulp off)."""
+    return ((e.long() + 1023) << 52).view(F64)
+
+
 def mxfp4_quantize_ref(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """(values the rows stand for, float64 [R, C]; scale bytes int64 [R, C / 32]).
     E = max(floor(log2 max|x|) - 2, -127); nearest of E2M1 * 2^E, ties to the
@@ -80,13 +85,13 @@ def mxfp4_quantize_ref(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     amax = torch.where(finite, b.abs().amax(-1), 1.0)
     E = (torch.frexp(amax)[1] - 3).clamp(min=-127)  # frexp: amax = m 2^e, m in [1/2, 1)
     E = torch.where(amax > 0, E, -127)
-    t = torch.ldexp(b.abs(), -E[..., None]).clamp(max=6.0)
+    t = (b.abs() * _pow2(-E)[..., None]).clamp(max=6.0)
     grid = torch.tensor(E2M1, dtype=F64, device=x.device)
     mid = (grid[1:] + grid[:-1]) / 2
     up = torch.bucketize(t, mid)                       # t on a midpoint goes down ...
     tie = (t == mid[up.clamp(max=6)]) & (up % 2 == 1)  # ... unless the lower code is odd
     code = up + tie.to(up.dtype)
-    v = torch.copysign(grid[code], b) * torch.exp2(E.to(F64))[..., None]
+    v = torch.copysign(grid[code], b) * _pow2(E)[..., None]
     v = torch.where(finite[..., None], v, float("nan"))
     return v.reshape(R, C), torch.where(finite, E + 127, 255).long()
 
@@ -95,6 +100,6 @@ def mxfp4_decode_ref(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     """float64 values of packed codes [R, C / 2] (low nibble first) and scale bytes [R, C / 32]."""
     n = torch.stack((codes & 15, codes >> 4), -1).reshape(codes.shape[0], -1).long()
     grid = torch.tensor(E2M1 + tuple(-g for g in E2M1), dtype=F64, device=codes.device)
-    unit = torch.exp2(scales.to(F64) - 127)
+    unit = _pow2(scales.long() - 127)
     unit = torch.where(scales == 255, float("nan"), unit)
     return grid[n] * unit.repeat_interleave(32, 1)

@@ -1,0 +1,332 @@
+"""Gated feed-forward projection: the kernels against the float64 formulas
+(``oracle/feed_forward_oracle.py``), gradients, refusals, streams and graphs.
+
+Tolerances.  A sum of n products in the matrix cores is n additions, each off by
+at most 2^-23 of the sum of the magnitudes S (a unit: they need not round to
+nearest); scales and the activation add fewer than 16 such units, its argument's
+2^-24 |z| among them (|z| <= 88 where it matters: 2^-17 of a(g) u).  |a'| < 1.13 and
+|a''| < 1.  The one rounding of h, dg and du is 2^-8 of the value.  dx and dW sum dg
+and du as they are rounded: 2^-8 of the magnitudes that meet, the sum's own
+units and their own rounding.  Rounding errors are independent and spread over
+their range, so the 2-norm of two of them is under sqrt(2 / 3) 2^-8 of the result's
+where the terms are independent too: NORM = 2^-8."""
+
+import pytest
+import torch
+
+from oracle import feed_forward_oracle as orc
+
+DEV = "cuda"
+ACTS = ["silu", "gelu", "sigmoid"]
+ULP, HALF, NORM, ARG = 2.0 ** -23, 2.0 ** -8, 2.0 ** -8, 2.0 ** -17
+gpu = pytest.mark.gpu
+
+
+def rnd(shape, seed, std=1.0):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * std).to(torch.bfloat16)
+
+
+def weights(F, D, seed=0):
+    return rnd((F, D), 100 + seed, 1.5 * D ** -0.5).to(DEV), rnd((F, D), 200 + seed, D ** -0.5).to(DEV)
+
+
+def within(got, want, tol, what):
+    off = (got.double() - want).abs()
+    bad = ~(off <= tol)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {off[bad].max():.3e}"
+
+
+def h_bound(x, wg, wu, name):
+    """(h, what h may be off)."""
+    x, wg, wu = x.double(), wg.double(), wu.double()
+    g, u = x @ wg.t(), x @ wu.t()
+    sg, su = x.abs() @ wg.abs().t(), x.abs() @ wu.abs().t()
+    a, _ = orc.activation_ref(name, g)
+    h = a * u
+    n = (x.shape[-1] + 16) * ULP
+    return h, h.abs() * (HALF + ARG) + n * (1.13 * sg * u.abs() + a.abs() * su + 1.13 * n * sg * su)
+
+
+SHAPES = [(1, 256, 128), (3, 256, 128), (16, 512, 256), (17, 512, 384), (33, 256, 640), (64, 512, 128), (65, 768, 128),
+          (127, 512, 256), (129, 512, 256), (300, 1024, 384), (1027, 512, 2048), (2050, 256, 512), (4100, 512, 640)]
+
+
+@gpu
+@pytest.mark.parametrize("name", ACTS)
+@pytest.mark.parametrize("M,D,F", SHAPES)
+def test_forward(hip_lib, M, D, F, name):
+    import hstu_amd
+
+    x = rnd((M, D), 1).to(DEV)
+    wg, wu = weights(F, D)
+    h = hstu_amd.gated_linear(x, wg, wu, name)
+    assert h.shape == (M, F) and h.dtype == torch.bfloat16
+    want, tol = h_bound(x, wg, wu, name)
+    within(h, want, tol, "h")
+
+
+@gpu
+@pytest.mark.parametrize("name", ACTS)
+@pytest.mark.parametrize("M,D,F", SHAPES)
+def test_backward(hip_lib, M, D, F, name):
+    import hstu_amd
+
+    x, dh = rnd((M, D), 1).to(DEV).requires_grad_(True), rnd((M, F), 2, 0.5).to(DEV)
+    wg, wu = (w.requires_grad_(True) for w in weights(F, D))
+    h = hstu_amd.gated_linear(x, wg, wu, name)
+    dx, dgate, dup = torch.autograd.grad(h, (x, wg, wu), dh)
+    xd, gd, ud = x.detach(), wg.detach(), wu.detach()
+    rx, rg, ru, dg, du = orc.gated_bwd_ref(dh, xd, gd, ud, name)
+    xa, ga, ua, da = xd.double().abs(), gd.double().abs(), ud.double().abs(), dh.double().abs()
+    sg, su = xa @ ga.t(), xa @ ua.t()
+    n = (D + 16) * ULP
+    u = (xd.double() @ ud.double().t()).abs()
+    # dg and du as they are rounded: their own rounding, and the sums' that they come from
+    og = dg.abs() * (HALF + ARG) + n * da * (1.13 * su + u * sg + n * su * sg) + da * u * ARG
+    ou = du.abs() * (HALF + ARG) + n * da * 1.13 * sg
+    top_g, top_u = dg.abs() + og, du.abs() + ou
+    within(dx, rx, rx.abs() * HALF + og @ ga + ou @ ua + 2 * F * ULP * (top_g @ ga + top_u @ ua), "dx")
+    within(dgate, rg, rg.abs() * HALF + og.t() @ xa + (M + 64) * ULP * (top_g.t() @ xa), "dgate")
+    within(dup, ru, ru.abs() * HALF + ou.t() @ xa + (M + 64) * ULP * (top_u.t() @ xa), "dup")
+    if M * F >= 4096:  # enough terms for the norm to be near its mean
+        for got, want in ((dx, rx), (dgate, rg), (dup, ru)):
+            assert float((got.double() - want).norm() / want.norm()) <= NORM
+
+
+@gpu
+@pytest.mark.parametrize("modes", [(0, 0), (1, 1), (1, 0), (0, 1)])
+@pytest.mark.parametrize("M,D,F", [(1, 128, 128), (5, 384, 128), (17, 512, 256), (65, 256, 384), (129, 1024, 128),
+                                   (300, 640, 256), (1027, 512, 1024), (4100, 256, 512)])
+def test_e4m3(hip_lib, M, D, F, modes):
+    import hstu_amd
+
+    def e4m3(v, by_row):
+        a = v.float().abs()
+        s = (a.amax(-1, keepdim=True) if by_row else a.max().reshape(1, 1)) / 448
+        return (v.float() / s).clamp(-448, 448).to(torch.float8_e4m3fn), s.reshape(-1)
+
+    wg, wu = weights(F, D)
+    (x8, xs), (g8, gs), (u8, us) = (e4m3(t, m) for t, m in ((rnd((M, D), 3).to(DEV), modes[0]), (wg, modes[1]), (wu, modes[1])))
+    h = hstu_amd.gated_linear_fp8(x8, xs, (g8, gs), (u8, us))
+    x = x8.double() * xs.double().reshape(-1, 1)
+    want, tol = h_bound(x, g8.double() * gs.double().reshape(-1, 1), u8.double() * us.double().reshape(-1, 1), "silu")
+    within(h, want, tol, "h")
+
+
+@gpu
+def test_large_arguments(hip_lib):
+    """Gates far out on both sides: silu, gelu and sigmoid saturate without NaN, values and derivatives."""
+    import hstu_amd
+
+    x = torch.zeros((2, 256), dtype=torch.bfloat16, device=DEV)
+    x[0, 0], x[1, 0] = 1.0, -1.0
+    wg, wu = torch.zeros((128, 256), dtype=torch.bfloat16, device=DEV), torch.zeros((128, 256), dtype=torch.bfloat16, device=DEV)
+    wg[:, 0] = torch.tensor([0.0, 1, 10, 60, 87, 89, 100, 1e4] * 16, device=DEV)
+    wu[:, 0] = 1.0
+    for name in ACTS:
+        want, tol = h_bound(x, wg, wu, name)
+        within(hstu_amd.gated_linear(x, wg, wu, name), want, tol + 2.0 ** -100, name)
+        dh = torch.ones((2, 128), dtype=torch.bfloat16, device=DEV)
+        for got in hstu_amd.gated_linear_bwd(dh, x, wg, wu, name):
+            assert torch.isfinite(got.float()).all(), name
+
+
+@gpu
+def test_gradient_against_differences(hip_lib):
+    """The kernels' gradient along a direction against a difference quotient of the float64 formula."""
+    import hstu_amd
+
+    M, D, F = 37, 256, 128
+    x, dh = rnd((M, D), 5).to(DEV), rnd((M, F), 6).to(DEV)
+    wg, wu = weights(F, D, 1)
+    for name in ACTS:
+        grads = hstu_amd.gated_linear_bwd(dh, x, wg, wu, name)
+        base = [t.double() for t in (x, wg, wu)]
+        vs = [torch.randn(t.shape, generator=torch.Generator().manual_seed(7 + i), dtype=torch.float64).to(DEV)
+              for i, t in enumerate(base)]
+
+        def loss(e):
+            return float((orc.gated_ref(*(b + e * v for b, v in zip(base, vs)), name) * dh.double()).sum())
+
+        e = 1e-5
+        diff = (loss(e) - loss(-e)) / (2 * e)
+        got = float(sum((g.double() * v).sum() for g, v in zip(grads, vs)))
+        # each gradient is off by 2^-8 of its 2-norm at most, along v by that times a unit normal number:
+        # four of its deviations, over the three gradients
+        tol = 4 * HALF * float(sum(g.double().norm() ** 2 for g in grads)) ** 0.5 + 1e-4
+        assert abs(got - diff) <= tol, name
+
+
+@gpu
+def test_strided_and_leading_dimensions(hip_lib):
+    import hstu_amd
+
+    wide, wgu = rnd((40, 1024), 8).to(DEV), rnd((256, 512), 9, 0.05).to(DEV)
+    x, wg, wu = wide[:, 512:768], wgu[:, :256], wgu[:, 256:]  # columns of wider buffers
+    want = hstu_amd.gated_linear(x.contiguous(), wg.contiguous(), wu.contiguous())
+    assert torch.equal(hstu_amd.gated_linear(x, wg, wu), want)
+    assert torch.equal(hstu_amd.gated_linear(wide[:, 3:259], wg, wu),
+                       hstu_amd.gated_linear(wide[:, 3:259].contiguous(), wg, wu))
+    x3 = x.contiguous().view(5, 8, 256).requires_grad_(True)
+    h = hstu_amd.gated_linear(x3, wg, wu)
+    assert h.shape == (5, 8, 256) and torch.equal(h.reshape(40, 256), want)
+    (dx,) = torch.autograd.grad(h.float().sum(), (x3,))  # an expanded gradient
+    assert dx.shape == x3.shape
+    ones = torch.ones((40, 256), dtype=torch.bfloat16, device=DEV)
+    assert torch.equal(dx.reshape(40, 256), hstu_amd.gated_linear_bwd(ones, x, wg, wu)[0])
+    # both weights of one [2F, D] parameter: their gradients meet in it
+    both = rnd((256, 256), 10, 0.1).to(DEV).requires_grad_(True)
+    out = hstu_amd.gated_linear(x, both[:128], both[128:])
+    (db,) = torch.autograd.grad(out, (both,), ones[:, :128])
+    _, dg, du = hstu_amd.gated_linear_bwd(ones[:, :128], x, both[:128].detach(), both[128:].detach())
+    assert torch.equal(db, torch.cat((dg, du)))
+    # one weight on both sides: its gradient is the sum
+    same = both[:128].detach().clone().requires_grad_(True)
+    (ds,) = torch.autograd.grad(hstu_amd.gated_linear(x, same, same), (same,), ones[:, :128])
+    _, dg, du = hstu_amd.gated_linear_bwd(ones[:, :128], x, same.detach(), same.detach())
+    assert torch.equal(ds, dg + du)
+
+
+@gpu
+def test_no_rows_and_partial_gradients(hip_lib):
+    import hstu_amd
+
+    wg, wu = (w.requires_grad_(True) for w in weights(128, 256))
+    x = torch.zeros((0, 256), dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    h = hstu_amd.gated_linear(x, wg, wu)
+    assert h.shape == (0, 128)
+    dx, dg, du = torch.autograd.grad(h, (x, wg, wu), torch.zeros_like(h))
+    assert dx.shape == x.shape and not dg.any() and not du.any()
+    x = rnd((20, 256), 11).to(DEV)
+    dh = rnd((20, 128), 12).to(DEV)
+    full = hstu_amd.gated_linear_bwd(dh, x, wg, wu)
+    (dg,) = torch.autograd.grad(hstu_amd.gated_linear(x, wg, wu.detach()), (wg,), dh)
+    assert torch.equal(dg, full[1])
+    xr = x.clone().requires_grad_(True)
+    (dx,) = torch.autograd.grad(hstu_amd.gated_linear(xr, wg.detach(), wu.detach()), (xr,), dh)
+    assert torch.equal(dx, full[0])
+
+
+@gpu
+def test_rows_past_the_last_are_left(hip_lib):
+    """The C entry writes M rows and F columns of a larger buffer, nothing else."""
+    import hstu_amd._lib as lib
+
+    D, F = 256, 128
+    wg, wu = weights(F, D)
+    for M in (1, 17, 130, 4100):
+        x = rnd((M, D), 13).to(DEV)
+        out = torch.full((M + 140, F + 8), 7.0, dtype=torch.bfloat16, device=DEV)
+        st = lib.fn("hstu_gated_fwd")(x.data_ptr(), D, wg.data_ptr(), D, wu.data_ptr(), D, M, F, D, 0, out.data_ptr(),
+                                      F + 8, lib.stream(x))
+        assert st == 0
+        assert (out[M:] == 7).all() and (out[:, F:] == 7).all()
+        assert not (out[:M, :F] == 7).all()
+
+
+@gpu
+def test_side_stream_graph_and_same_bytes(hip_lib):
+    import hstu_amd
+
+    x, dh = rnd((333, 512), 14).to(DEV), rnd((333, 256), 15).to(DEV)
+    wg, wu = weights(256, 512)
+
+    def step():
+        from hstu_amd.fp8 import quantize_e4m3_rows
+
+        (a8, s), (g8, gs), (u8, us) = (quantize_e4m3_rows(t) for t in (x, wg, wu))
+        return ((hstu_amd.gated_linear(x, wg, wu),) + hstu_amd.gated_linear_bwd(dh, x, wg, wu)
+                + (hstu_amd.gated_linear_fp8(a8, s, (g8, gs), (u8, us)),))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        on_side = step()
+    torch.cuda.current_stream().wait_stream(side)
+    want = step()
+    assert all(torch.equal(a, b) for a, b in zip(on_side, want))
+    assert all(torch.equal(a, b) for a, b in zip(step(), want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for k in range(4):
+        x.copy_(rnd((333, 512), 20 + k))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, step())), k
+
+
+# ---------------------------------------------------------------- refusals
+def test_refusals():
+    import hstu_amd
+
+    bf = torch.bfloat16
+    x, w = torch.zeros(2, 256, dtype=bf), torch.zeros(128, 256, dtype=bf)
+    with pytest.raises(NotImplementedError):
+        hstu_amd.gated_linear(x, w, w)  # not on a device
+    with pytest.raises(ValueError):
+        hstu_amd.gated_linear(x, w, w, "relu")
+    with pytest.raises(NotImplementedError):
+        hstu_amd.gated_linear(x.float(), w, w)
+
+
+@gpu
+def test_refusals_on_device(hip_lib):
+    import hstu_amd
+
+    bf = torch.bfloat16
+
+    def z(*shape, dtype=bf):
+        return torch.zeros(shape, dtype=dtype, device=DEV)
+
+    for args in ((z(2, 256), z(128, 512), z(128, 512)), (z(2, 256), z(128, 256), z(256, 256))):
+        with pytest.raises(ValueError):
+            hstu_amd.gated_linear(*args)
+    for args in ((z(2, 128), z(128, 128), z(128, 128)), (z(2, 256), z(64, 256), z(64, 256)),
+                 (z(2, 256), z(128, 256), torch.zeros(128, 256, dtype=bf)),
+                 (z(2, 256), z(128, 256, dtype=torch.float32), z(128, 256))):
+        with pytest.raises(NotImplementedError):
+            hstu_amd.gated_linear(*args)
+    with pytest.raises(ValueError):
+        hstu_amd.gated_linear_bwd(z(2, 256), z(2, 256), z(128, 256), z(128, 256))
+    x8, w8 = z(2, 256).to(torch.float8_e4m3fn), z(128, 256).to(torch.float8_e4m3fn)
+    s = z(1, dtype=torch.float32)
+    with pytest.raises(ValueError):
+        hstu_amd.gated_linear_fp8(x8, z(3, dtype=torch.float32), (w8, s), (w8, s))
+    with pytest.raises(ValueError):
+        hstu_amd.gated_linear_fp8(x8, s, (w8, z(2, dtype=torch.float32)), (w8, s))
+    with pytest.raises(NotImplementedError):
+        hstu_amd.gated_linear_fp8(x8, s, (w8.to(bf), s), (w8, s))
+
+
+def test_c_entry_refusals():
+    """Bad arguments are refused before any launch (no device is touched)."""
+    import hstu_amd._lib as lib
+
+    P = 64  # a stand-in address, never read
+    fwd, bwd, f8 = (lib.fn("hstu_gated_" + n) for n in ("fwd", "bwd", "fwd_fp8"))
+
+    def f(x=P, ldx=256, g=P, ldg=256, u=P, ldu=256, M=4, F=128, D=256, act=0, h=P, ldh=128):
+        return fwd(x, ldx, g, ldg, u, ldu, M, F, D, act, h, ldh, None)
+
+    for bad in (dict(M=-1), dict(F=0), dict(D=0), dict(act=3), dict(act=-1), dict(ldx=255), dict(ldg=8), dict(ldu=8),
+                dict(ldh=127), dict(x=None), dict(g=None), dict(u=None), dict(h=None)):
+        assert f(**bad) == lib.HSTU_E_BAD_ARG, bad
+    for bad in (dict(F=64), dict(D=128), dict(x=72), dict(ldx=260), dict(h=72), dict(ldh=132)):
+        assert f(**bad) == lib.HSTU_E_UNSUPPORTED, bad
+    assert f(M=0) == 0
+
+    def b(dh=P, lddh=128, M=4, out=P, ldo=256):
+        return bwd(dh, lddh, P, 256, P, 256, P, 256, M, 128, 256, 0, out, ldo, None)
+
+    for bad in (dict(dh=None), dict(lddh=100), dict(ldo=255), dict(out=None), dict(M=-1)):
+        assert b(**bad) == lib.HSTU_E_BAD_ARG, bad
+    for bad in (dict(dh=66), dict(lddh=132), dict(ldo=260)):
+        assert b(**bad) == lib.HSTU_E_UNSUPPORTED, bad
+
+    def e(xs=P, gs=P, us=P, D=128, M=4):
+        return f8(P, 128, xs, 1, P, 128, gs, 1, P, 128, us, 1, M, 128, D, 0, P, 128, None)
+
+    for bad in (dict(xs=None), dict(gs=None), dict(us=None), dict(D=256)):
+        assert e(**bad) == lib.HSTU_E_BAD_ARG, bad
+    assert e(D=64) == lib.HSTU_E_UNSUPPORTED and e(xs=65) == lib.HSTU_E_UNSUPPORTED
