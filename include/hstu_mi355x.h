@@ -645,7 +645,8 @@ int hstu_rms_norm_bwd(int dtype, const void* dy, int64_t lddy, const void* h, in
  * products and the activation in one kernel; x [M, D], w_gate and w_up [F, D]
  * (the contraction index contiguous), h [M, F], all bf16, fp32 accumulation,
  * rounded once; ld* in elements.  activation: 0 silu, 1 gelu (tanh form),
- * 2 sigmoid.  D % 256 == 0, F % 128 == 0, any M; rows 16-byte aligned.  Rows
+ * 2 sigmoid.  D % 256 == 0, F % 128 == 0, any M; rows 16-byte aligned and less
+ * than 2^24 bytes apart.  Rows
  * past M are not touched.
  * Replaces: two projections of ops/triton/triton_addmm.py:1756-1767 and an
  *           elementwise pass over both (the reference's UVQK projection has SiLU

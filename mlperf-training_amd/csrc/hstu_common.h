@@ -314,6 +314,43 @@ __device__ __forceinline__ void static_for(F&& f) {
   static_for_impl<N>(f, std::make_integer_sequence<int, N>{});
 }
 
+// ---------------------------------------------------------------- projection tiles
+// LDS operand tiles of the projection GEMMs: rows of 128 bytes, the 16-byte
+// chunk c of row r at position c ^ wide_swz(r), so that a ds_read_b128 of 16
+// consecutive rows (one chunk each) hits 16 distinct bank groups.
+__device__ __forceinline__ int wide_swz(int r) { return ((r >> 1) & 7) ^ (((r >> 5) & 1) << 2); }
+// The two-workgroup forms: a ring of 5 slots of 16 KiB (128 rows x 128 bytes).
+constexpr int kDuoThreads = 256;
+constexpr int kDuoItem = 128 * 128;  // 16 KiB
+constexpr int kDuoSlots = 5;         // 80 KiB: two workgroups per CU
+// 4 x 16 bytes per lane from the buffer to LDS: load j writes lds + 1024 j +
+// 16 lane, from voffset v[j] + soff.  M0 is saved and restored.
+__device__ __forceinline__ void duo_dma4(uint32_t lds, const uint32_t (&v)[4], i32x4 r, uint32_t soff) {
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %6, %7 offen lds\n\t"
+      "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %6, %7 offen lds\n\t"
+      "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tbuffer_load_dwordx4 %4, %6, %7 offen lds\n\t"
+      "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tbuffer_load_dwordx4 %5, %6, %7 offen lds\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "s"(lds), "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "s"(r), "s"(soff)
+      : "memory", "scc");
+}
+
+// Column (within a 32-column block) of accumulator element e (0..15) of lane
+// half h; the MFMA's row index is i = 8 (e / 4) + 4 h + e % 4.
+__device__ __forceinline__ int duo32_col(int h, int e) { return 16 * (e >> 3) + 8 * h + (e & 7); }
+
+__device__ __forceinline__ f32x16 mfma32_bf16(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                 0, 0);
+}
+
+// every wave's LDS reads are done (no memory fence: nothing waits for stores)
+__device__ __forceinline__ void pc_barrier_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 // ---------------------------------------------------------------- mask
 // _get_valid_attn_mask (ops/pytorch/pt_hstu_attention.py:32-84) in terms of
 // the position id(x) = min(max(x - c1, 0), clamp), nondecreasing in x: the

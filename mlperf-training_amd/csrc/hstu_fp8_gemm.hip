@@ -511,8 +511,6 @@ constexpr int kPcStages = 3;
 constexpr int kPcA = 128 * 128;          // A item: 128 rows x 128 bytes
 constexpr int kPcStage = kPcA + 256 * 128;  // + W item: 256 rows x 128 bytes = 48 KiB
 
-__device__ __forceinline__ int wide_swz(int r) { return ((r >> 1) & 7) ^ (((r >> 5) & 1) << 2); }
-
 // Column (within the wave's 64) of accumulator element e = 4 ns + r of lane
 // group g.
 template <bool E4M3_OUT>
@@ -522,9 +520,8 @@ __device__ __forceinline__ int wide_col(int g, int e) {
 }
 
 // Barriers without a memory fence (a fence would make the MFMA waves wait
-// for their own stores): the MFMA waves wait for their LDS reads only, the
-// loader for its loads up to the last VM outstanding ones.
-__device__ __forceinline__ void pc_barrier_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// for their own stores): the MFMA waves wait for their LDS reads only
+// (pc_barrier_lds), the loader for its loads up to the last VM outstanding ones.
 template <int VM>
 __device__ __forceinline__ void pc_barrier_vm() {
   static_assert(VM == 0 || VM == 48, "loader wait counts");
@@ -755,25 +752,6 @@ __global__ void __launch_bounds__(kPcThreads, 1) fp8_gemm_pc_kernel(GemmParams p
 //    vector memory operations is outstanding in the k-loop.
 //  * the epilogue's constants (the lane's column scales and bias, its rows'
 //    scales) are loaded to registers at the last k-step, once no DMA is left.
-constexpr int kDuoThreads = 256;
-constexpr int kDuoItem = 128 * 128;  // 16 KiB
-constexpr int kDuoSlots = 5;         // 80 KiB: two workgroups per CU
-
-// 4 x 16 bytes per lane from the buffer to LDS: load j writes lds + 1024 j +
-// 16 lane, from voffset v[j] + soff.  M0 is saved and restored.
-__device__ __forceinline__ void duo_dma4(uint32_t lds, const uint32_t (&v)[4], i32x4 r, uint32_t soff) {
-  uint32_t saved;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %6, %7 offen lds\n\t"
-      "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %6, %7 offen lds\n\t"
-      "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tbuffer_load_dwordx4 %4, %6, %7 offen lds\n\t"
-      "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tbuffer_load_dwordx4 %5, %6, %7 offen lds\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(saved)
-      : "s"(lds), "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "s"(r), "s"(soff)
-      : "memory", "scc");
-}
 template <bool E4M3_OUT, bool RESID, bool A_BF8>
 __global__ void __launch_bounds__(kDuoThreads, 2) fp8_gemm_duo_kernel(GemmParams p, int per_xcd) {
   __shared__ __attribute__((aligned(1024))) uint8_t ring[kDuoSlots][kDuoItem];
@@ -997,16 +975,6 @@ __global__ void __launch_bounds__(kDuoThreads, 2) fp8_gemm_duo_kernel(GemmParams
 // rows 124 -> 102, 80 -> 70, 96 -> 83 us.  With few rows the tiles no longer
 // cover the chip and a tile's serial k-steps (0.87 us each) are the time; those
 // calls take gemm_few_rows_kernel, or the tile kernel in between (hstu_bf16_gemm).
-//
-// Column (within a 32-column block) of accumulator element e (0..15) of lane
-// half h; the MFMA's row index is i = 8 (e / 4) + 4 h + e % 4.
-__device__ __forceinline__ int duo32_col(int h, int e) { return 16 * (e >> 3) + 8 * h + (e & 7); }
-
-__device__ __forceinline__ f32x16 mfma32_bf16(u32x4 a, u32x4 b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
-                                                 0, 0);
-}
-
 template <bool RESID>
 __global__ void __launch_bounds__(kDuoThreads, 2) bf16_gemm_duo_kernel(GemmParams p, int per_xcd) {
   __shared__ __attribute__((aligned(1024))) uint8_t ring[kDuoSlots][kDuoItem];

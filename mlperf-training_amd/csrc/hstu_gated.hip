@@ -16,6 +16,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "hstu_common.h"
 #include "hstu_mi355x.h"
@@ -63,37 +64,40 @@ struct GatedParams {
   int64_t ldo;         // elements
   int M, F, K;         // K = D in bytes
   int act;
+  int tiles_m;
 };
 
 __device__ __forceinline__ float bf16f(uint32_t b16) { return __builtin_bit_cast(float, b16 << 16); }
 
-// Four consecutive outputs (columns n .. n + 3 of row m) from their products.
-template <bool BWD>
-__device__ __forceinline__ void gated_store4(const GatedParams& p, int m, int n, const float (&g)[4],
-                                             const float (&u)[4]) {
+// N (4 or 8) consecutive outputs from column n of row m on, from their products.
+template <bool BWD, int N>
+__device__ __forceinline__ void gated_store(const GatedParams& p, int m, int n, const float (&g)[N],
+                                            const float (&u)[N]) {
+  using Vec = typename std::conditional<N == 8, u32x4, u32x2>::type;
+  Vec o0, o1;
   if constexpr (!BWD) {
-    float h[4], unused;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float a;
-      act<false>(p.act, g[e], a, unused);
-      h[e] = a * u[e];
+    for (int j = 0; j < N / 2; ++j) {
+      float a0, a1, unused;
+      act<false>(p.act, g[2 * j], a0, unused);
+      act<false>(p.act, g[2 * j + 1], a1, unused);
+      o0[j] = pack_bf16(a0 * u[2 * j], a1 * u[2 * j + 1]);
     }
-    *(u32x2*)(p.out + (int64_t)m * p.ldo + n) = u32x2{pack_bf16(h[0], h[1]), pack_bf16(h[2], h[3])};
+    *(Vec*)(p.out + (int64_t)m * p.ldo + n) = o0;
   } else {
-    const u32x2 d = *(const u32x2*)(p.dh + (int64_t)m * p.lddh + n);
-    float dg[4], du[4];
+    const Vec d = *(const Vec*)(p.dh + (int64_t)m * p.lddh + n);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float dh = bf16f(e & 1 ? d[e >> 1] >> 16 : d[e >> 1] & 0xffffu);
-      float a, da;
-      act<true>(p.act, g[e], a, da);
-      dg[e] = dh * u[e] * da;
-      du[e] = dh * a;
+    for (int j = 0; j < N / 2; ++j) {
+      const float d0 = bf16f(d[j] & 0xffffu), d1 = __builtin_bit_cast(float, d[j] & 0xffff0000u);
+      float a0, a1, b0, b1;
+      act<true>(p.act, g[2 * j], a0, b0);
+      act<true>(p.act, g[2 * j + 1], a1, b1);
+      o0[j] = pack_bf16(d0 * u[2 * j] * b0, d1 * u[2 * j + 1] * b1);
+      o1[j] = pack_bf16(d0 * a0, d1 * a1);
     }
     uint16_t* o = p.out + (int64_t)m * p.ldo + n;
-    *(u32x2*)o = u32x2{pack_bf16(dg[0], dg[1]), pack_bf16(dg[2], dg[3])};
-    *(u32x2*)(o + p.F) = u32x2{pack_bf16(du[0], du[1]), pack_bf16(du[2], du[3])};
+    *(Vec*)o = o0;
+    *(Vec*)(o + p.F) = o1;
   }
 }
 
@@ -160,12 +164,144 @@ __global__ void __launch_bounds__(kThreads) gated_rows_kernel(GatedParams p) {
         u[e] *= xs * p.us[p.us_row ? n + e : 0];
       }
     }
-    gated_store4<BWD>(p, m, n, g, u);
+    gated_store<BWD, 4>(p, m, n, g, u);
+  }
+}
+
+// ---------------------------------------------------------------- tile form, bf16
+// 128 rows x 128 columns of h a workgroup, so 128 x 256 of products: the
+// projection GEMM's two-workgroup form (ring of five 16 KiB slots, exact waits on
+// inline LDS DMAs) with W0 the tile's gate rows and W1 its up rows.  Wave w owns all
+// 128 rows and columns 32 w .. 32 w + 31 of both products, so a lane's
+// accumulators of one output pair up in registers and the epilogue is local.
+// W rows are permuted in LDS so that a lane holds runs of eight columns.
+// Tiles go in groups of kGroupM row panels, column by column: the 64 tiles that run on
+// an XCD at a time then share 8 panels of x and 8 of the weights in its L2,
+// where panel by panel they would stream all of the weights for one panel of x.
+constexpr int kGroupM = 8;
+__device__ __forceinline__ bool tile_of(int tiles_m, int tiles_n, int per_xcd, int& mt, int& nt) {
+  const int xcd = (int)blockIdx.x & 7, t = xcd * per_xcd + ((int)blockIdx.x >> 3);
+  if (t >= min((xcd + 1) * per_xcd, tiles_m * tiles_n)) return false;
+  const int group = t / (kGroupM * tiles_n), m_first = group * kGroupM, m_count = min(kGroupM, tiles_m - m_first);
+  const int in = t - group * kGroupM * tiles_n;
+  nt = in / m_count;
+  mt = m_first + (in - nt * m_count);
+  return true;
+}
+
+template <bool BWD>
+__global__ void __launch_bounds__(kDuoThreads, 2) gated_tile_kernel(GatedParams p, int per_xcd) {
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[kDuoSlots][kDuoItem];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  int mt, nt;
+  if (!tile_of(p.tiles_m, p.F / 128, per_xcd, mt, nt)) return;
+  const int m0 = mt * 128, n0 = nt * 128, mrows = min(128, p.M - m0);
+  const int nk = p.K >> 7;
+
+  uint32_t av[4], wv[2][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int q = 64 * (4 * wave + j) + lane, r = q >> 3, i = r & 31;
+    av[j] = (uint32_t)r * (uint32_t)p.ldx + (uint32_t)(((q & 7) ^ wide_swz(r)) * 16);
+    // W blocks of 32 rows all in one swizzle (a wave reads one block of each product)
+    const uint32_t pos = (uint32_t)(((q & 7) ^ wide_swz(i)) * 16);
+    const int col = (r & ~31) + duo32_col((i >> 2) & 1, 4 * (i >> 3) + (i & 3));
+    wv[0][j] = (uint32_t)col * (uint32_t)p.ldwg + pos;
+    wv[1][j] = (uint32_t)col * (uint32_t)p.ldwu + pos;
+  }
+  // rows past M read as zero
+  const i32x4 ars = rsrc_sgprs(p.x + (int64_t)m0 * p.ldx, (uint32_t)((mrows - 1) * p.ldx + p.K));
+  const i32x4 grs = rsrc_sgprs(p.wg + (int64_t)n0 * p.ldwg, (uint32_t)(127 * p.ldwg + p.K));
+  const i32x4 urs = rsrc_sgprs(p.wu + (int64_t)n0 * p.ldwu, (uint32_t)(127 * p.ldwu + p.K));
+  const uint32_t ring0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)&ring[0][0];
+  auto issue = [&](int it) {  // item it: k-step it / 3; 0 x, 1 gate, 2 up
+    const int s = it / 3, kind = it - 3 * s;
+    const uint32_t dst = __builtin_amdgcn_readfirstlane(ring0 + (uint32_t)((it % kDuoSlots) * kDuoItem + 4096 * wave));
+    if (kind == 0) duo_dma4(dst, av, ars, (uint32_t)(s * 128));
+    else if (kind == 1) duo_dma4(dst, wv[0], grs, (uint32_t)(s * 128));
+    else duo_dma4(dst, wv[1], urs, (uint32_t)(s * 128));
+  };
+  for (int it = 0; it < 5; ++it) issue(it);  // D % 256: at least four k-steps
+
+  const int lr = lane & 31, h = lane >> 5;
+  uint32_t rd[4];  // chunk 2 kk + h of row lr; in odd 32-row blocks of x, kk and kk ^ 2 trade places
+#pragma unroll
+  for (int kk = 0; kk < 4; ++kk) rd[kk] = lr * 128 + (((2 * kk + h) ^ wide_swz(lr)) * 16);
+  const uint32_t w_off = 4096 * wave;
+
+  f32x16 acc[4][2];
+#pragma unroll
+  for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[mb][nb][r] = 0.f;
+  auto kstep = [&](int s, auto items_c) {
+    constexpr int ITEMS = decltype(items_c)::value;
+    if constexpr (ITEMS == 0) dma_barrier<0>();
+    else dma_barrier<8>();
+    const uint8_t* sa = ring[(3 * s) % kDuoSlots];
+    u32x4 w[2][4], a[4][4];
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb) {
+      const uint8_t* sw = ring[(3 * s + 1 + nb) % kDuoSlots] + w_off;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) w[nb][kk] = lds_ld128(sw + rd[kk]);
+    }
+#pragma unroll
+    for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) a[mb][kk] = lds_ld128(sa + 4096 * mb + rd[mb & 1 ? kk ^ 2 : kk]);
+    pc_barrier_lds();  // every wave has read step s: its three slots are free
+    const uint32_t ka = (uint32_t)(128 * (s + 2)), kw1 = (uint32_t)(128 * (s + 1));
+    uint32_t dst[3];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+      dst[k] = __builtin_amdgcn_readfirstlane(ring0 + (uint32_t)(((3 * s + 5 + k) % kDuoSlots) * kDuoItem + 4096 * wave));
+    static_for<32>([&](auto nc) {
+      constexpr int n = decltype(nc)::value, mb = n >> 3, kk = (n >> 1) & 3, nb = n & 1;
+      acc[mb][nb] = mfma32_bf16(w[nb][kk], a[mb][kk], acc[mb][nb]);
+      if constexpr ((n & 1) == 1 && (n >> 1) < 4 * ITEMS) {  // items 3 s + 5 (up), 3 s + 6 (x), 3 s + 7 (gate)
+        constexpr int k = n >> 3, j = (n >> 1) & 3;
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (k == 0) dma_to_lds(dst[0] + 1024 * j, wv[1][j], urs, kw1);
+        else if constexpr (k == 1) dma_to_lds(dst[1] + 1024 * j, av[j], ars, ka);
+        else dma_to_lds(dst[2] + 1024 * j, wv[0][j], grs, ka);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    });
+  };
+  for (int s = 0; s < nk - 2; ++s) kstep(s, std::integral_constant<int, 3>{});
+  kstep(nk - 2, std::integral_constant<int, 1>{});
+  kstep(nk - 1, std::integral_constant<int, 0>{});
+
+  // lane: rows m0 + 32 mb + lr, columns n0 + 32 wave + 16 run + 8 h + (0..7) of both products
+  const int cl = n0 + 32 * wave + 8 * h;
+#pragma unroll
+  for (int mb = 0; mb < 4; ++mb) {
+    const int r = 32 * mb + lr;
+    if (r >= mrows) continue;
+#pragma unroll
+    for (int run = 0; run < 2; ++run) {
+      float g[8], u[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) g[e] = acc[mb][0][8 * run + e], u[e] = acc[mb][1][8 * run + e];
+      gated_store<BWD, 8>(p, m0 + r, cl + 16 * run, g, u);
+    }
   }
 }
 
 template <bool F8, bool BWD>
-int launch_gated(const GatedParams& p, hipStream_t stream) {
+int launch_gated(GatedParams p, hipStream_t stream) {
+  if constexpr (!F8) {
+    p.tiles_m = (p.M + 127) / 128;
+    const int64_t tiles = (int64_t)p.tiles_m * (p.F / 128);
+    if (p.M > 64 && tiles < (1 << 30)) {
+      const int per_xcd = (int)((tiles + 7) / 8);
+      hipLaunchKernelGGL((gated_tile_kernel<BWD>), dim3(8 * per_xcd), dim3(kDuoThreads), 0, stream, p, per_xcd);
+      return (int)hipGetLastError();
+    }
+  }
   const int mb = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
   const int64_t tiles = ((int64_t)p.M + 16 * mb - 1) / (16 * mb) * (p.F / 16);
   if (tiles >= ((int64_t)1 << 31)) return HSTU_E_UNSUPPORTED;
@@ -182,6 +318,8 @@ int check(const GatedParams& p, int es, int D, int kmul) {
   if (p.ldx < (int64_t)D * es || p.ldwg < (int64_t)D * es || p.ldwu < (int64_t)D * es) return HSTU_E_BAD_ARG;
   if (p.M > 0 && (!p.x || !p.wg || !p.wu || !p.out)) return HSTU_E_BAD_ARG;
   if (p.F % 128 || D % kmul) return HSTU_E_UNSUPPORTED;
+  // 32-bit offsets of a tile's rows
+  if ((p.ldx | p.ldwg | p.ldwu) >> 24 || (int64_t)D * es >= (1 << 24)) return HSTU_E_UNSUPPORTED;
   if (((uintptr_t)p.x | (uintptr_t)p.wg | (uintptr_t)p.wu | (uintptr_t)p.out) % 16 ||
       (p.ldx | p.ldwg | p.ldwu) % 16 || p.ldo % 8)
     return HSTU_E_UNSUPPORTED;
