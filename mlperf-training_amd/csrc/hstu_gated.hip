@@ -291,16 +291,128 @@ __global__ void __launch_bounds__(kDuoThreads, 2) gated_tile_kernel(GatedParams 
   }
 }
 
+// ---------------------------------------------------------------- tile form, e4m3
+// The same tile, ring and items on rows of e4m3 (a k-step is 128 elements) with
+// v_mfma_f32_16x16x128_f8f6f4: 16-row blocks 0, 1 of a wave's weights are gate
+// rows, 2, 3 up rows.
+__global__ void __launch_bounds__(kDuoThreads, 2) gated_tile_fp8_kernel(GatedParams p, int per_xcd) {
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[kDuoSlots][kDuoItem];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  int mt, nt;
+  if (!tile_of(p.tiles_m, p.F / 128, per_xcd, mt, nt)) return;
+  const int m0 = mt * 128, n0 = nt * 128, mrows = min(128, p.M - m0);
+  const int nk = p.K >> 7;  // at least two
+
+  uint32_t av[4], wv[2][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int q = 64 * (4 * wave + j) + lane, r = q >> 3, i = r & 31;
+    av[j] = (uint32_t)r * (uint32_t)p.ldx + (uint32_t)(((q & 7) ^ wide_swz(r)) * 16);
+    const uint32_t pos = (uint32_t)(((q & 7) ^ wide_swz(i)) * 16);
+    const int col = (r & ~31) + 8 * ((i & 15) >> 2) + 4 * (i >> 4) + (i & 3);  // a lane: 8 consecutive columns
+    wv[0][j] = (uint32_t)col * (uint32_t)p.ldwg + pos;
+    wv[1][j] = (uint32_t)col * (uint32_t)p.ldwu + pos;
+  }
+  const i32x4 ars = rsrc_sgprs(p.x + (int64_t)m0 * p.ldx, (uint32_t)((mrows - 1) * p.ldx + p.K));
+  const i32x4 grs = rsrc_sgprs(p.wg + (int64_t)n0 * p.ldwg, (uint32_t)(127 * p.ldwg + p.K));
+  const i32x4 urs = rsrc_sgprs(p.wu + (int64_t)n0 * p.ldwu, (uint32_t)(127 * p.ldwu + p.K));
+  const uint32_t ring0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)&ring[0][0];
+  auto issue = [&](int it) {  // item it: k-step it / 3; 0 x, 1 gate, 2 up
+    const int s = it / 3, kind = it - 3 * s;
+    const uint32_t dst = __builtin_amdgcn_readfirstlane(ring0 + (uint32_t)((it % kDuoSlots) * kDuoItem + 4096 * wave));
+    if (kind == 0) duo_dma4(dst, av, ars, (uint32_t)(s * 128));
+    else if (kind == 1) duo_dma4(dst, wv[0], grs, (uint32_t)(s * 128));
+    else duo_dma4(dst, wv[1], urs, (uint32_t)(s * 128));
+  };
+  for (int it = 0; it < 5; ++it) issue(it);
+
+  const int li = lane & 15, q = lane >> 4;
+  // chunks q and q + 4 of row li; in odd 32-row blocks of x the two trade places
+  const uint32_t rd0 = li * 128 + ((q ^ wide_swz(li)) * 16), rd1 = li * 128 + (((q + 4) ^ wide_swz(li)) * 16);
+  const uint32_t w_off = 4096 * wave;
+  const int cl = n0 + 32 * wave + 8 * q;  // the lane's columns: cl + 4 (ns % 2) + (0..3)
+  f32x4 gsv[2], usv[2];
+  float sav[8];
+  auto load_consts = [&]() {
+    const BufRsrc gsr = make_rsrc(p.gs, p.gs_row ? (uint32_t)p.F * 4u : 4u);
+    const BufRsrc usr = make_rsrc(p.us, p.us_row ? (uint32_t)p.F * 4u : 4u);
+    const BufRsrc xsr = make_rsrc(p.xs + (p.xs_row ? m0 : 0), p.xs_row ? (uint32_t)mrows * 4u : 4u);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (p.gs_row) gsv[i] = __builtin_bit_cast(f32x4, buf_ld128(gsr, (uint32_t)(cl + 4 * i) * 4u, 0));
+      else gsv[i] = zero4() + buf_ldf(gsr, 0, 0);
+      if (p.us_row) usv[i] = __builtin_bit_cast(f32x4, buf_ld128(usr, (uint32_t)(cl + 4 * i) * 4u, 0));
+      else usv[i] = zero4() + buf_ldf(usr, 0, 0);
+    }
+#pragma unroll
+    for (int ms = 0; ms < 8; ++ms) sav[ms] = buf_ldf(xsr, p.xs_row ? (uint32_t)(16 * ms + li) * 4u : 0u, 0);
+  };
+
+  f32x4 acc[8][4];
+  auto mfma_rows = [&](const i32x8 (&w)[4], const i32x8 (&a)[4], int ms0, bool first) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int ns = 0; ns < 4; ++ns) acc[ms0 + i][ns] = mfma_fp8(w[ns], a[i], first ? zero4() : acc[ms0 + i][ns]);
+  };
+  auto read_a = [&](const uint8_t* st, int ms0, i32x8 (&a)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int ms = ms0 + i;
+      a[i] = cat8(lds_ld128(st + (ms & 2 ? rd1 : rd0) + 2048 * ms), lds_ld128(st + (ms & 2 ? rd0 : rd1) + 2048 * ms));
+    }
+  };
+  auto kstep = [&](int s, auto first_c, auto last_c) {
+    constexpr bool FIRST = decltype(first_c)::value, LAST = decltype(last_c)::value;
+    if constexpr (LAST) dma_barrier<0>();
+    else dma_barrier<8>();
+    const uint8_t* sa = ring[(3 * s) % kDuoSlots];
+    i32x8 w[4], a0[4], a1[4];
+#pragma unroll
+    for (int ns = 0; ns < 4; ++ns) {
+      const uint8_t* sw = ring[(3 * s + 1 + (ns >> 1)) % kDuoSlots] + w_off + 2048 * (ns & 1);
+      w[ns] = cat8(lds_ld128(sw + rd0), lds_ld128(sw + rd1));
+    }
+    read_a(sa, 0, a0);
+    mfma_rows(w, a0, 0, FIRST);
+    read_a(sa, 4, a1);
+    pc_barrier_lds();  // every wave has read step s: its three slots are free
+    if constexpr (LAST) {
+      load_consts();
+    } else {
+#pragma unroll
+      for (int k = 5; k < 8; ++k)
+        if (3 * s + k < 3 * nk) issue(3 * s + k);
+    }
+    mfma_rows(w, a1, 4, FIRST);
+  };
+  kstep(0, std::true_type{}, std::false_type{});
+  for (int s = 1; s < nk - 1; ++s) kstep(s, std::false_type{}, std::false_type{});
+  kstep(nk - 1, std::false_type{}, std::true_type{});
+
+#pragma unroll
+  for (int ms = 0; ms < 8; ++ms) {
+    const int r = 16 * ms + li;
+    if (r >= mrows) continue;
+    float g[8], u[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      g[e] = acc[ms][e >> 2][e & 3] * (sav[ms] * gsv[e >> 2][e & 3]);
+      u[e] = acc[ms][2 + (e >> 2)][e & 3] * (sav[ms] * usv[e >> 2][e & 3]);
+    }
+    gated_store<false, 8>(p, m0 + r, cl, g, u);
+  }
+}
+
 template <bool F8, bool BWD>
 int launch_gated(GatedParams p, hipStream_t stream) {
-  if constexpr (!F8) {
-    p.tiles_m = (p.M + 127) / 128;
-    const int64_t tiles = (int64_t)p.tiles_m * (p.F / 128);
-    if (p.M > 64 && tiles < (1 << 30)) {
-      const int per_xcd = (int)((tiles + 7) / 8);
-      hipLaunchKernelGGL((gated_tile_kernel<BWD>), dim3(8 * per_xcd), dim3(kDuoThreads), 0, stream, p, per_xcd);
-      return (int)hipGetLastError();
-    }
+  p.tiles_m = (p.M + 127) / 128;
+  const int64_t big = (int64_t)p.tiles_m * (p.F / 128);
+  if (p.M > 64 && p.K >= 256 && big < (1 << 30)) {
+    const int per_xcd = (int)((big + 7) / 8);
+    if constexpr (F8) hipLaunchKernelGGL(gated_tile_fp8_kernel, dim3(8 * per_xcd), dim3(kDuoThreads), 0, stream, p, per_xcd);
+    else hipLaunchKernelGGL((gated_tile_kernel<BWD>), dim3(8 * per_xcd), dim3(kDuoThreads), 0, stream, p, per_xcd);
+    return (int)hipGetLastError();
   }
   const int mb = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
   const int64_t tiles = ((int64_t)p.M + 16 * mb - 1) / (16 * mb) * (p.F / 16);
