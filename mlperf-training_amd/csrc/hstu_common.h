@@ -351,6 +351,23 @@ __device__ __forceinline__ f32x16 mfma32_bf16(u32x4 a, u32x4 b, f32x16 c) {
 // every wave's LDS reads are done (no memory fence: nothing waits for stores)
 __device__ __forceinline__ void pc_barrier_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// Output tile of a workgroup: XCD x (workgroups x, x + 8, ...) runs the tile
+// range [x per_xcd, (x + 1) per_xcd), in groups of kGroupM row panels, column by
+// column: the tiles that run on an XCD at a time share a few panels of both
+// operands in its L2, where panel by panel they would stream all of the weights
+// for one panel of rows.  False for a workgroup past the last tile.
+constexpr int kGroupM = 8;
+__device__ __forceinline__ bool tile_of(int tiles_m, int tiles_n, int per_xcd, int& mt, int& nt) {
+  const int xcd = (int)blockIdx.x & 7, t = xcd * per_xcd + ((int)blockIdx.x >> 3);
+  if (t >= min((xcd + 1) * per_xcd, tiles_m * tiles_n)) return false;
+  const int group = t / (kGroupM * tiles_n), m_first = group * kGroupM, m_count = min(kGroupM, tiles_m - m_first);
+  const int in = t - group * kGroupM * tiles_n;
+  nt = in / m_count;
+  mt = m_first + (in - nt * m_count);
+  return true;
+}
+
+
 // ---------------------------------------------------------------- mask
 // _get_valid_attn_mask (ops/pytorch/pt_hstu_attention.py:32-84) in terms of
 // the position id(x) = min(max(x - c1, 0), clamp), nondecreasing in x: the

@@ -175,20 +175,6 @@ __global__ void __launch_bounds__(kThreads) gated_rows_kernel(GatedParams p) {
 // 128 rows and columns 32 w .. 32 w + 31 of both products, so a lane's
 // accumulators of one output pair up in registers and the epilogue is local.
 // W rows are permuted in LDS so that a lane holds runs of eight columns.
-// Tiles go in groups of kGroupM row panels, column by column: the 64 tiles that run on
-// an XCD at a time then share 8 panels of x and 8 of the weights in its L2,
-// where panel by panel they would stream all of the weights for one panel of x.
-constexpr int kGroupM = 8;
-__device__ __forceinline__ bool tile_of(int tiles_m, int tiles_n, int per_xcd, int& mt, int& nt) {
-  const int xcd = (int)blockIdx.x & 7, t = xcd * per_xcd + ((int)blockIdx.x >> 3);
-  if (t >= min((xcd + 1) * per_xcd, tiles_m * tiles_n)) return false;
-  const int group = t / (kGroupM * tiles_n), m_first = group * kGroupM, m_count = min(kGroupM, tiles_m - m_first);
-  const int in = t - group * kGroupM * tiles_n;
-  nt = in / m_count;
-  mt = m_first + (in - nt * m_count);
-  return true;
-}
-
 template <bool BWD>
 __global__ void __launch_bounds__(kDuoThreads, 2) gated_tile_kernel(GatedParams p, int per_xcd) {
   __shared__ __attribute__((aligned(1024))) uint8_t ring[kDuoSlots][kDuoItem];

@@ -15,6 +15,9 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <mutex>
+#include <type_traits>
+#include <vector>
 
 #include "hstu_common.h"
 #include "hstu_mi355x.h"
@@ -135,6 +138,14 @@ __device__ __forceinline__ f32x4 mfma_mx4(u32x4 a, u32x4 b, f32x4 c, int sa, int
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(cat8(a, z), cat8(b, z), c, 4, 4, 0, sa, 0, sb);
 }
 
+__device__ __forceinline__ void add8(u32x4 b, float (&v)[8]) {  // eight bf16
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t x = b[j];
+    v[2 * j] += bf16f(x & 0xffffu);
+    v[2 * j + 1] += __builtin_bit_cast(float, x & 0xffff0000u);
+  }
+}
 // Four consecutive outputs of row m from column n on.
 __device__ __forceinline__ void mx_store4(const MxParams& p, int m, int n, f32x4 v) {
   if (p.bias) {
@@ -193,6 +204,212 @@ __global__ void __launch_bounds__(kThreads) mx_rows_kernel(MxParams p) {
   }
 }
 
+// Tile form: 256 x 256 outputs a workgroup of 8 waves (2 x 4 of 128 x 64, 4 x 2
+// accumulators of 32 x 32), v_mfma_scale_f32_32x32x64_f8f6f4.
+//  * A step is 128 values of k: 64 bytes of each row and one dword of its
+//    scales, 34 KiB, in a ring of four (136 KiB).  LDS DMA (inline assembly,
+//    exact waits) fills a step's place four steps ahead.
+//  * Fragments roll: while step t's MFMAs run, the registers of an A block
+//    whose last MFMA is issued take the same block of step t + 1, and W's
+//    second set takes step t + 1's W; so step t's place in the ring is free
+//    when step t begins, and the one barrier a step finds its operands read.
+//  * Lane half h takes chunks 2 h and 2 h + 1 of its row for the two MFMAs of a
+//    step, in both operands, so its two scale bytes are neighbours: one 16-bit
+//    LDS read, the byte is the instruction's selector.
+//  * Steps come in pairs (the two W sets); an odd count ends with a step of
+//    zeros, read from past the operands' ends.
+//  * 16-byte chunk c of LDS row r (64 bytes) lies at c ^ ((r >> 2) & 3): 16
+//    consecutive rows read one chunk each from 16 distinct bank groups.  W rows
+//    are permuted in LDS so that a lane holds runs of eight columns.
+constexpr int kMxThreads = 512;
+constexpr int kMxTile = 256;
+constexpr int kMxRing = 4;
+constexpr int kMxOperand = kMxTile * 64;                  // 16 KiB
+constexpr int kMxStage = 2 * kMxOperand + 2 * kMxTile * 4;  // A, W, their scales
+constexpr int kMxLds = kMxRing * kMxStage;
+
+__device__ __forceinline__ f32x16 mfma32_mx4_lo(u32x4 a, u32x4 b, f32x16 c, int sa, int sb) {
+  const u32x4 z = {0u, 0u, 0u, 0u};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(cat8(a, z), cat8(b, z), c, 4, 4, 0, sa, 0, sb);
+}
+__device__ __forceinline__ f32x16 mfma32_mx4_hi(u32x4 a, u32x4 b, f32x16 c, int sa, int sb) {
+  const u32x4 z = {0u, 0u, 0u, 0u};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(cat8(a, z), cat8(b, z), c, 4, 4, 1, sa, 1, sb);
+}
+// 4 bytes a lane: lane l's dword to lds + 4 l
+__device__ __forceinline__ void dma4_to_lds(uint32_t lds, uint32_t v, i32x4 r, uint32_t soff) {
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dword %2, %3, %4 offen lds\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "s"(lds), "v"(v), "s"(r), "s"(soff)
+      : "memory");
+}
+
+__global__ void __launch_bounds__(kMxThreads, 2) mx_tile_kernel(MxParams p, int tiles_m, int tiles_n, int per_xcd) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  int mt, nt;
+  if (!tile_of(tiles_m, tiles_n, per_xcd, mt, nt)) return;
+  const int m0 = mt * kMxTile, n0 = nt * kMxTile;
+  const int mrows = min(kMxTile, p.M - m0), ncols = min(kMxTile, p.N - n0);
+  const int T = (p.K >> 7) + ((p.K >> 7) & 1);
+
+  // rows past M and N read as zero (code 0, scale byte 0)
+  const uint32_t a_bytes = (uint32_t)((mrows - 1) * p.lda + p.K / 2), w_bytes = (uint32_t)((ncols - 1) * p.ldw + p.K / 2);
+  const i32x4 ars = rsrc_sgprs(p.A + (int64_t)m0 * p.lda, a_bytes), wrs = rsrc_sgprs(p.W + (int64_t)n0 * p.ldw, w_bytes);
+  // waves 0-3 load A's scales, 4-7 W's: one dword of 64 rows each
+  const bool sw_wave = wave >= 4;
+  const uint32_t s_bytes = sw_wave ? (uint32_t)((ncols - 1) * p.ldws + p.K / 32) : (uint32_t)((mrows - 1) * p.ldas + p.K / 32);
+  const i32x4 srs = rsrc_sgprs(sw_wave ? p.ws + (int64_t)n0 * p.ldws : p.as + (int64_t)m0 * p.ldas, s_bytes);
+  auto column = [](int r) {  // output column (in the tile) of LDS row r of W
+    const int i = r & 31;
+    return (r & ~31) + duo32_col((i >> 2) & 1, 4 * (i >> 3) + (i & 3));
+  };
+  uint32_t av[2], wv[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int q = 64 * (2 * wave + j) + lane, r = q >> 2;
+    const uint32_t pos = (uint32_t)(((q & 3) ^ ((r >> 2) & 3)) * 16);
+    av[j] = (uint32_t)r * (uint32_t)p.lda + pos;
+    wv[j] = (uint32_t)column(r) * (uint32_t)p.ldw + pos;
+  }
+  const int sr = 64 * (wave & 3) + lane;
+  const uint32_t sv = sw_wave ? (uint32_t)column(sr) * (uint32_t)p.ldws : (uint32_t)sr * (uint32_t)p.ldas;
+  const uint32_t lds0 =
+      __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)smem);
+  auto issue = [&](int t) {  // five loads of this wave
+    const uint32_t st = lds0 + (uint32_t)((t & (kMxRing - 1)) * kMxStage);
+    const bool real = 128 * t < p.K;
+    const uint32_t ka = real ? (uint32_t)(64 * t) : a_bytes, kw = real ? (uint32_t)(64 * t) : w_bytes;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      dma_to_lds(st + 1024u * (uint32_t)(2 * wave + j), av[j], ars, ka);
+      dma_to_lds(st + kMxOperand + 1024u * (uint32_t)(2 * wave + j), wv[j], wrs, kw);
+    }
+    dma4_to_lds(st + 2 * kMxOperand + 256u * (uint32_t)wave, sv, srs, real ? (uint32_t)(4 * t) : s_bytes);
+  };
+
+  const int lr = lane & 31, h = lane >> 5, wm = wave >> 2, wn = wave & 3;
+  uint32_t rd[2];  // chunk 2 h + kk of row lr of a 32-row block
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk) rd[kk] = lr * 64 + (((2 * h + kk) ^ ((lr >> 2) & 3)) * 16);
+  const uint32_t a_off = 128 * 64 * wm, w_off = kMxOperand + 64 * 64 * wn;
+  const uint32_t as_off = 2 * kMxOperand + 4 * (128 * wm + lr) + 2 * h;
+  const uint32_t ws_off = 2 * kMxOperand + 4 * (kMxTile + 64 * wn + lr) + 2 * h;
+
+  u32x4 a[4][2], w[2][2][2];
+  int sa[4], sw[2][2];
+  auto read_a = [&](const uint8_t* st, int mb) {
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) a[mb][kk] = lds_ld128(st + a_off + 2048 * mb + rd[kk]);
+    sa[mb] = *(const uint16_t*)(st + as_off + 128 * mb);
+  };
+  auto read_w = [&](const uint8_t* st, int set) {
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb) {
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) w[set][nb][kk] = lds_ld128(st + w_off + 2048 * nb + rd[kk]);
+      sw[set][nb] = *(const uint16_t*)(st + ws_off + 128 * nb);
+    }
+  };
+  f32x16 acc[4][2];
+#pragma unroll
+  for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[mb][nb][r] = 0.f;
+
+  issue(0);
+  issue(1);
+  if (T > 2) {
+    issue(2);
+    issue(3);
+    dma_barrier<15>();
+  } else {
+    dma_barrier<5>();
+  }
+  read_w(smem, 0);
+#pragma unroll
+  for (int mb = 0; mb < 4; ++mb) read_a(smem, mb);
+
+  // step t on W set SET; NEXT: there is a step t + 1, which has landed
+  auto step = [&](int t, auto set_c, auto next_c) {
+    constexpr int SET = decltype(set_c)::value;
+    constexpr bool NEXT = decltype(next_c)::value;
+    const uint8_t* st = smem + ((t + 1) & (kMxRing - 1)) * kMxStage;
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (NEXT) read_w(st, SET ^ 1);
+    static_for<4>([&](auto mb_c) {
+      constexpr int mb = decltype(mb_c)::value;
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb) acc[mb][nb] = mfma32_mx4_lo(w[SET][nb][0], a[mb][0], acc[mb][nb], sw[SET][nb], sa[mb]);
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb) acc[mb][nb] = mfma32_mx4_hi(w[SET][nb][1], a[mb][1], acc[mb][nb], sw[SET][nb], sa[mb]);
+      if constexpr (NEXT) read_a(st, mb);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  // Before step t: every wave has read it, and step t + 1 has landed when only the
+  // later steps' loads (five each) are outstanding; its place takes step t + 4.
+  using Zero = std::integral_constant<int, 0>;
+  using One = std::integral_constant<int, 1>;
+  int t = 0;
+  for (; t + 5 < T; t += 2) {
+    dma_barrier<10>();
+    issue(t + 4);
+    step(t, Zero{}, std::true_type{});
+    dma_barrier<10>();
+    issue(t + 5);
+    step(t + 1, One{}, std::true_type{});
+  }
+  if (t + 2 < T) {
+    dma_barrier<10>();
+    step(t, Zero{}, std::true_type{});
+    dma_barrier<5>();
+    step(t + 1, One{}, std::true_type{});
+  }
+  dma_barrier<0>();
+  step(T - 2, Zero{}, std::true_type{});
+  step(T - 1, One{}, std::false_type{});
+
+  // lane: rows m0 + 128 wm + 32 mb + lr, columns n0 + 64 wn + 32 nb + 16 run + 8 h + (0..7)
+  const int cl = n0 + 64 * wn + 8 * h;
+#pragma unroll
+  for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+    for (int run = 0; run < 2; ++run) {
+      const int c = cl + 32 * nb + 16 * run;
+      if (c >= p.N) continue;
+      float b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (p.bias) add8(*(const u32x4*)(p.bias + c), b);
+#pragma unroll
+      for (int mb = 0; mb < 4; ++mb) {
+        const int m = m0 + 128 * wm + 32 * mb + lr;
+        if (m >= p.M) continue;
+        float o[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = acc[mb][nb][8 * run + e] + b[e];
+        if (p.resid) add8(*(const u32x4*)(p.resid + (int64_t)m * p.ldr + c), o);
+        *(u32x4*)(p.C + (int64_t)m * p.ldc + c) =
+            u32x4{pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7])};
+      }
+    }
+}
+
+hipError_t set_mx_lds(const void* fn) {
+  static std::mutex mu;
+  static std::vector<const void*> done;
+  std::lock_guard<std::mutex> lock(mu);
+  for (const void* d : done)
+    if (d == fn) return hipSuccess;
+  const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, kMxLds);
+  if (e == hipSuccess) done.push_back(fn);
+  return e;
+}
+
 }  // namespace
 
 extern "C" int hstu_mxfp4_quantize(int dtype, const void* x, int64_t ldx, int64_t rows, int cols, void* codes,
@@ -247,6 +464,15 @@ extern "C" int hstu_mxfp4_gemm(const void* A, int64_t lda, const void* a_scale, 
   if (M == 0) return 0;
   MxParams p{(const uint8_t*)A, (const uint8_t*)W, (const uint8_t*)a_scale, (const uint8_t*)w_scale, lda, ldw, ldas,
              ldws, (const uint16_t*)bias, (const uint16_t*)residual, (uint16_t*)C, ldr, ldc, M, N, K};
+  const int64_t tiles_m = ((int64_t)M + kMxTile - 1) / kMxTile, tiles_n = (N + kMxTile - 1) / kMxTile;
+  if (M > 64 && tiles_m * tiles_n < (1 << 30) && (int64_t)kMxTile * std::max(lda, ldw) < ((int64_t)1 << 31)) {
+    hipError_t e = set_mx_lds((const void*)mx_tile_kernel);
+    if (e != hipSuccess) return (int)e;
+    const int per_xcd = (int)((tiles_m * tiles_n + 7) / 8);
+    hipLaunchKernelGGL(mx_tile_kernel, dim3(8 * per_xcd), dim3(kMxThreads), kMxLds, stream, p, (int)tiles_m,
+                       (int)tiles_n, per_xcd);
+    return (int)hipGetLastError();
+  }
   const int mb = M <= 16 ? 1 : M <= 32 ? 2 : 4;
   const int64_t tiles = ((int64_t)M + 16 * mb - 1) / (16 * mb) * (N / 16);
   if (tiles >= ((int64_t)1 << 31)) return HSTU_E_UNSUPPORTED;
