@@ -279,17 +279,17 @@ __global__ void __launch_bounds__(kMxThreads, 2) mx_tile_kernel(MxParams p, int 
   const uint32_t sv = sw_wave ? (uint32_t)column(sr) * (uint32_t)p.ldws : (uint32_t)sr * (uint32_t)p.ldas;
   const uint32_t lds0 =
       __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)smem);
-  auto issue = [&](int t) {  // five loads of this wave
+  // load i (0 .. 4) of this wave for step t
+  auto load = [&](int t, auto i_c) {
+    constexpr int i = decltype(i_c)::value, j = i & 1;
     const uint32_t st = lds0 + (uint32_t)((t & (kMxRing - 1)) * kMxStage);
     const bool real = 128 * t < p.K;
-    const uint32_t ka = real ? (uint32_t)(64 * t) : a_bytes, kw = real ? (uint32_t)(64 * t) : w_bytes;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      dma_to_lds(st + 1024u * (uint32_t)(2 * wave + j), av[j], ars, ka);
-      dma_to_lds(st + kMxOperand + 1024u * (uint32_t)(2 * wave + j), wv[j], wrs, kw);
-    }
-    dma4_to_lds(st + 2 * kMxOperand + 256u * (uint32_t)wave, sv, srs, real ? (uint32_t)(4 * t) : s_bytes);
+    if constexpr (i < 2) dma_to_lds(st + 1024u * (uint32_t)(2 * wave + j), av[j], ars, real ? (uint32_t)(64 * t) : a_bytes);
+    else if constexpr (i < 4)
+      dma_to_lds(st + kMxOperand + 1024u * (uint32_t)(2 * wave + j), wv[j], wrs, real ? (uint32_t)(64 * t) : w_bytes);
+    else dma4_to_lds(st + 2 * kMxOperand + 256u * (uint32_t)wave, sv, srs, real ? (uint32_t)(4 * t) : s_bytes);
   };
+  auto issue = [&](int t) { static_for<5>([&](auto i_c) { load(t, i_c); }); };
 
   const int lr = lane & 31, h = lane >> 5, wm = wave >> 2, wn = wave & 3;
   uint32_t rd[2];  // chunk 2 h + kk of row lr of a 32-row block
@@ -335,17 +335,25 @@ __global__ void __launch_bounds__(kMxThreads, 2) mx_tile_kernel(MxParams p, int 
 #pragma unroll
   for (int mb = 0; mb < 4; ++mb) read_a(smem, mb);
 
-  // step t on W set SET; NEXT: there is a step t + 1, which has landed
-  auto step = [&](int t, auto set_c, auto next_c) {
+  // step t on W set SET; NEXT: there is a step t + 1, which has landed; MORE: and
+  // a step t + 4 to load, spread between the MFMAs
+  auto step = [&](int t, auto set_c, auto next_c, auto more_c) {
     constexpr int SET = decltype(set_c)::value;
-    constexpr bool NEXT = decltype(next_c)::value;
+    constexpr bool NEXT = decltype(next_c)::value, MORE = decltype(more_c)::value;
     const uint8_t* st = smem + ((t + 1) & (kMxRing - 1)) * kMxStage;
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0), which the barrier has seen to: tells the compiler
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (NEXT) read_w(st, SET ^ 1);
     static_for<4>([&](auto mb_c) {
       constexpr int mb = decltype(mb_c)::value;
 #pragma unroll
       for (int nb = 0; nb < 2; ++nb) acc[mb][nb] = mfma32_mx4_lo(w[SET][nb][0], a[mb][0], acc[mb][nb], sw[SET][nb], sa[mb]);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (MORE) {
+        load(t + kMxRing, mb_c);
+        if constexpr (mb == 3) load(t + kMxRing, std::integral_constant<int, 4>{});
+      }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int nb = 0; nb < 2; ++nb) acc[mb][nb] = mfma32_mx4_hi(w[SET][nb][1], a[mb][1], acc[mb][nb], sw[SET][nb], sa[mb]);
       if constexpr (NEXT) read_a(st, mb);
@@ -357,23 +365,23 @@ __global__ void __launch_bounds__(kMxThreads, 2) mx_tile_kernel(MxParams p, int 
   using Zero = std::integral_constant<int, 0>;
   using One = std::integral_constant<int, 1>;
   int t = 0;
+  using No = std::false_type;
+  using Yes = std::true_type;
   for (; t + 5 < T; t += 2) {
     dma_barrier<10>();
-    issue(t + 4);
-    step(t, Zero{}, std::true_type{});
+    step(t, Zero{}, Yes{}, Yes{});
     dma_barrier<10>();
-    issue(t + 5);
-    step(t + 1, One{}, std::true_type{});
+    step(t + 1, One{}, Yes{}, Yes{});
   }
   if (t + 2 < T) {
     dma_barrier<10>();
-    step(t, Zero{}, std::true_type{});
+    step(t, Zero{}, Yes{}, No{});
     dma_barrier<5>();
-    step(t + 1, One{}, std::true_type{});
+    step(t + 1, One{}, Yes{}, No{});
   }
   dma_barrier<0>();
-  step(T - 2, Zero{}, std::true_type{});
-  step(T - 1, One{}, std::false_type{});
+  step(T - 2, Zero{}, Yes{}, No{});
+  step(T - 1, One{}, No{}, No{});
 
   // lane: rows m0 + 128 wm + 32 mb + lr, columns n0 + 64 wn + 32 nb + 16 run + 8 h + (0..7)
   const int cl = n0 + 64 * wn + 8 * h;
