@@ -206,45 +206,32 @@ __global__ void __launch_bounds__(kThreads) mx_rows_kernel(MxParams p) {
 
 // Tile form: 256 x 256 outputs a workgroup of 8 waves (2 x 4 of 128 x 64, 4 x 2
 // accumulators of 32 x 32), v_mfma_scale_f32_32x32x64_f8f6f4.
-//  * A step is 128 values of k: 64 bytes of each row and one dword of its
-//    scales, 34 KiB, in a ring of four (136 KiB).  LDS DMA (inline assembly,
-//    exact waits) fills a step's place four steps ahead.
-//  * Fragments roll: while step t's MFMAs run, the registers of an A block
-//    whose last MFMA is issued take the same block of step t + 1, and W's
-//    second set takes step t + 1's W; so step t's place in the ring is free
-//    when step t begins, and the one barrier a step finds its operands read.
-//  * Lane half h takes chunks 2 h and 2 h + 1 of its row for the two MFMAs of a
-//    step, in both operands, so its two scale bytes are neighbours: one 16-bit
-//    LDS read, the byte is the instruction's selector.
-//  * Steps come in pairs (the two W sets); an odd count ends with a step of
-//    zeros, read from past the operands' ends.
-//  * 16-byte chunk c of LDS row r (64 bytes) lies at c ^ ((r >> 2) & 3): 16
-//    consecutive rows read one chunk each from 16 distinct bank groups.  W rows
-//    are permuted in LDS so that a lane holds runs of eight columns.
+//  * A step is 256 values of k, 128 bytes of each row: 64 KiB, in a ring of two,
+//    filled by LDS DMA (inline assembly, explicit waits).  Whole 128-byte lines
+//    halve the requests to L2 that 64-byte pieces make.  A row's scales come 16
+//    bytes (two steps) at a time, because every row of them is a line of its own.
+//  * Fragments roll: while step s's MFMAs run, each register whose last MFMA is
+//    issued takes the same fragment of step s + 1.  So step s's place in the ring
+//    is free when step s begins, step s + 2's loads go there, and have until step
+//    s + 1 begins to land: one barrier a step, which finds the operands read.
+//  * Lane half h takes chunks (16 bytes, one block) 4 h .. 4 h + 3 of its row for a
+//    step's four MFMAs, so one dword holds its scale bytes and the byte is the
+//    instruction's selector.  In a last step of 128 values half 1 has none: its
+//    W codes and scales are cleared in registers.
+//  * Chunk c of LDS row r lies at c ^ ((r >> 1) & 7): 16 consecutive rows read one
+//    chunk each from 16 distinct bank groups.  W rows are permuted in LDS so that a
+//    lane holds runs of eight columns.
 constexpr int kMxThreads = 512;
 constexpr int kMxTile = 256;
-constexpr int kMxRing = 4;
-constexpr int kMxOperand = kMxTile * 64;                  // 16 KiB
-constexpr int kMxStage = 2 * kMxOperand + 2 * kMxTile * 4;  // A, W, their scales
-constexpr int kMxLds = kMxRing * kMxStage;
+constexpr int kMxOperand = kMxTile * 128;    // 32 KiB
+constexpr int kMxStage = 2 * kMxOperand;     // A, W
+constexpr int kMxScales = 2 * kMxTile * 16;  // 16 bytes for each row of A and W: two steps
+constexpr int kMxLds = 2 * kMxStage + 2 * kMxScales;
 
-__device__ __forceinline__ f32x16 mfma32_mx4_lo(u32x4 a, u32x4 b, f32x16 c, int sa, int sb) {
+template <int BYTE>
+__device__ __forceinline__ f32x16 mfma32_mx4(u32x4 a, u32x4 b, f32x16 c, int sa, int sb) {
   const u32x4 z = {0u, 0u, 0u, 0u};
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(cat8(a, z), cat8(b, z), c, 4, 4, 0, sa, 0, sb);
-}
-__device__ __forceinline__ f32x16 mfma32_mx4_hi(u32x4 a, u32x4 b, f32x16 c, int sa, int sb) {
-  const u32x4 z = {0u, 0u, 0u, 0u};
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(cat8(a, z), cat8(b, z), c, 4, 4, 1, sa, 1, sb);
-}
-// 4 bytes a lane: lane l's dword to lds + 4 l
-__device__ __forceinline__ void dma4_to_lds(uint32_t lds, uint32_t v, i32x4 r, uint32_t soff) {
-  uint32_t saved;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dword %2, %3, %4 offen lds\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(saved)
-      : "s"(lds), "v"(v), "s"(r), "s"(soff)
-      : "memory");
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(cat8(a, z), cat8(b, z), c, 4, 4, BYTE, sa, BYTE, sb);
 }
 
 __global__ void __launch_bounds__(kMxThreads, 2) mx_tile_kernel(MxParams p, int tiles_m, int tiles_n, int per_xcd) {
@@ -254,24 +241,25 @@ __global__ void __launch_bounds__(kMxThreads, 2) mx_tile_kernel(MxParams p, int 
   if (!tile_of(tiles_m, tiles_n, per_xcd, mt, nt)) return;
   const int m0 = mt * kMxTile, n0 = nt * kMxTile;
   const int mrows = min(kMxTile, p.M - m0), ncols = min(kMxTile, p.N - n0);
-  const int T = (p.K >> 7) + ((p.K >> 7) & 1);
+  const int S = (p.K + 255) >> 8;
 
   // rows past M and N read as zero (code 0, scale byte 0)
-  const uint32_t a_bytes = (uint32_t)((mrows - 1) * p.lda + p.K / 2), w_bytes = (uint32_t)((ncols - 1) * p.ldw + p.K / 2);
-  const i32x4 ars = rsrc_sgprs(p.A + (int64_t)m0 * p.lda, a_bytes), wrs = rsrc_sgprs(p.W + (int64_t)n0 * p.ldw, w_bytes);
-  // waves 0-3 load A's scales, 4-7 W's: one dword of 64 rows each
+  const i32x4 ars = rsrc_sgprs(p.A + (int64_t)m0 * p.lda, (uint32_t)((mrows - 1) * p.lda + p.K / 2));
+  const i32x4 wrs = rsrc_sgprs(p.W + (int64_t)n0 * p.ldw, (uint32_t)((ncols - 1) * p.ldw + p.K / 2));
+  // waves 0-3 load A's scales, 4-7 W's: 16 bytes of 64 rows each
   const bool sw_wave = wave >= 4;
-  const uint32_t s_bytes = sw_wave ? (uint32_t)((ncols - 1) * p.ldws + p.K / 32) : (uint32_t)((mrows - 1) * p.ldas + p.K / 32);
-  const i32x4 srs = rsrc_sgprs(sw_wave ? p.ws + (int64_t)n0 * p.ldws : p.as + (int64_t)m0 * p.ldas, s_bytes);
+  const i32x4 srs = rsrc_sgprs(sw_wave ? p.ws + (int64_t)n0 * p.ldws : p.as + (int64_t)m0 * p.ldas,
+                               sw_wave ? (uint32_t)((ncols - 1) * p.ldws + p.K / 32) : (uint32_t)((mrows - 1) * p.ldas + p.K / 32));
   auto column = [](int r) {  // output column (in the tile) of LDS row r of W
     const int i = r & 31;
     return (r & ~31) + duo32_col((i >> 2) & 1, 4 * (i >> 3) + (i & 3));
   };
+  // chunk 4 wave + j of 8 LDS rows; j and j + 2 are 16 rows of memory apart
   uint32_t av[2], wv[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    const int q = 64 * (2 * wave + j) + lane, r = q >> 2;
-    const uint32_t pos = (uint32_t)(((q & 3) ^ ((r >> 2) & 3)) * 16);
+    const int q = 64 * (4 * wave + j) + lane, r = q >> 3;
+    const uint32_t pos = (uint32_t)(((q & 7) ^ ((r >> 1) & 7)) * 16);
     av[j] = (uint32_t)r * (uint32_t)p.lda + pos;
     wv[j] = (uint32_t)column(r) * (uint32_t)p.ldw + pos;
   }
@@ -279,41 +267,36 @@ __global__ void __launch_bounds__(kMxThreads, 2) mx_tile_kernel(MxParams p, int 
   const uint32_t sv = sw_wave ? (uint32_t)column(sr) * (uint32_t)p.ldws : (uint32_t)sr * (uint32_t)p.ldas;
   const uint32_t lds0 =
       __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)smem);
-  // load i (0 .. 4) of this wave for step t
-  auto load = [&](int t, auto i_c) {
-    constexpr int i = decltype(i_c)::value, j = i & 1;
-    const uint32_t st = lds0 + (uint32_t)((t & (kMxRing - 1)) * kMxStage);
-    const bool real = 128 * t < p.K;
-    if constexpr (i < 2) dma_to_lds(st + 1024u * (uint32_t)(2 * wave + j), av[j], ars, real ? (uint32_t)(64 * t) : a_bytes);
-    else if constexpr (i < 4)
-      dma_to_lds(st + kMxOperand + 1024u * (uint32_t)(2 * wave + j), wv[j], wrs, real ? (uint32_t)(64 * t) : w_bytes);
-    else dma4_to_lds(st + 2 * kMxOperand + 256u * (uint32_t)wave, sv, srs, real ? (uint32_t)(4 * t) : s_bytes);
+  // load i (0 .. 7) of this wave for step s; the scales of steps 2 q and 2 q + 1
+  auto load = [&](int s, auto i_c) {
+    constexpr int i = decltype(i_c)::value, j = i & 3;
+    const uint32_t dst = lds0 + (uint32_t)((s & 1) * kMxStage) + 1024u * (uint32_t)(4 * wave + j);
+    if constexpr (i < 4) dma_to_lds(dst, av[j & 1], ars, (uint32_t)(128 * s) + (j >> 1) * 16u * (uint32_t)p.lda);
+    else dma_to_lds(dst + kMxOperand, wv[j & 1], wrs, (uint32_t)(128 * s) + (j >> 1) * 16u * (uint32_t)p.ldw);
   };
-  auto issue = [&](int t) { static_for<5>([&](auto i_c) { load(t, i_c); }); };
+  auto load_scales = [&](int q) {
+    dma_to_lds(lds0 + 2 * kMxStage + (uint32_t)((q & 1) * kMxScales) + 1024u * (uint32_t)wave, sv, srs, (uint32_t)(16 * q));
+  };
 
   const int lr = lane & 31, h = lane >> 5, wm = wave >> 2, wn = wave & 3;
-  uint32_t rd[2];  // chunk 2 h + kk of row lr of a 32-row block
-#pragma unroll
-  for (int kk = 0; kk < 2; ++kk) rd[kk] = lr * 64 + (((2 * h + kk) ^ ((lr >> 2) & 3)) * 16);
-  const uint32_t a_off = 128 * 64 * wm, w_off = kMxOperand + 64 * 64 * wn;
-  const uint32_t as_off = 2 * kMxOperand + 4 * (128 * wm + lr) + 2 * h;
-  const uint32_t ws_off = 2 * kMxOperand + 4 * (kMxTile + 64 * wn + lr) + 2 * h;
+  // chunk 4 h + kk of row lr is at rd ^ 16 kk, its scales at rs
+  const uint32_t rd = lr * 128 + (((4 * h) ^ ((lr >> 1) & 7)) * 16), rs = 16 * lr + 4 * h;
+  const uint32_t a_off = 128 * 128 * wm, w_off = kMxOperand + 64 * 128 * wn;
+  const uint32_t as_off = 2 * kMxStage + 16 * 128 * wm, ws_off = 2 * kMxStage + 16 * (kMxTile + 64 * wn);
 
-  u32x4 a[4][2], w[2][2][2];
-  int sa[4], sw[2][2];
-  auto read_a = [&](const uint8_t* st, int mb) {
+  u32x4 a[4][4], w[2][4];
+  int sa[4], sw[2];
+  // fragments of the step at (f, q): its place in the ring, that of its scales
+  auto read_a = [&](uint32_t f, uint32_t q, int mb) {
+    const uint32_t at = f + a_off + rd;
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) a[mb][kk] = lds_ld128(st + a_off + 2048 * mb + rd[kk]);
-    sa[mb] = *(const uint16_t*)(st + as_off + 128 * mb);
+    for (int kk = 0; kk < 4; ++kk) a[mb][kk] = lds_ld128(smem + (at ^ (16 * kk)) + 4096 * mb);
+    sa[mb] = *(const int*)(smem + q + as_off + rs + 512 * mb);
   };
-  auto read_w = [&](const uint8_t* st, int set) {
-#pragma unroll
-    for (int nb = 0; nb < 2; ++nb) {
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) w[set][nb][kk] = lds_ld128(st + w_off + 2048 * nb + rd[kk]);
-      sw[set][nb] = *(const uint16_t*)(st + ws_off + 128 * nb);
-    }
-  };
+  auto read_w = [&](uint32_t f, int nb, int kk) { w[nb][kk] = lds_ld128(smem + ((f + w_off + rd) ^ (16 * kk)) + 4096 * nb); };
+  auto read_ws = [&](uint32_t q, int nb) { sw[nb] = *(const int*)(smem + q + ws_off + rs + 512 * nb); };
+  auto place = [](int s) { return (uint32_t)((s & 1) * kMxStage); };
+  auto scale_place = [](int s) { return (uint32_t)(((s >> 1) & 1) * kMxScales + 8 * (s & 1)); };
   f32x16 acc[4][2];
 #pragma unroll
   for (int mb = 0; mb < 4; ++mb)
@@ -322,66 +305,76 @@ __global__ void __launch_bounds__(kMxThreads, 2) mx_tile_kernel(MxParams p, int 
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[mb][nb][r] = 0.f;
 
-  issue(0);
-  issue(1);
-  if (T > 2) {
-    issue(2);
-    issue(3);
-    dma_barrier<15>();
+  static_for<8>([&](auto i_c) { load(0, i_c); });
+  load_scales(0);
+  if (S > 1) {
+    static_for<8>([&](auto i_c) { load(1, i_c); });
+    dma_barrier<8>();
   } else {
-    dma_barrier<5>();
+    dma_barrier<0>();
   }
-  read_w(smem, 0);
 #pragma unroll
-  for (int mb = 0; mb < 4; ++mb) read_a(smem, mb);
+  for (int nb = 0; nb < 2; ++nb) {
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) read_w(0, nb, kk);
+    read_ws(0, nb);
+  }
+#pragma unroll
+  for (int mb = 0; mb < 4; ++mb) read_a(0, 0, mb);
 
-  // step t on W set SET; NEXT: there is a step t + 1, which has landed; MORE: and
-  // a step t + 4 to load, spread between the MFMAs
-  auto step = [&](int t, auto set_c, auto next_c, auto more_c) {
-    constexpr int SET = decltype(set_c)::value;
-    constexpr bool NEXT = decltype(next_c)::value, MORE = decltype(more_c)::value;
-    const uint8_t* st = smem + ((t + 1) & (kMxRing - 1)) * kMxStage;
+  // step s; NEXT: there is a step s + 1, which has landed; MORE: and a step s + 2
+  // to load, spread between the MFMAs (an even one with the scales of two)
+  auto step = [&](int s, auto next_c, auto more_c, auto even_c) {
+    constexpr bool NEXT = decltype(next_c)::value, MORE = decltype(more_c)::value, EVEN = decltype(even_c)::value;
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0), which the barrier has seen to: tells the compiler
+    const uint32_t f = place(s + 1), q = scale_place(s + 1);
     __builtin_amdgcn_sched_barrier(0);
-    if constexpr (NEXT) read_w(st, SET ^ 1);
-    static_for<4>([&](auto mb_c) {
-      constexpr int mb = decltype(mb_c)::value;
-#pragma unroll
-      for (int nb = 0; nb < 2; ++nb) acc[mb][nb] = mfma32_mx4_lo(w[SET][nb][0], a[mb][0], acc[mb][nb], sw[SET][nb], sa[mb]);
+    static_for<16>([&](auto n_c) {
+      constexpr int n = decltype(n_c)::value, mb = n >> 2, kk = n & 3;
+      static_for<2>([&](auto nb_c) {
+        constexpr int nb = decltype(nb_c)::value;
+        acc[mb][nb] = mfma32_mx4<kk>(w[nb][kk], a[mb][kk], acc[mb][nb], sw[nb], sa[mb]);
+        if constexpr (NEXT && mb == 3) {
+          read_w(f, nb, kk);
+          if constexpr (kk == 3) read_ws(q, nb);
+        }
+      });
+      if constexpr (NEXT && kk == 3) read_a(f, q, mb);
       __builtin_amdgcn_sched_barrier(0);
-      if constexpr (MORE) {
-        load(t + kMxRing, mb_c);
-        if constexpr (mb == 3) load(t + kMxRing, std::integral_constant<int, 4>{});
-      }
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int nb = 0; nb < 2; ++nb) acc[mb][nb] = mfma32_mx4_hi(w[SET][nb][1], a[mb][1], acc[mb][nb], sw[SET][nb], sa[mb]);
-      if constexpr (NEXT) read_a(st, mb);
+      if constexpr (MORE && n < 8) load(s + 2, std::integral_constant<int, n>{});
+      if constexpr (MORE && EVEN && n == 8) load_scales((s + 2) >> 1);
       __builtin_amdgcn_sched_barrier(0);
     });
   };
-  // Before step t: every wave has read it, and step t + 1 has landed when only the
-  // later steps' loads (five each) are outstanding; its place takes step t + 4.
-  using Zero = std::integral_constant<int, 0>;
-  using One = std::integral_constant<int, 1>;
-  int t = 0;
   using No = std::false_type;
   using Yes = std::true_type;
-  for (; t + 5 < T; t += 2) {
-    dma_barrier<10>();
-    step(t, Zero{}, Yes{}, Yes{});
-    dma_barrier<10>();
-    step(t + 1, One{}, Yes{}, Yes{});
+  int s = 0;
+  for (; s + 3 < S; s += 2) {  // no branches inside: the compiler would move MFMAs across them
+    dma_barrier<0>();
+    step(s, Yes{}, Yes{}, Yes{});
+    dma_barrier<0>();
+    step(s + 1, Yes{}, Yes{}, No{});
   }
-  if (t + 2 < T) {
-    dma_barrier<10>();
-    step(t, Zero{}, Yes{}, No{});
-    dma_barrier<5>();
-    step(t + 1, One{}, Yes{}, No{});
+  if (s + 2 < S) {
+    dma_barrier<0>();
+    step(s, Yes{}, Yes{}, Yes{});
+    ++s;
   }
-  dma_barrier<0>();
-  step(T - 2, Zero{}, Yes{}, No{});
-  step(T - 1, One{}, No{}, No{});
+  if (s + 1 < S) {
+    dma_barrier<0>();
+    step(s, Yes{}, No{}, No{});
+  }
+  if ((p.K & 255) && h == 1) {
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb) {
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) w[nb][kk] = u32x4{0u, 0u, 0u, 0u};
+      sw[nb] = 0;
+    }
+#pragma unroll
+    for (int mb = 0; mb < 4; ++mb) sa[mb] = 0;
+  }
+  step(S - 1, No{}, No{}, No{});
 
   // lane: rows m0 + 128 wm + 32 mb + lr, columns n0 + 64 wn + 32 nb + 16 run + 8 h + (0..7)
   const int cl = n0 + 64 * wn + 8 * h;
