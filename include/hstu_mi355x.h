@@ -653,7 +653,7 @@ int hstu_rms_norm_bwd(int dtype, const void* dy, int64_t lddy, const void* h, in
  *           on a column range, ops/hstu_compute.py:140, but no product).
  */
 int hstu_gated_fwd(const void* x, int64_t ldx, const void* w_gate, int64_t ldg, const void* w_up, int64_t ldu, int M,
-                   int F, int D, int activation, void* h, int64_t ldh, hipStream_t stream);
+                   int F, int D, int activation, void* h, int64_t ldh, float* keep, hipStream_t stream);
 /*
  * The same from e4m3 x and weights (D % 128 == 0): g and u are multiplied by
  * x_scale (mode 0: one fp32 on the device, 1: [M]) and by their weight's scale
@@ -672,6 +672,19 @@ int hstu_gated_fwd_fp8(const void* x, int64_t ldx, const float* x_scale, int x_s
 int hstu_gated_bwd(const void* dh, int64_t lddh, const void* x, int64_t ldx, const void* w_gate, int64_t ldg,
                    const void* w_up, int64_t ldu, int M, int F, int D, int activation, void* dgu, int64_t lddgu,
                    hipStream_t stream);
+
+/*
+ * The same from [g | u] that hstu_gated_fwd kept: memory bound, 14 bytes a value,
+ * where computing them again costs 4 D operations.  F % 8 == 0.
+ */
+int hstu_gated_bwd_kept(const void* dh, int64_t lddh, const float* keep, int64_t rows, int F, int activation, void* dgu,
+                        int64_t lddgu, hipStream_t stream);
+/*
+ * out [D, 2F] = [w_gate^T | w_up^T] (bf16, F and D multiples of 64): the weight
+ * hstu_bf16_gemm takes for dx = dgu [Wg; Wu].
+ */
+int hstu_gated_transpose(const void* w_gate, int64_t ldg, const void* w_up, int64_t ldu, int F, int D, void* out,
+                         int64_t ldo, hipStream_t stream);
 
 /*
  * Microscaled 4-bit floating point (OCP MX, e2m1 values with one E8M0 scale for

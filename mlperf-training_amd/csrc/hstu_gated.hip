@@ -5,11 +5,12 @@
 //     silu    g s(g)
 //     gelu    g s(2 sqrt(2 / pi) (g + 0.044715 g^3))    (the tanh form)
 //     sigmoid s(g),                                      s(z) = 1 / (1 + e^-z)
-//   and the elementwise part of its backward from dh, g and u computed again:
+//   and the elementwise part of its backward, from dh and g and u in fp32, either
+//   computed again or kept by the forward:
 //     dg = dh u a'(g),  du = dh a(g),  written as [dg | du] [M, 2F].
 //
-// Both products of one output meet in one lane's accumulators, so nothing of
-// [M, F] but h (or [dg | du]) is written, and the values that meet are fp32:
+// Both products of one output meet in one lane's accumulators, so h (or
+// [dg | du]) is all that has to be written, and the values that meet are fp32:
 // the one rounding is that of the output.
 
 #include <hip/hip_runtime.h>
@@ -61,6 +62,7 @@ struct GatedParams {
   const uint16_t* dh;  // backward
   int64_t lddh;        // elements
   uint16_t* out;       // h [M, F], or [dg | du] [M, 2F]
+  float* keep;         // [g | u] [M, 2F] contiguous, or null
   int64_t ldo;         // elements
   int M, F, K;         // K = D in bytes
   int act;
@@ -84,6 +86,14 @@ __device__ __forceinline__ void gated_store(const GatedParams& p, int m, int n, 
       o0[j] = pack_bf16(a0 * u[2 * j], a1 * u[2 * j + 1]);
     }
     *(Vec*)(p.out + (int64_t)m * p.ldo + n) = o0;
+    if (p.keep) {
+      float* k = p.keep + (int64_t)m * 2 * p.F + n;
+#pragma unroll
+      for (int i = 0; i < N; i += 4) {
+        *(f32x4*)(k + i) = f32x4{g[i], g[i + 1], g[i + 2], g[i + 3]};
+        *(f32x4*)(k + p.F + i) = f32x4{u[i], u[i + 1], u[i + 2], u[i + 3]};
+      }
+    }
   } else {
     const Vec d = *(const Vec*)(p.dh + (int64_t)m * p.lddh + n);
 #pragma unroll
@@ -390,6 +400,75 @@ __global__ void __launch_bounds__(kDuoThreads, 2) gated_tile_fp8_kernel(GatedPar
   }
 }
 
+// ---------------------------------------------------------------- backward from kept g and u
+// Memory alone bounds it: 10 bytes in and 4 out a value.  A thread takes eight
+// consecutive columns.
+struct KeptArgs {
+  const uint16_t* dh;
+  const float* keep;
+  uint16_t* out;
+  int64_t lddh, ldo;  // elements
+  int64_t rows;
+  int F, act;
+};
+__global__ void __launch_bounds__(256) gated_kept_kernel(KeptArgs a) {
+  const int chunks = a.F / 8;
+  const int64_t total = a.rows * chunks;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t m = i / chunks;
+    const int n = (int)(i - m * chunks) * 8;
+    const float* k = a.keep + m * 2 * a.F + n;
+    const u32x4 d = *(const u32x4*)(a.dh + m * a.lddh + n);
+    const f32x4 gv[2] = {*(const f32x4*)k, *(const f32x4*)(k + 4)};
+    const f32x4 uv[2] = {*(const f32x4*)(k + a.F), *(const f32x4*)(k + a.F + 4)};
+    u32x4 o0, o1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t w = d[j];
+      const float d0 = bf16f(w & 0xffffu), d1 = __builtin_bit_cast(float, w & 0xffff0000u);
+      float a0, a1, b0, b1;
+      act<true>(a.act, gv[j >> 1][2 * (j & 1)], a0, b0);
+      act<true>(a.act, gv[j >> 1][2 * (j & 1) + 1], a1, b1);
+      o0[j] = pack_bf16(d0 * uv[j >> 1][2 * (j & 1)] * b0, d1 * uv[j >> 1][2 * (j & 1) + 1] * b1);
+      o1[j] = pack_bf16(d0 * a0, d1 * a1);
+    }
+    uint16_t* o = a.out + m * a.ldo + n;
+    *(u32x4*)o = o0;
+    *(u32x4*)(o + a.F) = o1;
+  }
+}
+
+// The weights side by side with the contraction index of dx = [dg | du] [Wg; Wu]
+// contiguous: out[d][f] = Wg[f][d], out[d][F + f] = Wu[f][d].  64 x 64 tiles through
+// LDS (pitch 66 elements: both the row and the column accesses spread over the
+// banks), 16-byte loads and stores; bound by memory.
+__global__ void __launch_bounds__(256) gated_transpose_kernel(const uint16_t* wg, const uint16_t* wu, int64_t ldg,
+                                                              int64_t ldu, int F, uint16_t* out, int64_t ldo) {
+  __shared__ uint16_t tile[64 * 66];
+  const int half = blockIdx.z, f0 = blockIdx.x * 64, d0 = blockIdx.y * 64;
+  const uint16_t* w = half ? wu : wg;
+  const int64_t ld = half ? ldu : ldg;
+  const int r = threadIdx.x >> 3, c = (threadIdx.x & 7) * 8;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const u32x4 v = *(const u32x4*)(w + (int64_t)(f0 + r + 32 * k) * ld + d0 + c);
+    uint32_t* t = (uint32_t*)(tile + (r + 32 * k) * 66 + c);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) t[j] = v[j];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    uint32_t v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t lo = tile[(c + 2 * j) * 66 + r + 32 * k], hi = tile[(c + 2 * j + 1) * 66 + r + 32 * k];
+      v[j] = lo | hi << 16;
+    }
+    *(u32x4*)(out + (int64_t)(d0 + r + 32 * k) * ldo + (int64_t)half * F + f0 + c) = u32x4{v[0], v[1], v[2], v[3]};
+  }
+}
+
 template <bool F8, bool BWD>
 int launch_gated(GatedParams p, hipStream_t stream) {
   p.tiles_m = (p.M + 127) / 128;
@@ -428,8 +507,10 @@ int check(const GatedParams& p, int es, int D, int kmul) {
 
 extern "C" int hstu_gated_fwd(const void* x, int64_t ldx, const void* w_gate, int64_t ldg, const void* w_up,
                               int64_t ldu, int M, int F, int D, int activation, void* h, int64_t ldh,
-                              hipStream_t stream) {
+                              float* keep, hipStream_t stream) {
   GatedParams p{};
+  p.keep = keep;
+  if ((uintptr_t)keep % 16) return HSTU_E_UNSUPPORTED;
   p.x = (const uint8_t*)x;
   p.wg = (const uint8_t*)w_gate;
   p.wu = (const uint8_t*)w_up;
@@ -501,4 +582,28 @@ extern "C" int hstu_gated_fwd_fp8(const void* x, int64_t ldx, const float* x_sca
   if (st != 0 || M == 0) return st;
   if (((uintptr_t)x_scale | (uintptr_t)gate_scale | (uintptr_t)up_scale) % 4) return HSTU_E_UNSUPPORTED;
   return launch_gated<true, false>(p, stream);
+}
+
+extern "C" int hstu_gated_bwd_kept(const void* dh, int64_t lddh, const float* keep, int64_t rows, int F, int activation,
+                                   void* dgu, int64_t lddgu, hipStream_t stream) {
+  if (rows < 0 || F <= 0 || lddh < F || lddgu < 2 * (int64_t)F || activation < kSilu || activation > kSigmoid)
+    return HSTU_E_BAD_ARG;
+  if (rows > 0 && (!dh || !keep || !dgu)) return HSTU_E_BAD_ARG;
+  if (F % 8 || ((uintptr_t)dh | (uintptr_t)keep | (uintptr_t)dgu) % 16 || lddh % 8 || lddgu % 8) return HSTU_E_UNSUPPORTED;
+  if (rows == 0) return 0;
+  const KeptArgs a{(const uint16_t*)dh, keep, (uint16_t*)dgu, lddh, lddgu, rows, F, activation};
+  const int64_t blocks = std::min<int64_t>((rows * (F / 8) + 255) / 256, 8192);
+  hipLaunchKernelGGL(gated_kept_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  return (int)hipGetLastError();
+}
+
+extern "C" int hstu_gated_transpose(const void* w_gate, int64_t ldg, const void* w_up, int64_t ldu, int F, int D, void* out,
+                                    int64_t ldo, hipStream_t stream) {
+  if (F <= 0 || D <= 0 || ldg < D || ldu < D || ldo < 2 * (int64_t)F || !w_gate || !w_up || !out) return HSTU_E_BAD_ARG;
+  if (F % 64 || D % 64 || D / 64 > 65535 || ((uintptr_t)w_gate | (uintptr_t)w_up | (uintptr_t)out) % 16 || ldg % 8 ||
+      ldu % 8 || ldo % 8)
+    return HSTU_E_UNSUPPORTED;
+  hipLaunchKernelGGL(gated_transpose_kernel, dim3(F / 64, D / 64, 2), dim3(256), 0, stream, (const uint16_t*)w_gate,
+                     (const uint16_t*)w_up, ldg, ldu, F, (uint16_t*)out, ldo);
+  return (int)hipGetLastError();
 }

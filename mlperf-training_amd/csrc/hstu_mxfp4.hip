@@ -341,8 +341,11 @@ __global__ void __launch_bounds__(kMxThreads, 2) mx_tile_kernel(MxParams p, int 
       });
       if constexpr (NEXT && kk == 3) read_a(f, q, mb);
       __builtin_amdgcn_sched_barrier(0);
-      if constexpr (MORE && n < 8) load(s + 2, std::integral_constant<int, n>{});
-      if constexpr (MORE && EVEN && n == 8) load_scales((s + 2) >> 1);
+      if constexpr (MORE && EVEN && n == 0) load_scales((s + 2) >> 1);
+      if constexpr (MORE && n < 4) {
+        load(s + 2, std::integral_constant<int, 2 * n>{});
+        load(s + 2, std::integral_constant<int, 2 * n + 1>{});
+      }
       __builtin_amdgcn_sched_barrier(0);
     });
   };

@@ -73,6 +73,8 @@ EXPORTED_SYMBOLS = (
     "hstu_gated_fwd",
     "hstu_gated_fwd_fp8",
     "hstu_gated_bwd",
+    "hstu_gated_bwd_kept",
+    "hstu_gated_transpose",
     "hstu_mxfp4_quantize",
     "hstu_mxfp4_dequantize",
     "hstu_mxfp4_gemm",
@@ -197,12 +199,14 @@ _SIGNATURES = {
         _i32,
         [_i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _vp, _i64, _i32, _vp, _i64, _vp, _i32, _vp, _i64, _vp],
     ),
-    "hstu_gated_fwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp]),
+    "hstu_gated_fwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _vp]),
     "hstu_gated_fwd_fp8": (
         _i32,
         [_vp, _i64, _vp, _i32, _vp, _i64, _vp, _i32, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _vp],
     ),
     "hstu_gated_bwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp]),
+    "hstu_gated_bwd_kept": (_i32, [_vp, _i64, _vp, _i64, _i32, _i32, _vp, _i64, _vp]),
+    "hstu_gated_transpose": (_i32, [_vp, _i64, _vp, _i64, _i32, _i32, _vp, _i64, _vp]),
     "hstu_mxfp4_quantize": (_i32, [_i32, _vp, _i64, _i64, _i32, _vp, _vp, _vp]),
     "hstu_mxfp4_dequantize": (_i32, [_vp, _vp, _i64, _i32, _i32, _vp, _i64, _vp]),
     "hstu_mxfp4_gemm": (

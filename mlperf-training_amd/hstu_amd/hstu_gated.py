@@ -13,9 +13,9 @@ of one product, not the product of two.
   ``fp8.quantize_e4m3_rows``' output), D a multiple of 128;
 * ``gated_linear_fwd`` / ``gated_linear_bwd``: the two directions.
 
-The backward keeps x and the weights only: it computes g and u again, in fp32,
-and writes [dg | du], whose products with the weights and with x are the bf16
-projection GEMM and the token-axis weight gradient.
+The backward takes g and u in fp32, kept by the forward or computed again
+(``recompute``), and writes [dg | du], whose products with the weights and with
+x are the bf16 projection GEMM and the token-axis weight gradient.
 """
 
 from __future__ import annotations
@@ -70,9 +70,9 @@ def _check(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, dtype: tor
         raise NotImplementedError("x: fewer than 2^31 rows")
 
 
-def gated_linear_fwd(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = "silu"
-                     ) -> torch.Tensor:
-    """h [.., F] in bf16."""
+def gated_linear_fwd(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = "silu",
+                     keep: bool = False):
+    """h [.., F] in bf16; with ``keep`` (h, gu): gu fp32 [rows, 2F] holds g and u for ``gated_linear_bwd``."""
     act = _act(activation)
     x, w_gate, w_up = x.detach(), w_gate.detach(), w_up.detach()
     _check(x, w_gate, w_up, torch.bfloat16, 256)
@@ -80,18 +80,22 @@ def gated_linear_fwd(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, 
     x2, g, u = _rows2d(x), _rows2d(w_gate), _rows2d(w_up)
     M = x2.shape[0]
     h = torch.empty((M, F), dtype=torch.bfloat16, device=x.device)
+    gu = torch.empty((M, 2 * F), dtype=torch.float32, device=x.device) if keep else None
     if M > 0:
         with _lib.on_device(x):
             st = _lib.fn("hstu_gated_fwd")(x2.data_ptr(), _ld(x2), g.data_ptr(), _ld(g), u.data_ptr(), _ld(u), M, F, D,
-                                           act, h.data_ptr(), F, _lib.stream(x))
+                                           act, h.data_ptr(), F, _lib.ptr(gu), _lib.stream(x))
         _lib.check(st, "hstu_gated_fwd")
-    return h.view(x.shape[:-1] + (F,))
+    h = h.view(x.shape[:-1] + (F,))
+    return (h, gu) if keep else h
 
 
 def gated_linear_bwd(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
-                     activation: str = "silu", need_dx: bool = True, need_dw: bool = True
+                     activation: str = "silu", need_dx: bool = True, need_dw: bool = True,
+                     gu: Optional[torch.Tensor] = None
                      ) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor], Optional[torch.Tensor]]:
-    """(dx, dw_gate, dw_up) in bf16; None for what is not needed."""
+    """(dx, dw_gate, dw_up) in bf16; None for what is not needed.  ``gu``: what
+    ``gated_linear_fwd(keep=True)`` kept; without it g and u are computed again."""
     act = _act(activation)
     dh, x, w_gate, w_up = dh.detach(), x.detach(), w_gate.detach(), w_up.detach()
     _check(x, w_gate, w_up, torch.bfloat16, 256)
@@ -100,21 +104,40 @@ def gated_linear_bwd(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_
         raise ValueError(f"dh {tuple(dh.shape)} {dh.dtype}; expected {tuple(x.shape[:-1] + (F,))} bf16 on {x.device}")
     x2, g, u, d2 = _rows2d(x), _rows2d(w_gate), _rows2d(w_up), _rows2d(dh)
     M = x2.shape[0]
+    if gu is not None and (gu.shape != (M, 2 * F) or gu.dtype != torch.float32 or not gu.is_contiguous()
+                           or gu.device != x.device):
+        raise ValueError(f"gu {tuple(gu.shape)} {gu.dtype}; expected contiguous fp32 [{M}, {2 * F}] on {x.device}")
     if M == 0:
         dw = torch.zeros((2 * F, D), dtype=torch.bfloat16, device=x.device)
         return torch.empty_like(x) if need_dx else None, dw[:F] if need_dw else None, dw[F:] if need_dw else None
     dgu = torch.empty((M, 2 * F), dtype=torch.bfloat16, device=x.device)
     with _lib.on_device(x):
-        st = _lib.fn("hstu_gated_bwd")(d2.data_ptr(), _ld(d2), x2.data_ptr(), _ld(x2), g.data_ptr(), _ld(g),
-                                       u.data_ptr(), _ld(u), M, F, D, act, dgu.data_ptr(), 2 * F, _lib.stream(x))
-        _lib.check(st, "hstu_gated_bwd")
+        stream = _lib.stream(x)
+        if gu is not None:
+            st = _lib.fn("hstu_gated_bwd_kept")(d2.data_ptr(), _ld(d2), gu.data_ptr(), M, F, act, dgu.data_ptr(),
+                                                2 * F, stream)
+            _lib.check(st, "hstu_gated_bwd_kept")
+        else:
+            st = _lib.fn("hstu_gated_bwd")(d2.data_ptr(), _ld(d2), x2.data_ptr(), _ld(x2), g.data_ptr(), _ld(g),
+                                           u.data_ptr(), _ld(u), M, F, D, act, dgu.data_ptr(), 2 * F, stream)
+            _lib.check(st, "hstu_gated_bwd")
         dx = dg = du = None
         if need_dx:  # the contraction runs over both halves of dgu: the weights side by side, transposed
-            dx = bf16_gemm(dgu, torch.cat((g, u)).t().contiguous()).view(x.shape)
+            wt = torch.empty((D, 2 * F), dtype=torch.bfloat16, device=x.device)
+            st = _lib.fn("hstu_gated_transpose")(g.data_ptr(), _ld(g), u.data_ptr(), _ld(u), F, D, wt.data_ptr(), 2 * F,
+                                                 stream)
+            _lib.check(st, "hstu_gated_transpose")
+            dx = bf16_gemm(dgu, wt).view(x.shape)
         if need_dw:
             dw = wgrad(dgu, x2, split=_wgrad_split(M, 2 * F, D))
             dg, du = dw[:F], dw[F:]
     return dx, dg, du
+
+
+# Keeping g and u costs 16 bytes of memory traffic a value (written and read in
+# fp32), computing them again 4 D operations: equal near D = 900 at this card's
+# rates.  Measured (us a training step, kept / computed again): KEPT_FIGURES
+RECOMPUTE_BELOW = 1024
 
 
 def _wgrad_split(T: int, n1: int, n2: int) -> Optional[int]:
@@ -125,26 +148,38 @@ def _wgrad_split(T: int, n1: int, n2: int) -> Optional[int]:
 
 
 class GatedLinearFunction(torch.autograd.Function):
-    """Autograd of the gated projection: keeps x and the weights, not g, u or h."""
+    """Autograd of the gated projection: keeps x, the weights and, with ``keep``, g and u in fp32."""
 
     @staticmethod
-    def forward(ctx, x, w_gate, w_up, activation):
-        ctx.save_for_backward(x, w_gate, w_up)
+    def forward(ctx, x, w_gate, w_up, activation, keep):
         ctx.activation = activation
-        return gated_linear_fwd(x, w_gate, w_up, activation)
+        if not keep:
+            ctx.save_for_backward(x, w_gate, w_up, None)
+            return gated_linear_fwd(x, w_gate, w_up, activation)
+        h, gu = gated_linear_fwd(x, w_gate, w_up, activation, keep=True)
+        ctx.save_for_backward(x, w_gate, w_up, gu)
+        return h
 
     @staticmethod
     def backward(ctx, dh):
-        x, w_gate, w_up = ctx.saved_tensors
-        need_x, need_g, need_u, _ = ctx.needs_input_grad
-        dx, dg, du = gated_linear_bwd(dh, x, w_gate, w_up, ctx.activation, need_x, need_g or need_u)
-        return dx, dg if need_g else None, du if need_u else None, None
+        x, w_gate, w_up, gu = ctx.saved_tensors
+        need_x, need_g, need_u = ctx.needs_input_grad[:3]
+        dx, dg, du = gated_linear_bwd(dh, x, w_gate, w_up, ctx.activation, need_x, need_g or need_u, gu)
+        return dx, dg if need_g else None, du if need_u else None, None, None
 
 
-def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = "silu") -> torch.Tensor:
+def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = "silu",
+                 recompute: Optional[bool] = None) -> torch.Tensor:
     """a(x @ w_gate^T) * (x @ w_up^T): x [.., D], weights [F, D], h [.., F], bf16.
-    Differentiable in x and both weights."""
-    return GatedLinearFunction.apply(x, w_gate, w_up, activation)
+    Differentiable in x and both weights.  ``recompute``: the backward computes g
+    and u again (nothing but x and the weights is kept) instead of keeping them
+    in fp32, 8 bytes a value of h; None: where that is the faster way (D < 1024).
+    The gradients are the same bytes."""
+    if not (torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad)):
+        return gated_linear_fwd(x, w_gate, w_up, activation)
+    if recompute is None:
+        recompute = x.shape[-1] < RECOMPUTE_BELOW
+    return GatedLinearFunction.apply(x, w_gate, w_up, activation, not recompute)
 
 
 def _scale(name: str, s: torch.Tensor, n: int, x: torch.Tensor) -> Tuple[torch.Tensor, int]:

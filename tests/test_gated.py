@@ -114,6 +114,30 @@ def test_e4m3(hip_lib, M, D, F, modes):
 
 
 @gpu
+@pytest.mark.parametrize("name", ACTS)
+@pytest.mark.parametrize("M,D,F", [(1, 256, 128), (40, 512, 384), (130, 1024, 256), (1030, 256, 640)])
+def test_kept_and_computed_again_give_the_same_bytes(hip_lib, M, D, F, name):
+    import hstu_amd
+
+    x, dh = rnd((M, D), 31).to(DEV).requires_grad_(True), rnd((M, F), 32).to(DEV)
+    wg, wu = (w.requires_grad_(True) for w in weights(F, D, 3))
+    both = []
+    for recompute in (True, False, None):
+        h = hstu_amd.gated_linear(x, wg, wu, name, recompute=recompute)
+        both.append((h.detach(),) + torch.autograd.grad(h, (x, wg, wu), dh))
+    for other in both[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(both[0], other))
+    h, gu = hstu_amd.gated_linear_fwd(x, wg, wu, name, keep=True)
+    assert torch.equal(h, both[0][0]) and gu.shape == (M, 2 * F) and gu.dtype == torch.float32
+    n = (D + 16) * ULP
+    for part, w in ((gu[:, :F], wg), (gu[:, F:], wu)):
+        want = x.detach().double() @ w.detach().double().t()
+        within(part, want, n * (x.detach().double().abs() @ w.detach().double().abs().t()), "kept")
+    with torch.no_grad():
+        assert torch.equal(hstu_amd.gated_linear(x, wg, wu, name), h)
+
+
+@gpu
 def test_large_arguments(hip_lib):
     """Gates far out on both sides: silu, gelu and sigmoid saturate without NaN, values and derivatives."""
     import hstu_amd
@@ -218,7 +242,7 @@ def test_rows_past_the_last_are_left(hip_lib):
         x = rnd((M, D), 13).to(DEV)
         out = torch.full((M + 140, F + 8), 7.0, dtype=torch.bfloat16, device=DEV)
         st = lib.fn("hstu_gated_fwd")(x.data_ptr(), D, wg.data_ptr(), D, wu.data_ptr(), D, M, F, D, 0, out.data_ptr(),
-                                      F + 8, lib.stream(x))
+                                      F + 8, None, lib.stream(x))
         assert st == 0
         assert (out[M:] == 7).all() and (out[:, F:] == 7).all()
         assert not (out[:M, :F] == 7).all()
@@ -306,13 +330,13 @@ def test_c_entry_refusals():
     P = 64  # a stand-in address, never read
     fwd, bwd, f8 = (lib.fn("hstu_gated_" + n) for n in ("fwd", "bwd", "fwd_fp8"))
 
-    def f(x=P, ldx=256, g=P, ldg=256, u=P, ldu=256, M=4, F=128, D=256, act=0, h=P, ldh=128):
-        return fwd(x, ldx, g, ldg, u, ldu, M, F, D, act, h, ldh, None)
+    def f(x=P, ldx=256, g=P, ldg=256, u=P, ldu=256, M=4, F=128, D=256, act=0, h=P, ldh=128, keep=None):
+        return fwd(x, ldx, g, ldg, u, ldu, M, F, D, act, h, ldh, keep, None)
 
     for bad in (dict(M=-1), dict(F=0), dict(D=0), dict(act=3), dict(act=-1), dict(ldx=255), dict(ldg=8), dict(ldu=8),
                 dict(ldh=127), dict(x=None), dict(g=None), dict(u=None), dict(h=None)):
         assert f(**bad) == lib.HSTU_E_BAD_ARG, bad
-    for bad in (dict(F=64), dict(D=128), dict(x=72), dict(ldx=260), dict(h=72), dict(ldh=132)):
+    for bad in (dict(F=64), dict(D=128), dict(x=72), dict(ldx=260), dict(h=72), dict(ldh=132), dict(keep=72)):
         assert f(**bad) == lib.HSTU_E_UNSUPPORTED, bad
     assert f(M=0) == 0
 
@@ -330,3 +354,22 @@ def test_c_entry_refusals():
     for bad in (dict(xs=None), dict(gs=None), dict(us=None), dict(D=256)):
         assert e(**bad) == lib.HSTU_E_BAD_ARG, bad
     assert e(D=64) == lib.HSTU_E_UNSUPPORTED and e(xs=65) == lib.HSTU_E_UNSUPPORTED
+    kept, tr = lib.fn("hstu_gated_bwd_kept"), lib.fn("hstu_gated_transpose")
+
+    def k(dh=P, lddh=128, keep=P, rows=4, F=128, act=0, out=P, ldo=256):
+        return kept(dh, lddh, keep, rows, F, act, out, ldo, None)
+
+    for bad in (dict(dh=None), dict(keep=None), dict(out=None), dict(rows=-1), dict(F=0), dict(act=3), dict(lddh=100),
+                dict(ldo=255)):
+        assert k(**bad) == lib.HSTU_E_BAD_ARG, bad
+    for bad in (dict(F=100), dict(dh=72), dict(keep=72), dict(out=72), dict(lddh=132), dict(ldo=260)):
+        assert k(**bad) == lib.HSTU_E_UNSUPPORTED, bad
+    assert k(rows=0) == 0
+
+    def t(g=P, ldg=256, u=P, ldu=256, F=128, D=256, out=P, ldo=256):
+        return tr(g, ldg, u, ldu, F, D, out, ldo, None)
+
+    for bad in (dict(g=None), dict(u=None), dict(out=None), dict(ldg=255), dict(ldu=100), dict(ldo=200), dict(F=0), dict(D=0)):
+        assert t(**bad) == lib.HSTU_E_BAD_ARG, bad
+    for bad in (dict(F=96), dict(D=200), dict(g=72), dict(out=72), dict(ldg=260), dict(ldo=260)):
+        assert t(**bad) == lib.HSTU_E_UNSUPPORTED, bad
