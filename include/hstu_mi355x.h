@@ -646,8 +646,9 @@ int hstu_rms_norm_bwd(int dtype, const void* dy, int64_t lddy, const void* h, in
  * (the contraction index contiguous), h [M, F], all bf16, fp32 accumulation,
  * rounded once; ld* in elements.  activation: 0 silu, 1 gelu (tanh form),
  * 2 sigmoid.  D % 256 == 0, F % 128 == 0, any M; rows 16-byte aligned and less
- * than 2^24 bytes apart.  Rows
- * past M are not touched.
+ * than 2^24 bytes apart.  Rows past M are not touched.  keep: NULL, or fp32
+ * [M, 2F] contiguous (16-byte aligned), which receives [g | u] for
+ * hstu_gated_bwd_kept.
  * Replaces: two projections of ops/triton/triton_addmm.py:1756-1767 and an
  *           elementwise pass over both (the reference's UVQK projection has SiLU
  *           on a column range, ops/hstu_compute.py:140, but no product).
@@ -711,6 +712,17 @@ int hstu_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, i
 int hstu_mxfp4_gemm(const void* A, int64_t lda, const void* a_scale, int64_t ldas, const void* W, int64_t ldw,
                     const void* w_scale, int64_t ldws, const void* bias, const void* residual, int64_t ldr, void* C,
                     int64_t ldc, int M, int N, int K, hipStream_t stream);
+
+/*
+ * The same product from bf16 x [M, K] (ldx in elements, rows 16-byte aligned),
+ * quantised on the way, for few rows: the codes and scales, and so the bytes of
+ * C, are those of hstu_mxfp4_quantize and hstu_mxfp4_gemm up to the order of the sum.
+ * Every workgroup quantises its rows of x itself, so this is for few rows (16);
+ * any M is served.
+ */
+int hstu_mxfp4_linear_rows(const void* x, int64_t ldx, const void* W, int64_t ldw, const void* w_scale, int64_t ldws,
+                           const void* bias, const void* residual, int64_t ldr, void* C, int64_t ldc, int M, int N,
+                           int K, hipStream_t stream);
 
 #ifdef __cplusplus
 }

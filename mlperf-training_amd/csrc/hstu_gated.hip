@@ -111,16 +111,18 @@ __device__ __forceinline__ void gated_store(const GatedParams& p, int m, int n, 
   }
 }
 
-// Row form: a workgroup owns 16 columns and 16 MB rows, its four waves split
-// the contraction and meet in LDS in wave order.  Operands go from memory to
-// registers as the MFMA takes them: lane (li, q) reads 16 (bf16) or 32 (e4m3)
-// contiguous bytes of row li.
-template <bool F8, int MB, bool BWD>
-__global__ void __launch_bounds__(kThreads) gated_rows_kernel(GatedParams p) {
+// ---------------------------------------------------------------- row form
+// Few rows: the weights' bytes are the time.  A workgroup owns 16 columns and 16 MB
+// rows; its WAVES waves take one contiguous piece of the contraction each, with the
+// operands going from memory to registers as the MFMA takes them (lane (li, q):
+// 16 or 32 contiguous bytes of row li), and meet in LDS: wave b sums row block b
+// over the waves in order.
+template <bool F8, int MB, int WAVES, bool BWD>
+__global__ void __launch_bounds__(64 * WAVES) gated_rows_kernel(GatedParams p) {
   constexpr int STEP = F8 ? 128 : 64;  // bytes of a row per MFMA
   constexpr int LB = STEP / 4;         // bytes of a lane
-  __shared__ f32x4 part[3][2 * MB][64];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, li = lane & 15, q = lane >> 4;
+  __shared__ f32x4 part[WAVES][2 * MB][64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, q = lane >> 4;
   const int nt = p.F / 16, mt = blockIdx.x / nt, n0 = (blockIdx.x - mt * nt) * 16, m0 = mt * 16 * MB;
   const uint8_t* gp = p.wg + (int64_t)(n0 + li) * p.ldwg + LB * q;
   const uint8_t* up = p.wu + (int64_t)(n0 + li) * p.ldwu + LB * q;
@@ -130,8 +132,10 @@ __global__ void __launch_bounds__(kThreads) gated_rows_kernel(GatedParams p) {
   f32x4 ag[MB], au[MB];
 #pragma unroll
   for (int b = 0; b < MB; ++b) ag[b] = au[b] = zero4();
+  const int steps = p.K / STEP, each = (steps + WAVES - 1) / WAVES;
+  const int k_end = min((wave + 1) * each, steps) * STEP;
 #pragma unroll 4
-  for (int k = wave * STEP; k < p.K; k += 4 * STEP) {
+  for (int k = wave * each * STEP; k < k_end; k += STEP) {
     if constexpr (F8) {
       const i32x8 g = cat8(*(const u32x4*)(gp + k), *(const u32x4*)(gp + k + 16));
       const i32x8 u = cat8(*(const u32x4*)(up + k), *(const u32x4*)(up + k + 16));
@@ -151,31 +155,27 @@ __global__ void __launch_bounds__(kThreads) gated_rows_kernel(GatedParams p) {
       }
     }
   }
-  if (wave > 0) {
 #pragma unroll
-    for (int b = 0; b < MB; ++b) part[wave - 1][2 * b][lane] = ag[b], part[wave - 1][2 * b + 1][lane] = au[b];
-  }
+  for (int b = 0; b < MB; ++b) part[wave][2 * b][lane] = ag[b], part[wave][2 * b + 1][lane] = au[b];
   __syncthreads();
-  if (wave > 0) return;
+  if (wave >= MB) return;
+  const int b = wave, m = m0 + 16 * b + li, n = n0 + 4 * q;
+  if (m >= p.M) return;
+  f32x4 tg = part[0][2 * b][lane], tu = part[0][2 * b + 1][lane];
 #pragma unroll
-  for (int b = 0; b < MB; ++b) {
+  for (int w = 1; w < WAVES; ++w) tg += part[w][2 * b][lane], tu += part[w][2 * b + 1][lane];
+  float g[4], u[4];
+  const float xs = F8 ? p.xs[p.xs_row ? m : 0] : 1.f;
 #pragma unroll
-    for (int w = 0; w < 3; ++w) ag[b] += part[w][2 * b][lane], au[b] += part[w][2 * b + 1][lane];
-    const int m = m0 + 16 * b + li, n = n0 + 4 * q;
-    if (m >= p.M) continue;
-    float g[4], u[4];
-    const float xs = F8 ? p.xs[p.xs_row ? m : 0] : 1.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      g[e] = ag[b][e];
-      u[e] = au[b][e];
-      if constexpr (F8) {
-        g[e] *= xs * p.gs[p.gs_row ? n + e : 0];
-        u[e] *= xs * p.us[p.us_row ? n + e : 0];
-      }
+  for (int e = 0; e < 4; ++e) {
+    g[e] = tg[e];
+    u[e] = tu[e];
+    if constexpr (F8) {
+      g[e] *= xs * p.gs[p.gs_row ? n + e : 0];
+      u[e] *= xs * p.us[p.us_row ? n + e : 0];
     }
-    gated_store<BWD, 4>(p, m, n, g, u);
   }
+  gated_store<BWD, 4>(p, m, n, g, u);
 }
 
 // ---------------------------------------------------------------- tile form, bf16
@@ -483,9 +483,10 @@ int launch_gated(GatedParams p, hipStream_t stream) {
   const int64_t tiles = ((int64_t)p.M + 16 * mb - 1) / (16 * mb) * (p.F / 16);
   if (tiles >= ((int64_t)1 << 31)) return HSTU_E_UNSUPPORTED;
   const dim3 grid((unsigned)tiles);
-  if (mb == 1) hipLaunchKernelGGL((gated_rows_kernel<F8, 1, BWD>), grid, dim3(kThreads), 0, stream, p);
-  else if (mb == 2) hipLaunchKernelGGL((gated_rows_kernel<F8, 2, BWD>), grid, dim3(kThreads), 0, stream, p);
-  else hipLaunchKernelGGL((gated_rows_kernel<F8, 4, BWD>), grid, dim3(kThreads), 0, stream, p);
+  constexpr int W = 8;
+  if (mb == 1) hipLaunchKernelGGL((gated_rows_kernel<F8, 1, W, BWD>), grid, dim3(64 * W), 0, stream, p);
+  else if (mb == 2) hipLaunchKernelGGL((gated_rows_kernel<F8, 2, W, BWD>), grid, dim3(64 * W), 0, stream, p);
+  else hipLaunchKernelGGL((gated_rows_kernel<F8, 4, W, BWD>), grid, dim3(64 * W), 0, stream, p);
   return (int)hipGetLastError();
 }
 

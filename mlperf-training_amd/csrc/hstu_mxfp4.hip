@@ -53,6 +53,39 @@ __device__ __forceinline__ uint32_t mx_encode8(const float (&v)[8], uint32_t& by
   return w;
 }
 
+// A whole block, 32 bf16 of one lane, the same way.
+__device__ __forceinline__ void mx_encode32(const u32x4 (&v)[4], u32x4& codes, uint32_t& byte) {
+  // the largest magnitude of both halves of the words at once, as 16-bit integers
+  uint32_t lo = 0, hi = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t x = v[j][e];
+      lo = max(lo, x & 0x7fffu);
+      hi = max(hi, x & 0x7fff0000u);
+    }
+  const uint32_t ex = max(lo >> 7, hi >> 23);
+  byte = ex == 255u ? 255u : ex >= 2u ? ex - 2u : 0u;
+  const float up = ex == 255u ? 0.f : __builtin_bit_cast(float, (254u - byte) << 23);  // 2^-E
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t w = 0;
+    float t[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t x = v[j][e];
+      t[2 * e] = bf16f(x & 0xffffu) * up;
+      t[2 * e + 1] = __builtin_bit_cast(float, x & 0xffff0000u) * up;
+    }
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[0], t[1], 1.f, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[2], t[3], 1.f, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[4], t[5], 1.f, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[6], t[7], 1.f, 3);
+    codes[j] = w;
+  }
+}
+
 struct QuantArgs {
   const uint8_t* x;
   int64_t ldx;  // bytes
@@ -161,12 +194,16 @@ __device__ __forceinline__ void mx_store4(const MxParams& p, int m, int n, f32x4
   *(u32x2*)(p.C + (int64_t)m * p.ldc + n) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
 }
 
-// Row form: 16 columns and 16 MB rows a workgroup, its four waves split the
-// contraction and meet in LDS in wave order.
-template <int MB>
-__global__ void __launch_bounds__(kThreads) mx_rows_kernel(MxParams p) {
-  __shared__ f32x4 part[3][MB][64];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, li = lane & 15, q = lane >> 4;
+// Row form, for few rows, where the weights' bytes and the calls are the time: 16
+// columns and 16 MB rows a workgroup, whose WAVES waves take one contiguous piece
+// of the contraction each, operands going from memory to registers as the MFMA takes
+// them, and meet in LDS: wave b sums row block b over the waves in order.
+// QUANT: A is bf16 and quantised here: lane (li, q) of a step holds the 32 values of
+// its own block, so the block's scale and codes need no other lane.
+template <int MB, int WAVES, bool QUANT>
+__global__ void __launch_bounds__(64 * WAVES) mx_rows_kernel(MxParams p) {
+  __shared__ f32x4 part[WAVES][MB][64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, q = lane >> 4;
   const int nt = p.N / 16, mt = blockIdx.x / nt, n0 = (blockIdx.x - mt * nt) * 16, m0 = mt * 16 * MB;
   const uint8_t* wp = p.W + (int64_t)(n0 + li) * p.ldw + 16 * q;
   const uint8_t* wsp = p.ws + (int64_t)(n0 + li) * p.ldws + q;
@@ -175,33 +212,41 @@ __global__ void __launch_bounds__(kThreads) mx_rows_kernel(MxParams p) {
 #pragma unroll
   for (int b = 0; b < MB; ++b) {
     const int m = min(m0 + 16 * b + li, p.M - 1);
-    ap[b] = p.A + (int64_t)m * p.lda + 16 * q;
-    asp[b] = p.as + (int64_t)m * p.ldas + q;
+    ap[b] = p.A + (int64_t)m * p.lda + (QUANT ? 64 : 16) * q;
+    asp[b] = QUANT ? nullptr : p.as + (int64_t)m * p.ldas + q;
   }
   f32x4 acc[MB];
 #pragma unroll
   for (int b = 0; b < MB; ++b) acc[b] = zero4();
-  const int steps = p.K / 128;
+  const int steps = p.K / 128, each = (steps + WAVES - 1) / WAVES, s_end = min((wave + 1) * each, steps);
 #pragma unroll 4
-  for (int s = wave; s < steps; s += 4) {
+  for (int s = wave * each; s < s_end; ++s) {
     const u32x4 w = *(const u32x4*)(wp + 64 * s);
     const int ws = wsp[4 * s];
 #pragma unroll
-    for (int b = 0; b < MB; ++b) acc[b] = mfma_mx4(w, *(const u32x4*)(ap[b] + 64 * s), acc[b], ws, asp[b][4 * s]);
+    for (int b = 0; b < MB; ++b) {
+      if constexpr (QUANT) {
+        const u32x4* x = (const u32x4*)(ap[b] + 256 * s);
+        const u32x4 v[4] = {x[0], x[1], x[2], x[3]};
+        u32x4 codes;
+        uint32_t byte;
+        mx_encode32(v, codes, byte);
+        acc[b] = mfma_mx4(w, codes, acc[b], ws, (int)byte);
+      } else {
+        acc[b] = mfma_mx4(w, *(const u32x4*)(ap[b] + 64 * s), acc[b], ws, asp[b][4 * s]);
+      }
+    }
   }
-  if (wave > 0) {
 #pragma unroll
-    for (int b = 0; b < MB; ++b) part[wave - 1][b][lane] = acc[b];
-  }
+  for (int b = 0; b < MB; ++b) part[wave][b][lane] = acc[b];
   __syncthreads();
-  if (wave > 0) return;
+  if (wave >= MB) return;
+  const int m = m0 + 16 * wave + li;
+  if (m >= p.M) return;
+  f32x4 t = part[0][wave][lane];
 #pragma unroll
-  for (int b = 0; b < MB; ++b) {
-#pragma unroll
-    for (int w = 0; w < 3; ++w) acc[b] += part[w][b][lane];
-    const int m = m0 + 16 * b + li;
-    if (m < p.M) mx_store4(p, m, n0 + 4 * q, acc[b]);
-  }
+  for (int w = 1; w < WAVES; ++w) t += part[w][wave][lane];
+  mx_store4(p, m, n0 + 4 * q, t);
 }
 
 // Tile form: 256 x 256 outputs a workgroup of 8 waves (2 x 4 of 128 x 64, 4 x 2
@@ -453,21 +498,40 @@ extern "C" int hstu_mxfp4_dequantize(const void* codes, const void* scales, int6
   return (int)hipGetLastError();
 }
 
+namespace {
+int check_product(const MxParams& p, bool quant) {
+  if (p.M < 0 || p.N <= 0 || p.K <= 0 || p.ldw < p.K / 2 || p.ldws < p.K / 32 || p.ldc < p.N || (p.resid && p.ldr < p.N) ||
+      (quant ? p.lda < 2 * (int64_t)p.K : p.lda < p.K / 2 || p.ldas < p.K / 32))
+    return HSTU_E_BAD_ARG;
+  if (p.M > 0 && (!p.A || !p.W || !p.ws || !p.C || (!quant && !p.as))) return HSTU_E_BAD_ARG;
+  if (p.N % 16 || p.K % 128) return HSTU_E_UNSUPPORTED;
+  if (((uintptr_t)p.A | (uintptr_t)p.W | (uintptr_t)p.C | (uintptr_t)p.resid | (uintptr_t)p.bias) % 16 ||
+      (p.lda | p.ldw) % 16 || ((uintptr_t)p.as | (uintptr_t)p.ws) % 4 || (p.ldas | p.ldws) % 4 || p.ldc % 8 ||
+      (p.resid && p.ldr % 8))
+    return HSTU_E_UNSUPPORTED;
+  return 0;
+}
+template <bool QUANT>
+int launch_rows(const MxParams& p, hipStream_t stream) {
+  const int mb = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
+  const int64_t tiles = ((int64_t)p.M + 16 * mb - 1) / (16 * mb) * (p.N / 16);
+  if (tiles >= ((int64_t)1 << 31)) return HSTU_E_UNSUPPORTED;
+  constexpr int W = 8;
+  const dim3 grid((unsigned)tiles), block(64 * W);
+  if (mb == 1) hipLaunchKernelGGL((mx_rows_kernel<1, W, QUANT>), grid, block, 0, stream, p);
+  else if (mb == 2) hipLaunchKernelGGL((mx_rows_kernel<2, W, QUANT>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((mx_rows_kernel<4, W, QUANT>), grid, block, 0, stream, p);
+  return (int)hipGetLastError();
+}
+}  // namespace
+
 extern "C" int hstu_mxfp4_gemm(const void* A, int64_t lda, const void* a_scale, int64_t ldas, const void* W,
                                int64_t ldw, const void* w_scale, int64_t ldws, const void* bias, const void* residual,
                                int64_t ldr, void* C, int64_t ldc, int M, int N, int K, hipStream_t stream) {
-  if (M < 0 || N <= 0 || K <= 0 || lda < K / 2 || ldw < K / 2 || ldas < K / 32 || ldws < K / 32 || ldc < N ||
-      (residual && ldr < N))
-    return HSTU_E_BAD_ARG;
-  if (M > 0 && (!A || !a_scale || !W || !w_scale || !C)) return HSTU_E_BAD_ARG;
-  if (N % 16 || K % 128) return HSTU_E_UNSUPPORTED;
-  if (((uintptr_t)A | (uintptr_t)W | (uintptr_t)C | (uintptr_t)residual) % 16 || (lda | ldw) % 16 ||
-      ((uintptr_t)a_scale | (uintptr_t)w_scale) % 4 || (ldas | ldws) % 4 || ldc % 8 || (residual && ldr % 8) ||
-      (uintptr_t)bias % 16)
-    return HSTU_E_UNSUPPORTED;
-  if (M == 0) return 0;
   MxParams p{(const uint8_t*)A, (const uint8_t*)W, (const uint8_t*)a_scale, (const uint8_t*)w_scale, lda, ldw, ldas,
              ldws, (const uint16_t*)bias, (const uint16_t*)residual, (uint16_t*)C, ldr, ldc, M, N, K};
+  const int st = check_product(p, false);
+  if (st != 0 || M == 0) return st;
   const int64_t tiles_m = ((int64_t)M + kMxTile - 1) / kMxTile, tiles_n = (N + kMxTile - 1) / kMxTile;
   if (M > 64 && tiles_m * tiles_n < (1 << 30) && (int64_t)kMxTile * std::max(lda, ldw) < ((int64_t)1 << 31)) {
     hipError_t e = set_mx_lds((const void*)mx_tile_kernel);
@@ -477,12 +541,15 @@ extern "C" int hstu_mxfp4_gemm(const void* A, int64_t lda, const void* a_scale, 
                        (int)tiles_n, per_xcd);
     return (int)hipGetLastError();
   }
-  const int mb = M <= 16 ? 1 : M <= 32 ? 2 : 4;
-  const int64_t tiles = ((int64_t)M + 16 * mb - 1) / (16 * mb) * (N / 16);
-  if (tiles >= ((int64_t)1 << 31)) return HSTU_E_UNSUPPORTED;
-  const dim3 grid((unsigned)tiles);
-  if (mb == 1) hipLaunchKernelGGL((mx_rows_kernel<1>), grid, dim3(kThreads), 0, stream, p);
-  else if (mb == 2) hipLaunchKernelGGL((mx_rows_kernel<2>), grid, dim3(kThreads), 0, stream, p);
-  else hipLaunchKernelGGL((mx_rows_kernel<4>), grid, dim3(kThreads), 0, stream, p);
-  return (int)hipGetLastError();
+  return launch_rows<false>(p, stream);
+}
+
+extern "C" int hstu_mxfp4_linear_rows(const void* x, int64_t ldx, const void* W, int64_t ldw, const void* w_scale,
+                                      int64_t ldws, const void* bias, const void* residual, int64_t ldr, void* C,
+                                      int64_t ldc, int M, int N, int K, hipStream_t stream) {
+  MxParams p{(const uint8_t*)x, (const uint8_t*)W, nullptr, (const uint8_t*)w_scale, 2 * ldx, ldw, 0,
+             ldws, (const uint16_t*)bias, (const uint16_t*)residual, (uint16_t*)C, ldr, ldc, M, N, K};
+  const int st = check_product(p, true);
+  if (st != 0 || M == 0) return st;
+  return launch_rows<true>(p, stream);
 }

@@ -10,7 +10,6 @@ is missing or does not load, every entry point raises ``HstuUnavailableError``
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -78,6 +77,7 @@ EXPORTED_SYMBOLS = (
     "hstu_mxfp4_quantize",
     "hstu_mxfp4_dequantize",
     "hstu_mxfp4_gemm",
+    "hstu_mxfp4_linear_rows",
 )
 
 
@@ -213,6 +213,9 @@ _SIGNATURES = {
         _i32,
         [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _vp],
     ),
+    "hstu_mxfp4_linear_rows": (
+        _i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _vp],
+    ),
 }
 
 
@@ -269,13 +272,28 @@ def stream(t) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
-def on_device(t):
-    """A context in which the tensor's device is the current one, which a launch on its stream needs."""
-    import torch
+_raw = None
 
-    if t.device.index is None or t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+
+def launch(name: str, t, *args) -> None:
+    """Call entry point ``name`` with ``args`` and the current stream of the
+    tensor's device as the last argument, with that device current (a launch on
+    its stream needs it); raise on a status.  One call costs the host as little
+    as it can: a decoding step is made of such calls."""
+    global _raw
+    if _raw is None:
+        import torch
+
+        _raw = (torch.cuda.current_device, torch._C._cuda_getCurrentRawStream, torch.cuda.device)
+    f = _bound.get(name) or fn(name)
+    index = t.device.index
+    if index == _raw[0]():
+        status = f(*args, _raw[1](index))
+    else:
+        with _raw[2](index):
+            status = f(*args, _raw[1](index))
+    if status != 0:
+        check(status, name)
 
 
 def ptr(t) -> Optional[int]:

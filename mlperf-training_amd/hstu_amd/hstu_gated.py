@@ -41,10 +41,10 @@ def _act(activation: str) -> int:
 
 def _rows2d(t: torch.Tensor) -> torch.Tensor:
     """[rows, width] with unit column stride and 16-byte aligned rows."""
-    t = t.reshape(-1, t.shape[-1])
-    ok = (t.stride(1) == 1 and t.data_ptr() % 16 == 0
-          and (t.shape[0] <= 1 or (t.stride(0) >= t.shape[1] and t.stride(0) * t.element_size() % 16 == 0)))
-    if ok:
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    s0, s1 = t.stride()
+    if s1 == 1 and t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or (s0 >= t.shape[1] and s0 * t.element_size() % 16 == 0)):
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
@@ -54,39 +54,37 @@ def _ld(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _check(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, dtype: torch.dtype, multiple: int) -> None:
-    for name, t in (("x", x), ("w_gate", w_gate), ("w_up", w_up)):
-        if t.dtype != dtype:
-            raise NotImplementedError(f"{name}: {dtype} (got {t.dtype})")
-        if t.device != x.device or not t.is_cuda:
-            raise NotImplementedError(f"{name}: on one device (got {t.device}, x on {x.device})")
-    if x.dim() < 1 or w_gate.dim() != 2 or w_up.shape != w_gate.shape or w_gate.shape[1] != x.shape[-1]:
-        raise ValueError(f"x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)}: expected "
+def _check(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, dtype: torch.dtype, multiple: int) -> Tuple[int, int]:
+    """(F, D)"""
+    if x.dtype != dtype or w_gate.dtype != dtype or w_up.dtype != dtype:
+        raise NotImplementedError(f"x, w_gate, w_up: {dtype} (got {x.dtype}, {w_gate.dtype}, {w_up.dtype})")
+    device = x.device
+    if not x.is_cuda or w_gate.device != device or w_up.device != device:
+        raise NotImplementedError(f"x, w_gate, w_up: on one device (got {device}, {w_gate.device}, {w_up.device})")
+    shape = w_gate.shape
+    if x.dim() < 1 or len(shape) != 2 or w_up.shape != shape or shape[1] != x.shape[-1]:
+        raise ValueError(f"x {tuple(x.shape)}, w_gate {tuple(shape)}, w_up {tuple(w_up.shape)}: expected "
                          "[.., D], [F, D], [F, D]")
-    F, D = w_gate.shape
+    F, D = shape
     if D == 0 or F == 0 or D % multiple or F % 128:
         raise NotImplementedError(f"D = {D}, F = {F}: D a multiple of {multiple} and F of 128")
     if x.numel() // D >= 2 ** 31 - 256:
         raise NotImplementedError("x: fewer than 2^31 rows")
+    return F, D
 
 
 def gated_linear_fwd(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = "silu",
                      keep: bool = False):
     """h [.., F] in bf16; with ``keep`` (h, gu): gu fp32 [rows, 2F] holds g and u for ``gated_linear_bwd``."""
     act = _act(activation)
-    x, w_gate, w_up = x.detach(), w_gate.detach(), w_up.detach()
-    _check(x, w_gate, w_up, torch.bfloat16, 256)
-    F, D = w_gate.shape
+    F, D = _check(x, w_gate, w_up, torch.bfloat16, 256)
     x2, g, u = _rows2d(x), _rows2d(w_gate), _rows2d(w_up)
     M = x2.shape[0]
-    h = torch.empty((M, F), dtype=torch.bfloat16, device=x.device)
+    h = torch.empty(x.shape[:-1] + (F,), dtype=torch.bfloat16, device=x.device)
     gu = torch.empty((M, 2 * F), dtype=torch.float32, device=x.device) if keep else None
     if M > 0:
-        with _lib.on_device(x):
-            st = _lib.fn("hstu_gated_fwd")(x2.data_ptr(), _ld(x2), g.data_ptr(), _ld(g), u.data_ptr(), _ld(u), M, F, D,
-                                           act, h.data_ptr(), F, _lib.ptr(gu), _lib.stream(x))
-        _lib.check(st, "hstu_gated_fwd")
-    h = h.view(x.shape[:-1] + (F,))
+        _lib.launch("hstu_gated_fwd", x, x2.data_ptr(), _ld(x2), g.data_ptr(), _ld(g), u.data_ptr(), _ld(u), M, F, D,
+                    act, h.data_ptr(), F, _lib.ptr(gu))
     return (h, gu) if keep else h
 
 
@@ -97,36 +95,29 @@ def gated_linear_bwd(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_
     """(dx, dw_gate, dw_up) in bf16; None for what is not needed.  ``gu``: what
     ``gated_linear_fwd(keep=True)`` kept; without it g and u are computed again."""
     act = _act(activation)
-    dh, x, w_gate, w_up = dh.detach(), x.detach(), w_gate.detach(), w_up.detach()
-    _check(x, w_gate, w_up, torch.bfloat16, 256)
-    F, D = w_gate.shape
-    if dh.shape != x.shape[:-1] + (F,) or dh.dtype != torch.bfloat16 or dh.device != x.device:
-        raise ValueError(f"dh {tuple(dh.shape)} {dh.dtype}; expected {tuple(x.shape[:-1] + (F,))} bf16 on {x.device}")
+    F, D = _check(x, w_gate, w_up, torch.bfloat16, 256)
+    device = x.device
+    if dh.shape != x.shape[:-1] + (F,) or dh.dtype != torch.bfloat16 or dh.device != device:
+        raise ValueError(f"dh {tuple(dh.shape)} {dh.dtype}; expected {tuple(x.shape[:-1] + (F,))} bf16 on {device}")
     x2, g, u, d2 = _rows2d(x), _rows2d(w_gate), _rows2d(w_up), _rows2d(dh)
     M = x2.shape[0]
     if gu is not None and (gu.shape != (M, 2 * F) or gu.dtype != torch.float32 or not gu.is_contiguous()
-                           or gu.device != x.device):
-        raise ValueError(f"gu {tuple(gu.shape)} {gu.dtype}; expected contiguous fp32 [{M}, {2 * F}] on {x.device}")
+                           or gu.device != device):
+        raise ValueError(f"gu {tuple(gu.shape)} {gu.dtype}; expected contiguous fp32 [{M}, {2 * F}] on {device}")
     if M == 0:
-        dw = torch.zeros((2 * F, D), dtype=torch.bfloat16, device=x.device)
+        dw = torch.zeros((2 * F, D), dtype=torch.bfloat16, device=device)
         return torch.empty_like(x) if need_dx else None, dw[:F] if need_dw else None, dw[F:] if need_dw else None
-    dgu = torch.empty((M, 2 * F), dtype=torch.bfloat16, device=x.device)
-    with _lib.on_device(x):
-        stream = _lib.stream(x)
-        if gu is not None:
-            st = _lib.fn("hstu_gated_bwd_kept")(d2.data_ptr(), _ld(d2), gu.data_ptr(), M, F, act, dgu.data_ptr(),
-                                                2 * F, stream)
-            _lib.check(st, "hstu_gated_bwd_kept")
-        else:
-            st = _lib.fn("hstu_gated_bwd")(d2.data_ptr(), _ld(d2), x2.data_ptr(), _ld(x2), g.data_ptr(), _ld(g),
-                                           u.data_ptr(), _ld(u), M, F, D, act, dgu.data_ptr(), 2 * F, stream)
-            _lib.check(st, "hstu_gated_bwd")
-        dx = dg = du = None
+    dgu = torch.empty((M, 2 * F), dtype=torch.bfloat16, device=device)
+    if gu is not None:
+        _lib.launch("hstu_gated_bwd_kept", x, d2.data_ptr(), _ld(d2), gu.data_ptr(), M, F, act, dgu.data_ptr(), 2 * F)
+    else:
+        _lib.launch("hstu_gated_bwd", x, d2.data_ptr(), _ld(d2), x2.data_ptr(), _ld(x2), g.data_ptr(), _ld(g),
+                    u.data_ptr(), _ld(u), M, F, D, act, dgu.data_ptr(), 2 * F)
+    dx = dg = du = None
+    with torch.cuda.device(device):
         if need_dx:  # the contraction runs over both halves of dgu: the weights side by side, transposed
-            wt = torch.empty((D, 2 * F), dtype=torch.bfloat16, device=x.device)
-            st = _lib.fn("hstu_gated_transpose")(g.data_ptr(), _ld(g), u.data_ptr(), _ld(u), F, D, wt.data_ptr(), 2 * F,
-                                                 stream)
-            _lib.check(st, "hstu_gated_transpose")
+            wt = torch.empty((D, 2 * F), dtype=torch.bfloat16, device=device)
+            _lib.launch("hstu_gated_transpose", x, g.data_ptr(), _ld(g), u.data_ptr(), _ld(u), F, D, wt.data_ptr(), 2 * F)
             dx = bf16_gemm(dgu, wt).view(x.shape)
         if need_dw:
             dw = wgrad(dgu, x2, split=_wgrad_split(M, 2 * F, D))
@@ -185,7 +176,9 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, acti
 def _scale(name: str, s: torch.Tensor, n: int, x: torch.Tensor) -> Tuple[torch.Tensor, int]:
     if s.device != x.device or s.numel() not in (1, n):
         raise ValueError(f"{name}: 1 or {n} values on {x.device} (got {tuple(s.shape)} on {s.device})")
-    return s.detach().to(torch.float32).reshape(-1).contiguous(), 1 if s.numel() > 1 else 0
+    if s.dtype != torch.float32 or s.dim() != 1 or not s.is_contiguous():
+        s = s.detach().to(torch.float32).reshape(-1).contiguous()
+    return s, 1 if s.numel() > 1 else 0
 
 
 def gated_linear_fp8(x8: torch.Tensor, x_scale: torch.Tensor, gate: Scaled, up: Scaled, activation: str = "silu"
@@ -194,18 +187,14 @@ def gated_linear_fp8(x8: torch.Tensor, x_scale: torch.Tensor, gate: Scaled, up: 
     ``gate``, ``up`` as pairs (e4m3 [F, D], scale: one or [F]).  h [.., F] in bf16."""
     act = _act(activation)
     (g8, gs), (u8, us) = gate, up
-    _check(x8, g8, u8, E4M3, 128)
-    F, D = g8.shape
+    F, D = _check(x8, g8, u8, E4M3, 128)
     x2, g2, u2 = _rows2d(x8), _rows2d(g8), _rows2d(u8)
     M = x2.shape[0]
     xs, xm = _scale("x_scale", x_scale, M, x8)
     gs, gm = _scale("gate scale", gs, F, x8)
     us, um = _scale("up scale", us, F, x8)
-    h = torch.empty((M, F), dtype=torch.bfloat16, device=x8.device)
+    h = torch.empty(x8.shape[:-1] + (F,), dtype=torch.bfloat16, device=x8.device)
     if M > 0:
-        with _lib.on_device(x8):
-            st = _lib.fn("hstu_gated_fwd_fp8")(
-                x2.data_ptr(), _ld(x2), xs.data_ptr(), xm, g2.data_ptr(), _ld(g2), gs.data_ptr(), gm, u2.data_ptr(),
-                _ld(u2), us.data_ptr(), um, M, F, D, act, h.data_ptr(), F, _lib.stream(x8))
-        _lib.check(st, "hstu_gated_fwd_fp8")
-    return h.view(x8.shape[:-1] + (F,))
+        _lib.launch("hstu_gated_fwd_fp8", x8, x2.data_ptr(), _ld(x2), xs.data_ptr(), xm, g2.data_ptr(), _ld(g2),
+                    gs.data_ptr(), gm, u2.data_ptr(), _ld(u2), us.data_ptr(), um, M, F, D, act, h.data_ptr(), F)
+    return h

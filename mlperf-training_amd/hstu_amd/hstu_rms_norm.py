@@ -34,13 +34,20 @@ MAX_D = 32768
 
 def _rows2d(t: torch.Tensor) -> torch.Tensor:
     """[rows, D] with unit column stride and disjoint rows (column slices of a wider buffer stay in place)."""
+    if t.dim() == 2:
+        s0, s1 = t.stride()
+        if s1 == 1 and (s0 >= t.shape[1] or t.shape[0] <= 1):
+            return t
+        return t.contiguous()
     t = t.reshape(-1, t.shape[-1])
     return t if t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
 
 
-def _ld(t: Optional[torch.Tensor]) -> int:
+def _ld(t: torch.Tensor) -> int:
     """Row stride; a single row may have any."""
-    return 0 if t is None else max(t.stride(0), t.shape[1])
+    n = t.shape[1]
+    s = t.stride(0)
+    return s if s > n else n
 
 
 def _like(name: str, t: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
@@ -50,21 +57,20 @@ def _like(name: str, t: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
     return _rows2d(t)
 
 
-def _weight(weight: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
-    if weight.dim() != 1 or weight.shape[0] != x.shape[-1] or weight.device != x.device:
-        raise ValueError(f"weight {tuple(weight.shape)} on {weight.device} must be [{x.shape[-1]}] on {x.device}")
-    if weight.dtype not in _TYPES:
-        raise NotImplementedError(f"weight: bf16 or fp32 (got {weight.dtype})")
-    return weight.contiguous()
-
-
-def _check(x: torch.Tensor) -> None:
-    if x.dtype not in _TYPES:
+def _check(x: torch.Tensor, weight: torch.Tensor) -> Tuple[int, torch.Tensor, int]:
+    """(code of x's type, the weight with unit stride, code of its type)"""
+    code, wcode = _TYPES.get(x.dtype), _TYPES.get(weight.dtype)
+    if code is None:
         raise NotImplementedError(f"x: bf16 or fp32 (got {x.dtype})")
     if x.dim() < 1 or not 0 < x.shape[-1] <= MAX_D:
         raise NotImplementedError(f"x {tuple(x.shape)}: a last dimension of 1 .. {MAX_D}")
     if not x.is_cuda:
         raise NotImplementedError("x: device tensors only")
+    if weight.dim() != 1 or weight.shape[0] != x.shape[-1] or weight.device != x.device:
+        raise ValueError(f"weight {tuple(weight.shape)} on {weight.device} must be [{x.shape[-1]}] on {x.device}")
+    if wcode is None:
+        raise NotImplementedError(f"weight: bf16 or fp32 (got {weight.dtype})")
+    return code, weight if weight.stride(0) == 1 else weight.contiguous(), wcode
 
 
 def rms_norm_fwd(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None,
@@ -73,35 +79,33 @@ def rms_norm_fwd(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
     """(y, h, rstd, y_scale).  ``h`` is ``x`` itself without a residual; ``rstd``
     fp32 [rows]; ``output_fp8``: y e4m3 and ``y_scale`` the fp32 scales of the
     rows, or ``scale`` (one fp32 value on the device) where it is given."""
-    _check(x)
-    w = _weight(weight.detach(), x)
-    D = x.shape[-1]
-    x2 = _rows2d(x.detach())
+    code, w, wcode = _check(x, weight)
+    shape, device, D = x.shape, x.device, x.shape[-1]
+    x2 = _rows2d(x)
     rows = x2.shape[0]
-    r2 = None if residual is None else _like("residual", residual.detach(), x)
-    h2 = None if residual is None else torch.empty((rows, D), dtype=x.dtype, device=x.device)
-    y = torch.empty((rows, D), dtype=E4M3 if output_fp8 else x.dtype, device=x.device)
-    rstd = torch.empty((rows,), dtype=torch.float32, device=x.device) if want_rstd else None
+    r2 = h = None
+    r_ptr = h_ptr = r_ld = 0
+    if residual is not None:
+        r2 = _like("residual", residual, x)
+        h = torch.empty(shape, dtype=x.dtype, device=device)
+        r_ptr, r_ld, h_ptr = r2.data_ptr(), _ld(r2), h.data_ptr()
+    y = torch.empty(shape, dtype=E4M3 if output_fp8 else x.dtype, device=device)
+    rstd = torch.empty(rows, dtype=torch.float32, device=device) if want_rstd else None
     given = y_scale = None
     if output_fp8:
         if scale is None:
-            y_scale = torch.empty((rows,), dtype=torch.float32, device=x.device)
+            y_scale = torch.empty(rows, dtype=torch.float32, device=device)
         else:
-            if scale.numel() != 1 or scale.device != x.device:
+            if scale.numel() != 1 or scale.device != device:
                 raise ValueError("scale must be one value on x's device")
-            given = scale.detach().to(torch.float32).reshape(1)
+            given = y_scale = scale.detach().to(torch.float32).reshape(1)
     elif scale is not None:
         raise ValueError("scale goes with output_fp8")
     if rows > 0:
-        with _lib.on_device(x):
-            st = _lib.fn("hstu_rms_norm_fwd")(
-                _TYPES[x.dtype], x2.data_ptr(), _ld(x2), _lib.ptr(r2), _ld(r2), w.data_ptr(), _TYPES[w.dtype],
-                float(eps), rows, D, _lib.ptr(h2), D, y.data_ptr(), D,
-                _lib.HSTU_DTYPE_FP8_E4M3 if output_fp8 else _TYPES[x.dtype], _lib.ptr(given), _lib.ptr(y_scale),
-                _lib.ptr(rstd), _lib.stream(x))
-        _lib.check(st, "hstu_rms_norm_fwd")
-    h = x if residual is None else h2.view(x.shape)
-    return y.view(x.shape), h, rstd, given if given is not None else y_scale
+        _lib.launch("hstu_rms_norm_fwd", x, code, x2.data_ptr(), _ld(x2), r_ptr, r_ld, w.data_ptr(), wcode, eps, rows,
+                    D, h_ptr, D, y.data_ptr(), D, _lib.HSTU_DTYPE_FP8_E4M3 if output_fp8 else code, _lib.ptr(given),
+                    None if given is not None else _lib.ptr(y_scale), _lib.ptr(rstd))
+    return y, x if h is None else h, rstd, y_scale
 
 
 def rms_norm_bwd(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor,
@@ -109,28 +113,24 @@ def rms_norm_bwd(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, rstd: 
                  ) -> Tuple[torch.Tensor, torch.Tensor]:
     """(dx, dweight): dx is the gradient of x and of the residual; ``dh`` the
     gradient of the returned h.  dweight in ``dweight_dtype`` (the weight's)."""
-    _check(h)
-    w = _weight(weight.detach(), h)
-    D = h.shape[-1]
+    code, w, wcode = _check(h, weight)
+    device, D = h.device, h.shape[-1]
     dt = w.dtype if dweight_dtype is None else dweight_dtype
     if dt not in _TYPES:
         raise NotImplementedError(f"dweight: bf16 or fp32 (got {dt})")
-    h2, dy2 = _rows2d(h.detach()), _like("dy", dy.detach(), h)
-    d2 = None if dh is None else _like("dh", dh.detach(), h)
+    h2, dy2 = _rows2d(h), _like("dy", dy, h)
+    d2 = None if dh is None else _like("dh", dh, h)
     rows = h2.shape[0]
-    if rstd.dtype != torch.float32 or rstd.numel() != rows or rstd.device != h.device:
-        raise ValueError(f"rstd must be fp32 [{rows}] on {h.device}")
-    dx = torch.empty((rows, D), dtype=h.dtype, device=h.device)
-    dw = torch.empty((D,), dtype=dt, device=h.device)
-    nbytes = int(_lib.fn("hstu_rms_norm_bwd_workspace_bytes")(rows, D))
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=h.device)
-    with _lib.on_device(h):
-        st = _lib.fn("hstu_rms_norm_bwd")(
-            _TYPES[h.dtype], dy2.data_ptr(), _ld(dy2), h2.data_ptr(), _ld(h2), _lib.ptr(d2), _ld(d2), w.data_ptr(),
-            _TYPES[w.dtype], rstd.contiguous().data_ptr(), rows, D, dx.data_ptr(), D, dw.data_ptr(), _TYPES[dt],
-            ws.data_ptr(), nbytes, _lib.stream(h))
-    _lib.check(st, "hstu_rms_norm_bwd")
-    return dx.view(h.shape), dw
+    if rstd.dtype != torch.float32 or rstd.shape != (rows,) or rstd.device != device or rstd.stride(0) != 1:
+        raise ValueError(f"rstd must be contiguous fp32 [{rows}] on {device}")
+    dx = torch.empty(h.shape, dtype=h.dtype, device=device)
+    dw = torch.empty(D, dtype=dt, device=device)
+    nbytes = _lib.fn("hstu_rms_norm_bwd_workspace_bytes")(rows, D)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    _lib.launch("hstu_rms_norm_bwd", h, code, dy2.data_ptr(), _ld(dy2), h2.data_ptr(), _ld(h2), _lib.ptr(d2),
+                0 if d2 is None else _ld(d2), w.data_ptr(), wcode, rstd.data_ptr(), rows, D, dx.data_ptr(), D,
+                dw.data_ptr(), _TYPES[dt], ws.data_ptr(), nbytes)
+    return dx, dw
 
 
 class RMSNormFunction(torch.autograd.Function):
@@ -143,7 +143,7 @@ class RMSNormFunction(torch.autograd.Function):
         y, h, rstd, _ = rms_norm_fwd(x, weight, eps, residual)
         ctx.save_for_backward(h, weight, rstd)
         ctx.has_residual = residual is not None
-        return (y, h) if residual is not None else y
+        return (y, h) if ctx.has_residual else y
 
     @staticmethod
     def backward(ctx, dy, dh=None):
@@ -158,7 +158,11 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     """``y``, or ``(y, h)`` with a residual: h = x + residual is the new residual
     stream and y its norm times ``weight``.  Differentiable in x, residual and
     weight, through y and h."""
-    return RMSNormFunction.apply(x, weight, eps, residual)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
+                                    or (residual is not None and residual.requires_grad)):
+        return RMSNormFunction.apply(x, weight, eps, residual)
+    y, h, _, _ = rms_norm_fwd(x, weight, eps, residual, want_rstd=False)
+    return y if residual is None else (y, h)
 
 
 def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None,

@@ -24,6 +24,9 @@ import torch
 from . import _lib
 
 _TYPES = {torch.bfloat16: _lib.HSTU_DTYPE_BF16, torch.float32: _lib.HSTU_DTYPE_FP32}
+# Up to here the product's kernel quantizes its rows of x itself (one launch, the
+# work repeated for every 16 outputs); beyond, a kernel of its own does it once.
+ROWS_QUANT = 16
 Packed = Tuple[torch.Tensor, torch.Tensor]
 
 
@@ -35,19 +38,18 @@ def quantize_mxfp4(x: torch.Tensor) -> Packed:
         raise NotImplementedError(f"x {tuple(x.shape)}: a last dimension that is a multiple of 32")
     if not x.is_cuda:
         raise NotImplementedError("x: device tensors only")
-    C = x.shape[-1]
-    x2 = x.detach().reshape(-1, C)
-    if x2.stride(1) != 1 or (x2.shape[0] > 1 and x2.stride(0) < C):
-        x2 = x2.contiguous()
+    shape, C = x.shape, x.shape[-1]
+    x2 = x if x.dim() == 2 else x.reshape(-1, C)
     R = x2.shape[0]
-    codes = torch.empty((R, C // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((R, C // 32), dtype=torch.uint8, device=x.device)
+    s0, s1 = x2.stride()
+    if s1 != 1 or (R > 1 and s0 < C):
+        x2, s0 = x2.contiguous(), C
+    codes = torch.empty(shape[:-1] + (C // 2,), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(shape[:-1] + (C // 32,), dtype=torch.uint8, device=x.device)
     if R > 0:
-        with _lib.on_device(x):
-            st = _lib.fn("hstu_mxfp4_quantize")(_TYPES[x.dtype], x2.data_ptr(), x2.stride(0) if R > 1 else C, R, C,
-                                                codes.data_ptr(), scales.data_ptr(), _lib.stream(x))
-        _lib.check(st, "hstu_mxfp4_quantize")
-    return codes.view(x.shape[:-1] + (C // 2,)), scales.view(x.shape[:-1] + (C // 32,))
+        _lib.launch("hstu_mxfp4_quantize", x, _TYPES[x.dtype], x2.data_ptr(), s0 if R > 1 else C, R, C,
+                    codes.data_ptr(), scales.data_ptr())
+    return codes, scales
 
 
 def _pair(name: str, codes: torch.Tensor, scales: torch.Tensor) -> None:
@@ -66,23 +68,22 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dty
     if dtype not in _TYPES:
         raise NotImplementedError(f"dtype: bf16 or fp32 (got {dtype})")
     _pair("dequantize_mxfp4", codes, scales)
-    lead, C = codes.shape[:-1], 2 * codes.shape[-1]
-    c2, s2 = codes.reshape(-1, C // 2).contiguous(), scales.reshape(-1, C // 32).contiguous()
+    C = 2 * codes.shape[-1]
+    c2, s2 = codes.contiguous(), scales.contiguous()
     c2 = c2 if c2.data_ptr() % 4 == 0 else c2.clone()
-    R = c2.shape[0]
-    out = torch.empty((R, C), dtype=dtype, device=codes.device)
+    out = torch.empty(codes.shape[:-1] + (C,), dtype=dtype, device=codes.device)
+    R = out.numel() // C
     if R > 0:
-        with _lib.on_device(codes):
-            st = _lib.fn("hstu_mxfp4_dequantize")(c2.data_ptr(), s2.data_ptr(), R, C, _TYPES[dtype], out.data_ptr(), C,
-                                                  _lib.stream(codes))
-        _lib.check(st, "hstu_mxfp4_dequantize")
-    return out.view(lead + (C,))
+        _lib.launch("hstu_mxfp4_dequantize", codes, c2.data_ptr(), s2.data_ptr(), R, C, _TYPES[dtype], out.data_ptr(), C)
+    return out
 
 
 def _aligned(t: torch.Tensor, n: int) -> torch.Tensor:
     """A 2-D operand with unit column stride and rows at multiples of n bytes."""
-    if (t.stride(1) == 1 and t.data_ptr() % n == 0
-            and (t.shape[0] <= 1 or (t.stride(0) >= t.shape[1] and t.stride(0) * t.element_size() % n == 0))):
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    s0, s1 = t.stride()
+    if s1 == 1 and t.data_ptr() % n == 0 and (t.shape[0] <= 1 or (s0 >= t.shape[1] and s0 * t.element_size() % n == 0)):
         return t
     t = t.contiguous()
     return t if t.data_ptr() % n == 0 else t.clone()
@@ -96,13 +97,14 @@ def _epilogue(bias: Optional[torch.Tensor], residual: Optional[torch.Tensor], sh
     if bias is not None:
         if bias.shape != shape[-1:] or bias.device != device:
             raise ValueError(f"bias {tuple(bias.shape)} on {bias.device}; expected [{shape[-1]}] on {device}")
-        bias = bias.detach().to(torch.bfloat16).contiguous()
+        if bias.dtype != torch.bfloat16 or bias.stride(0) != 1:
+            bias = bias.detach().to(torch.bfloat16).contiguous()
         bias = bias if bias.data_ptr() % 16 == 0 else bias.clone()
     if residual is not None:
         if residual.shape != shape or residual.device != device or residual.dtype != torch.bfloat16:
             raise ValueError(f"residual {tuple(residual.shape)} {residual.dtype} on {residual.device}; expected "
                              f"{tuple(shape)} bf16 on {device}")
-        residual = _aligned(residual.detach().reshape(-1, shape[-1]), 16)
+        residual = _aligned(residual, 16)
     return bias, residual
 
 
@@ -128,18 +130,16 @@ def mxfp4_mm(a: Packed, weight: Packed, bias: Optional[torch.Tensor] = None,
         raise ValueError(f"a codes {tuple(ac.shape)} on {ac.device} against weight [{N}, {K}] on {wc.device}")
     shape = ac.shape[:-1] + (N,)
     bias, r2 = _epilogue(bias, residual, shape, wc.device)
-    a2, s2 = _aligned(ac.reshape(-1, K // 2), 16), _aligned(as_.reshape(-1, K // 32), 4)
+    a2, s2 = _aligned(ac, 16), _aligned(as_, 4)
     M = a2.shape[0]
     if M >= 2 ** 31 - 256:
         raise NotImplementedError("a: fewer than 2^31 rows")
-    out = torch.empty((M, N), dtype=torch.bfloat16, device=wc.device)
+    out = torch.empty(shape, dtype=torch.bfloat16, device=wc.device)
     if M > 0:
-        with _lib.on_device(wc):
-            st = _lib.fn("hstu_mxfp4_gemm")(
-                a2.data_ptr(), _ld(a2), s2.data_ptr(), _ld(s2), wc.data_ptr(), _ld(wc), ws.data_ptr(), _ld(ws),
-                _lib.ptr(bias), _lib.ptr(r2), 0 if r2 is None else _ld(r2), out.data_ptr(), N, M, N, K, _lib.stream(wc))
-        _lib.check(st, "hstu_mxfp4_gemm")
-    return out.view(shape)
+        _lib.launch("hstu_mxfp4_gemm", wc, a2.data_ptr(), _ld(a2), s2.data_ptr(), _ld(s2), wc.data_ptr(), _ld(wc),
+                    ws.data_ptr(), _ld(ws), _lib.ptr(bias), _lib.ptr(r2), 0 if r2 is None else _ld(r2), out.data_ptr(),
+                    N, M, N, K)
+    return out
 
 
 def mxfp4_linear(x: torch.Tensor, weight: Packed, bias: Optional[torch.Tensor] = None,
@@ -147,4 +147,18 @@ def mxfp4_linear(x: torch.Tensor, weight: Packed, bias: Optional[torch.Tensor] =
     """quantize(x) @ weight^T (+ bias) (+ residual) in bf16, for bf16 x [.., K]."""
     if x.dtype != torch.bfloat16:
         raise NotImplementedError(f"x: bf16 (got {x.dtype})")
-    return mxfp4_mm(quantize_mxfp4(x), weight, bias, residual)
+    wc, ws, N, K = _weight(weight)
+    shape = x.shape
+    if shape[-1] != K or x.device != wc.device:
+        raise ValueError(f"x {tuple(shape)} on {x.device} against weight [{N}, {K}] on {wc.device}")
+    M = x.numel() // K
+    if M > ROWS_QUANT:
+        return mxfp4_mm(quantize_mxfp4(x), weight, bias, residual)
+    shape = shape[:-1] + (N,)
+    bias, r2 = _epilogue(bias, residual, shape, wc.device)
+    out = torch.empty(shape, dtype=torch.bfloat16, device=wc.device)
+    if M > 0:
+        x2 = _aligned(x, 16)
+        _lib.launch("hstu_mxfp4_linear_rows", wc, x2.data_ptr(), _ld(x2), wc.data_ptr(), _ld(wc), ws.data_ptr(), _ld(ws),
+                    _lib.ptr(bias), _lib.ptr(r2), 0 if r2 is None else _ld(r2), out.data_ptr(), N, M, N, K)
+    return out

@@ -345,3 +345,14 @@ def test_c_entry_refusals():
                 dict(ldc=20), dict(bias=66), dict(res=66, ldr=16)):
         assert gemm(**bad) == lib.HSTU_E_UNSUPPORTED, bad
     assert gemm(M=0) == 0
+    rows = lib.fn("hstu_mxfp4_linear_rows")
+
+    def linear(x=P, ldx=128, W=P, ldw=64, sw=P, ldsw=4, res=None, ldr=0, C=P, ldc=16, M=2, N=16, K=128):
+        return rows(x, ldx, W, ldw, sw, ldsw, None, res, ldr, C, ldc, M, N, K, None)
+
+    for bad in (dict(M=-1), dict(ldx=127), dict(x=None), dict(W=None), dict(sw=None), dict(C=None), dict(ldc=8),
+                dict(res=P, ldr=8)):
+        assert linear(**bad) == lib.HSTU_E_BAD_ARG, bad
+    for bad in (dict(x=72), dict(ldx=132), dict(K=96), dict(N=24, ldc=24)):
+        assert linear(**bad) == lib.HSTU_E_UNSUPPORTED, bad
+    assert linear(M=0) == 0
