@@ -610,7 +610,7 @@ int hstu_dequantize_do_e4m3_blk(const void* dout_e4m3, const void* e8, int64_t T
  *   h = round(x + residual) (h = x when residual is NULL; then the h argument
  *   is ignored), rstd = 1 / sqrt(mean(h^2) + eps), y = h * rstd * weight.
  * x, residual, h: [rows, D] of dtype (HSTU_DTYPE_BF16 or HSTU_DTYPE_FP32), row
- * strides in elements; any D up to 32768, any alignment of whole elements
+ * strides in elements; any D up to 16384, any alignment of whole elements
  * (rows of 16-byte multiples at 16-byte addresses take 16-byte accesses).
  * weight [D] bf16 or fp32 (param_dtype).  The norm is of the rounded h, the one
  * a backward has.  out_dtype: dtype, or HSTU_DTYPE_FP8_E4M3: y = e4m3(clamp(y /

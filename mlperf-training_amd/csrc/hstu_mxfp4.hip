@@ -33,57 +33,58 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
   v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true));  // quad_perm 1 0 3 2
   return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true));  // quad_perm 2 3 0 1
 }
-// Eight values (bits of fp32) of a lane, the block being those of its quad ->
-// codes and the scale byte.  Magnitudes compare as integers, NaN above infinity.
+// Scale byte from the exponent field of a block's largest magnitude (255: it is
+// infinite or NaN), and the float whose exponent the conversions divide by: 2^E
+// (they use the exponent field alone, so byte 0 is 2^-127 there too).
+__device__ __forceinline__ uint32_t mx_byte(uint32_t field) { return field == 255u ? 255u : field >= 2u ? field - 2u : 0u; }
+__device__ __forceinline__ float mx_divisor(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
+
+// Largest magnitude of bf16 pairs, as 16-bit integers (NaN above infinity)
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u16x2 mag_max(u16x2 top, uint32_t x) {
+  return __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, x & 0x7fff7fffu));
+}
+__device__ __forceinline__ uint32_t field_of(u16x2 top) { return (uint32_t)max(top[0], top[1]) >> 7; }
+// Eight bf16 -> eight codes (round to nearest even, at most 6)
+__device__ __forceinline__ uint32_t mx_codes8(u32x4 v, float divisor) {
+  const uint32_t x0 = v[0], x1 = v[1], x2 = v[2], x3 = v[3];
+  uint32_t w = 0;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2, x0), divisor, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2, x1), divisor, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2, x2), divisor, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2, x3), divisor, 3);
+}
+// Eight values of a lane, the block being those of its quad -> codes, scale byte
+__device__ __forceinline__ uint32_t mx_encode8(u32x4 v, uint32_t& byte) {
+  u16x2 top = {0, 0};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) top = mag_max(top, v[j]);
+  byte = mx_byte(quad_max(field_of(top)));
+  const uint32_t w = mx_codes8(v, mx_divisor(byte));
+  return byte == 255u ? 0u : w;
+}
 __device__ __forceinline__ uint32_t mx_encode8(const float (&v)[8], uint32_t& byte) {
   uint32_t top = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) top = max(top, __builtin_bit_cast(uint32_t, v[e]) & 0x7fffffffu);
-  const uint32_t ex = quad_max(top) >> 23;
-  byte = ex == 255u ? 255u : ex >= 2u ? ex - 2u : 0u;
-  const float up = ex == 255u ? 0.f : __builtin_bit_cast(float, (254u - byte) << 23);  // 2^-E
+  byte = mx_byte(quad_max(top >> 23));
+  const float d = mx_divisor(byte);
   uint32_t w = 0;
-  float t[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) t[e] = ex == 255u ? 0.f : v[e] * up;
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[0], t[1], 1.f, 0);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[2], t[3], 1.f, 1);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[4], t[5], 1.f, 2);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[6], t[7], 1.f, 3);
-  return w;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], d, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], d, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], d, 2);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], d, 3);
+  return byte == 255u ? 0u : w;
 }
-
-// A whole block, 32 bf16 of one lane, the same way.
-__device__ __forceinline__ void mx_encode32(const u32x4 (&v)[4], u32x4& codes, uint32_t& byte) {
-  // the largest magnitude of both halves of the words at once, as 16-bit integers
-  uint32_t lo = 0, hi = 0;
+// A whole block, 32 bf16 of one lane
+__device__ __forceinline__ u32x4 mx_encode32(const u32x4* x, uint32_t& byte) {
+  const u32x4 v0 = x[0], v1 = x[1], v2 = x[2], v3 = x[3];
+  u16x2 top = {0, 0};
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t x = v[j][e];
-      lo = max(lo, x & 0x7fffu);
-      hi = max(hi, x & 0x7fff0000u);
-    }
-  const uint32_t ex = max(lo >> 7, hi >> 23);
-  byte = ex == 255u ? 255u : ex >= 2u ? ex - 2u : 0u;
-  const float up = ex == 255u ? 0.f : __builtin_bit_cast(float, (254u - byte) << 23);  // 2^-E
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    uint32_t w = 0;
-    float t[8];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t x = v[j][e];
-      t[2 * e] = bf16f(x & 0xffffu) * up;
-      t[2 * e + 1] = __builtin_bit_cast(float, x & 0xffff0000u) * up;
-    }
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[0], t[1], 1.f, 0);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[2], t[3], 1.f, 1);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[4], t[5], 1.f, 2);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[6], t[7], 1.f, 3);
-    codes[j] = w;
-  }
+  for (int j = 0; j < 4; ++j) top = mag_max(mag_max(mag_max(mag_max(top, v0[j]), v1[j]), v2[j]), v3[j]);
+  byte = mx_byte(field_of(top));
+  const float d = mx_divisor(byte);
+  return u32x4{mx_codes8(v0, d), mx_codes8(v1, d), mx_codes8(v2, d), mx_codes8(v3, d)};
 }
 
 struct QuantArgs {
@@ -103,21 +104,29 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(QuantArgs a) {
     const int64_t row = i / a.chunks;
     const int c = (int)(i - row * a.chunks);
     const uint8_t* src = a.x + row * a.ldx + (int64_t)c * (F32 ? 32 : 16);
-    float v[8];
-    if constexpr (VEC && F32) {
-      const f32x4 p = *(const f32x4*)src, q = *(const f32x4*)(src + 16);
+    uint32_t byte, w;
+    if constexpr (F32) {
+      float v[8];
+      if constexpr (VEC) {
+        const f32x4 p = *(const f32x4*)src, q = *(const f32x4*)(src + 16);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = p[e], v[4 + e] = q[e];
-    } else if constexpr (VEC) {
-      const u32x4 p = *(const u32x4*)src;
+        for (int e = 0; e < 4; ++e) v[e] = p[e], v[4 + e] = q[e];
+      } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[2 * e] = bf16f(p[e] & 0xffffu), v[2 * e + 1] = bf16f(p[e] >> 16);
+        for (int e = 0; e < 8; ++e) v[e] = ((const float*)src)[e];
+      }
+      w = mx_encode8(v, byte);
     } else {
+      u32x4 v;
+      if constexpr (VEC) {
+        v = *(const u32x4*)src;
+      } else {
+        const uint16_t* h = (const uint16_t*)src;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = F32 ? ((const float*)src)[e] : bf16f(((const uint16_t*)src)[e]);
+        for (int e = 0; e < 4; ++e) v[e] = (uint32_t)h[2 * e] | (uint32_t)h[2 * e + 1] << 16;
+      }
+      w = mx_encode8(v, byte);
     }
-    uint32_t byte;
-    const uint32_t w = mx_encode8(v, byte);
     ((uint32_t*)a.codes)[i] = w;
     if ((i & 3) == 0) a.scales[i >> 2] = (uint8_t)byte;
   }
@@ -194,59 +203,92 @@ __device__ __forceinline__ void mx_store4(const MxParams& p, int m, int n, f32x4
   *(u32x2*)(p.C + (int64_t)m * p.ldc + n) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
 }
 
-// Row form, for few rows, where the weights' bytes and the calls are the time: 16
+// Row form, for few rows, where the weights' bytes and the calls are the time: 16 NB
 // columns and 16 MB rows a workgroup, whose WAVES waves take one contiguous piece
 // of the contraction each, operands going from memory to registers as the MFMA takes
-// them, and meet in LDS: wave b sums row block b over the waves in order.
-// QUANT: A is bf16 and quantised here: lane (li, q) of a step holds the 32 values of
-// its own block, so the block's scale and codes need no other lane.
-template <int MB, int WAVES, bool QUANT>
+// them, and meet in LDS, where the blocks are summed over the waves in order.
+// A step is 256 values: lane (li, q) holds blocks 2 q and 2 q + 1 of row li, so its two
+// loads hit one line; a last step of 128 takes block q.
+// QUANT: A is bf16 and quantised here: a lane holds whole blocks, so their scales and
+// codes need no other lane.  It costs 60 instructions a block, for every 16 NB
+// columns again.
+template <int MB, int NB, int WAVES, bool QUANT>
 __global__ void __launch_bounds__(64 * WAVES) mx_rows_kernel(MxParams p) {
-  __shared__ f32x4 part[WAVES][MB][64];
+  __shared__ f32x4 part[WAVES][MB * NB][64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, q = lane >> 4;
-  const int nt = p.N / 16, mt = blockIdx.x / nt, n0 = (blockIdx.x - mt * nt) * 16, m0 = mt * 16 * MB;
-  const uint8_t* wp = p.W + (int64_t)(n0 + li) * p.ldw + 16 * q;
-  const uint8_t* wsp = p.ws + (int64_t)(n0 + li) * p.ldws + q;
-  const uint8_t* ap[MB];
-  const uint8_t* asp[MB];
+  const int nt = (p.N + 16 * NB - 1) / (16 * NB), mt = blockIdx.x / nt, n0 = (blockIdx.x - mt * nt) * 16 * NB;
+  const int m0 = mt * 16 * MB;
+  const uint8_t *wp[NB], *wsp[NB], *ap[MB], *asp[MB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {  // columns past N repeat the last
+    const int row = min(n0 + 16 * n + li, p.N - 1);
+    wp[n] = p.W + (int64_t)row * p.ldw;
+    wsp[n] = p.ws + (int64_t)row * p.ldws;
+  }
 #pragma unroll
   for (int b = 0; b < MB; ++b) {
     const int m = min(m0 + 16 * b + li, p.M - 1);
-    ap[b] = p.A + (int64_t)m * p.lda + (QUANT ? 64 : 16) * q;
-    asp[b] = QUANT ? nullptr : p.as + (int64_t)m * p.ldas + q;
+    ap[b] = p.A + (int64_t)m * p.lda;
+    asp[b] = QUANT ? nullptr : p.as + (int64_t)m * p.ldas;
   }
-  f32x4 acc[MB];
+  f32x4 acc[MB][NB];
 #pragma unroll
-  for (int b = 0; b < MB; ++b) acc[b] = zero4();
-  const int steps = p.K / 128, each = (steps + WAVES - 1) / WAVES, s_end = min((wave + 1) * each, steps);
-#pragma unroll 4
-  for (int s = wave * each; s < s_end; ++s) {
-    const u32x4 w = *(const u32x4*)(wp + 64 * s);
-    const int ws = wsp[4 * s];
+  for (int b = 0; b < MB; ++b)
+#pragma unroll
+    for (int n = 0; n < NB; ++n) acc[b][n] = zero4();
+  // block `blk` of the contraction against that of the other lanes' q
+  auto block = [&](int blk, const u32x4 (&w)[NB], const int (&ws)[NB]) {
 #pragma unroll
     for (int b = 0; b < MB; ++b) {
+      u32x4 a;
+      uint32_t as;
       if constexpr (QUANT) {
-        const u32x4* x = (const u32x4*)(ap[b] + 256 * s);
-        const u32x4 v[4] = {x[0], x[1], x[2], x[3]};
-        u32x4 codes;
-        uint32_t byte;
-        mx_encode32(v, codes, byte);
-        acc[b] = mfma_mx4(w, codes, acc[b], ws, (int)byte);
+        a = mx_encode32((const u32x4*)(ap[b] + 64 * blk), as);
       } else {
-        acc[b] = mfma_mx4(w, *(const u32x4*)(ap[b] + 64 * s), acc[b], ws, asp[b][4 * s]);
+        a = *(const u32x4*)(ap[b] + 16 * blk);
+        as = asp[b][blk];
       }
+#pragma unroll
+      for (int n = 0; n < NB; ++n) acc[b][n] = mfma_mx4(w[n], a, acc[b][n], ws[n], (int)as);
     }
+  };
+  const int steps = p.K / 256, each = (steps + WAVES - 1) / WAVES, s_end = min((wave + 1) * each, steps);
+#pragma unroll 2
+  for (int s = wave * each; s < s_end; ++s) {
+    const int blk = 8 * s + 2 * q;
+    u32x4 w0[NB], w1[NB];
+    int ws0[NB], ws1[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      w0[n] = *(const u32x4*)(wp[n] + 16 * blk);
+      w1[n] = *(const u32x4*)(wp[n] + 16 * blk + 16);
+      const int both = *(const uint16_t*)(wsp[n] + blk);
+      ws0[n] = both & 255;
+      ws1[n] = both >> 8;
+    }
+    block(blk, w0, ws0);
+    block(blk + 1, w1, ws1);
+  }
+  if ((p.K & 255) && wave == WAVES - 1) {
+    const int blk = 8 * steps + q;
+    u32x4 w0[NB];
+    int ws0[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) w0[n] = *(const u32x4*)(wp[n] + 16 * blk), ws0[n] = wsp[n][blk];
+    block(blk, w0, ws0);
   }
 #pragma unroll
-  for (int b = 0; b < MB; ++b) part[wave][b][lane] = acc[b];
+  for (int b = 0; b < MB; ++b)
+#pragma unroll
+    for (int n = 0; n < NB; ++n) part[wave][b * NB + n][lane] = acc[b][n];
   __syncthreads();
-  if (wave >= MB) return;
-  const int m = m0 + 16 * wave + li;
-  if (m >= p.M) return;
+  if (wave >= MB * NB) return;
+  const int m = m0 + 16 * (wave / NB) + li, n = n0 + 16 * (wave % NB) + 4 * q;
+  if (m >= p.M || n >= p.N) return;
   f32x4 t = part[0][wave][lane];
 #pragma unroll
   for (int w = 1; w < WAVES; ++w) t += part[w][wave][lane];
-  mx_store4(p, m, n0 + 4 * q, t);
+  mx_store4(p, m, n, t);
 }
 
 // Tile form: 256 x 256 outputs a workgroup of 8 waves (2 x 4 of 128 x 64, 4 x 2
@@ -511,16 +553,13 @@ int check_product(const MxParams& p, bool quant) {
     return HSTU_E_UNSUPPORTED;
   return 0;
 }
-template <bool QUANT>
+template <int MB, int NB, bool QUANT>
 int launch_rows(const MxParams& p, hipStream_t stream) {
-  const int mb = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
-  const int64_t tiles = ((int64_t)p.M + 16 * mb - 1) / (16 * mb) * (p.N / 16);
-  if (tiles >= ((int64_t)1 << 31)) return HSTU_E_UNSUPPORTED;
   constexpr int W = 8;
-  const dim3 grid((unsigned)tiles), block(64 * W);
-  if (mb == 1) hipLaunchKernelGGL((mx_rows_kernel<1, W, QUANT>), grid, block, 0, stream, p);
-  else if (mb == 2) hipLaunchKernelGGL((mx_rows_kernel<2, W, QUANT>), grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((mx_rows_kernel<4, W, QUANT>), grid, block, 0, stream, p);
+  static_assert(MB * NB <= W, "a wave joins each block");
+  const int64_t tiles = ((int64_t)p.M + 16 * MB - 1) / (16 * MB) * ((p.N + 16 * NB - 1) / (16 * NB));
+  if (tiles >= ((int64_t)1 << 31)) return HSTU_E_UNSUPPORTED;
+  hipLaunchKernelGGL((mx_rows_kernel<MB, NB, W, QUANT>), dim3((unsigned)tiles), dim3(64 * W), 0, stream, p);
   return (int)hipGetLastError();
 }
 }  // namespace
@@ -541,7 +580,7 @@ extern "C" int hstu_mxfp4_gemm(const void* A, int64_t lda, const void* a_scale, 
                        (int)tiles_n, per_xcd);
     return (int)hipGetLastError();
   }
-  return launch_rows<false>(p, stream);
+  return M <= 16 ? launch_rows<1, 1, false>(p, stream) : M <= 32 ? launch_rows<2, 1, false>(p, stream) : launch_rows<4, 2, false>(p, stream);
 }
 
 extern "C" int hstu_mxfp4_linear_rows(const void* x, int64_t ldx, const void* W, int64_t ldw, const void* w_scale,
@@ -551,5 +590,8 @@ extern "C" int hstu_mxfp4_linear_rows(const void* x, int64_t ldx, const void* W,
              ldws, (const uint16_t*)bias, (const uint16_t*)residual, (uint16_t*)C, ldr, ldc, M, N, K};
   const int st = check_product(p, true);
   if (st != 0 || M == 0) return st;
-  return launch_rows<true>(p, stream);
+  // Two column blocks a workgroup where that still leaves one for every CU: half of
+  // the quantisation (us, one / two: 8 x 8 192 x 8 192 (M x K x N) 17.7 / 13.0, 16 x
+  // 2 048 x 8 192 8.2 / 6.6; 16 x 4 096 x 4 096 8.3 / 9.5, 5 x 5 632 x 2 048 6.9 / 8.2).
+  return N >= 8192 ? launch_rows<1, 2, true>(p, stream) : launch_rows<1, 1, true>(p, stream);
 }

@@ -75,6 +75,35 @@ __device__ __forceinline__ void load8(const uint8_t* row, int c0, int D, float (
     }
   }
 }
+// The same in two parts, so that a row's loads can be issued before its turn.
+// Without VEC the second part loads.
+template <bool F32, bool VEC>
+struct Raw8 {
+  u32x4 v[F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const uint8_t* row, int c0) {
+    if constexpr (VEC) {
+      const u32x4* p = (const u32x4*)(row + (F32 ? 4 : 2) * (int64_t)c0);
+      v[0] = p[0];
+      if constexpr (F32) v[1] = p[1];
+    }
+  }
+  __device__ __forceinline__ void get(const uint8_t* row, int c0, int D, float (&o)[8]) const {
+    if constexpr (!VEC) {
+      load8<F32, false>(row, c0, D, o);
+    } else if constexpr (F32) {
+      const f32x4 a = __builtin_bit_cast(f32x4, v[0]), b = __builtin_bit_cast(f32x4, v[1]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = a[e], o[4 + e] = b[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t x = v[0][e];
+        o[2 * e] = __builtin_bit_cast(float, x << 16);
+        o[2 * e + 1] = __builtin_bit_cast(float, x & 0xffff0000u);
+      }
+    }
+  }
+};
 template <bool F32, bool VEC>
 __device__ __forceinline__ void store8(uint8_t* row, int c0, int D, const float (&v)[8]) {
   if constexpr (VEC && F32) {
@@ -240,21 +269,49 @@ __global__ void __launch_bounds__(BLOCK) rms_bwd_kernel(BwdArgs a) {
       else load8<false, VEC>(a.w, c0, a.D, w[i]);
     }
   }
+  // AHEAD: a row's operands are loaded while the row before it is worked on (a
+  // block with one row at a time otherwise waits for each; measured with the
+  // blocks of bwd_blocks, 4 099 x 5 120 fp32 61.0 -> 53.2 us, 8 192 x 4 096 bf16 63.8 ->
+  // 59.5; rows of one wave overlap by themselves, 162 251 x 512 123.7 -> 128.2)
+  constexpr bool AHEAD = G == 256 || G == 512;
+  Raw8<F32, VEC> hr[NV], yr[NV], dr[NV];
+  float rn = 0.f;
+  auto fetch = [&](int64_t row) {
+    if (row >= a.rows) return;
+    rn = a.rstd[row];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c0 = 8 * (tg + G * i);
+      if (c0 >= a.D) continue;
+      hr[i].load(a.h + row * a.ldh, c0);
+      yr[i].load(a.dy + row * a.lddy, c0);
+      if (a.dh) dr[i].load(a.dh + row * a.lddh, c0);
+    }
+  };
+  if constexpr (AHEAD) fetch((int64_t)blockIdx.x * GROUPS + group);
   int par = 0;
   for (int64_t r0 = (int64_t)blockIdx.x * GROUPS; r0 < a.rows; r0 += (int64_t)gridDim.x * GROUPS, par ^= 1) {
     const int64_t row = r0 + group;
     const bool live = row < a.rows;
-    float h[NV][8], dy[NV][8];
+    float h[NV][8], dy[NV][8], d[NV][8];
     float m = 0.f;
-    const float rstd = live ? a.rstd[row] : 0.f;
+    if constexpr (!AHEAD) fetch(row);
+    const float rstd = live ? rn : 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c0 = 8 * (tg + G * i);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) h[i][e] = dy[i][e] = 0.f;
+      for (int e = 0; e < 8; ++e) h[i][e] = dy[i][e] = d[i][e] = 0.f;
       if (!live || c0 >= a.D) continue;
-      load8<F32, VEC>(a.h + row * a.ldh, c0, a.D, h[i]);
-      load8<F32, VEC>(a.dy + row * a.lddy, c0, a.D, dy[i]);
+      hr[i].get(a.h + row * a.ldh, c0, a.D, h[i]);
+      yr[i].get(a.dy + row * a.lddy, c0, a.D, dy[i]);
+      if constexpr (AHEAD) {
+        if (a.dh) dr[i].get(a.dh + row * a.lddh, c0, a.D, d[i]);
+      }
+    }
+    if constexpr (AHEAD) fetch(row + (int64_t)gridDim.x * GROUPS);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         h[i][e] *= rstd;  // xhat
@@ -262,7 +319,6 @@ __global__ void __launch_bounds__(BLOCK) rms_bwd_kernel(BwdArgs a) {
         dy[i][e] *= w[i][e];  // c
         m = __builtin_fmaf(dy[i][e], h[i][e], m);
       }
-    }
     m = wave_sum(m);
     if constexpr (WPG > 1) {
       if ((tg & 63) == 0) red[par][group][wg] = m;
@@ -277,12 +333,12 @@ __global__ void __launch_bounds__(BLOCK) rms_bwd_kernel(BwdArgs a) {
     for (int i = 0; i < NV; ++i) {
       const int c0 = 8 * (tg + G * i);
       if (c0 >= a.D) continue;
-      float dx[8], d[8];
+      float dx[8];
+      if constexpr (!AHEAD) {
+        if (a.dh) dr[i].get(a.dh + row * a.lddh, c0, a.D, d[i]);
+      }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) d[e] = 0.f;
-      if (a.dh) load8<F32, VEC>(a.dh + row * a.lddh, c0, a.D, d);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) dx[e] = __builtin_fmaf(rstd, __builtin_fmaf(-h[i][e], m, dy[i][e]), d[e]);
+      for (int e = 0; e < 8; ++e) dx[e] = __builtin_fmaf(rstd, __builtin_fmaf(-h[i][e], m, dy[i][e]), d[i][e]);
       store8<F32, VEC>(a.dx + row * a.lddx, c0, a.D, dx);
     }
   }
@@ -313,31 +369,45 @@ __global__ void __launch_bounds__(BLOCK) rms_bwd_kernel(BwdArgs a) {
   }
 }
 
-// dw[c] = sum of the blocks' partials, in a fixed order (16 strided sums, then those)
+// dw[c] = sum of the blocks' partials, in a fixed order: a workgroup owns 16
+// columns, its 64 row lanes sum every 64th partial, four loads in flight, then
+// those sums.  Few columns a workgroup, because the time is the chain of loads.
 __global__ void __launch_bounds__(1024) rms_dw_kernel(const float* __restrict__ part, int blocks, int D, void* dw,
                                                       int f32) {
-  __shared__ float red[16][64];
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), k = threadIdx.x >> 6;
-  float t = 0.f;
-  if (c < D)
-    for (int b = k; b < blocks; b += 16) t += part[(int64_t)b * D + c];
-  red[k][threadIdx.x & 63] = t;
-  __syncthreads();
-  if (k == 0 && c < D) {
-    t = 0.f;
+  __shared__ float red[64][17];
+  const int cl = threadIdx.x & 15, c = blockIdx.x * 16 + cl, k = threadIdx.x >> 4;
+  float t[4] = {0.f, 0.f, 0.f, 0.f};
+  if (c < D) {
+    int b = k;
+    for (; b + 192 < blocks; b += 256)
 #pragma unroll
-    for (int j = 0; j < 16; ++j) t += red[j][threadIdx.x];
-    if (f32) ((float*)dw)[c] = t;
-    else ((uint16_t*)dw)[c] = to_bf16(t);
+      for (int j = 0; j < 4; ++j) t[j] += part[(int64_t)(b + 64 * j) * D + c];
+    for (; b < blocks; b += 64) t[0] += part[(int64_t)b * D + c];
+  }
+  red[k][cl] = (t[0] + t[1]) + (t[2] + t[3]);
+  __syncthreads();
+  // 64 sums -> 4 (a wave's 16 columns x 4) -> 1
+  if (threadIdx.x < 64) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) s += red[16 * k + j][cl];
+    red[16 * k][cl] = s;
+  }
+  __syncthreads();
+  if (threadIdx.x < 16 && c < D) {
+    const float s = (red[0][cl] + red[16][cl]) + (red[32][cl] + red[48][cl]);
+    if (f32) ((float*)dw)[c] = s;
+    else ((uint16_t*)dw)[c] = to_bf16(s);
   }
 }
 
-constexpr int kMaxD = 32768;
+constexpr int kMaxD = 16384;
 // row groups of a backward block: 8 or 16 waves, whose sums for dw meet in 32 KiB of LDS
 int bwd_groups(int D) { return D <= 512 ? 16 : D <= 1024 ? 8 : 1; }
+// as many as the chip holds at a time: their sums are written and read again
 int bwd_blocks(int64_t rows, int D) {
   const int groups = bwd_groups(D);
-  return (int)std::min<int64_t>((rows + groups - 1) / groups, groups > 1 ? 512 : 1024);
+  return (int)std::min<int64_t>((rows + groups - 1) / groups, D <= 1024 ? 512 : D <= 4096 ? 768 : 256);
 }
 
 template <template <bool, bool, int, int> class L, bool F32, bool VEC, typename... A>
@@ -346,9 +416,8 @@ void by_width(int D, A... args) {
   else if (D <= 1024) L<F32, VEC, 64, 2>::go(args...);
   else if (D <= 2048) L<F32, VEC, 256, 1>::go(args...);
   else if (D <= 4096) L<F32, VEC, 256, 2>::go(args...);
-  else if (D <= 8192) L<F32, VEC, 256, 4>::go(args...);
-  else if (D <= 16384) L<F32, VEC, 512, 4>::go(args...);
-  else L<F32, VEC, 1024, 4>::go(args...);
+  else if (D <= 8192) L<F32, VEC, 512, 2>::go(args...);
+  else L<F32, VEC, 1024, 2>::go(args...);
 }
 template <bool F32, bool VEC, int G, int NV>
 struct Fwd {
@@ -469,7 +538,7 @@ extern "C" int hstu_rms_norm_bwd(int dtype, const void* dy, int64_t lddy, const 
                      aligned16(dx, a.lddx) && (!dh || aligned16(dh, a.lddh));
     by_type<Bwd>(f32, vec, D, a, blocks, stream);
   }
-  hipLaunchKernelGGL(rms_dw_kernel, dim3((unsigned)((D + 63) / 64)), dim3(1024), 0, stream, (const float*)workspace,
+  hipLaunchKernelGGL(rms_dw_kernel, dim3((unsigned)((D + 15) / 16)), dim3(1024), 0, stream, (const float*)workspace,
                      blocks, D, dweight, dweight_dtype == HSTU_DTYPE_FP32 ? 1 : 0);
   return (int)hipGetLastError();
 }

@@ -4,7 +4,7 @@
     y = h / sqrt(mean(h^2) + eps) * weight
 
 over the last dimension, for bf16 and fp32 activations and bf16 or fp32
-weights of any width up to 32768.  It stands beside the weighted LayerNorm
+weights of any width up to 16384.  It stands beside the weighted LayerNorm
 (``triton_weighted_layer_norm_fwd``), which the reference norms with
 (``ops/triton/triton_layer_norm.py:1668-1740``); the reference's HSTU layer
 has no RMS norm.
@@ -29,7 +29,7 @@ from . import _lib
 
 E4M3 = torch.float8_e4m3fn
 _TYPES = {torch.bfloat16: _lib.HSTU_DTYPE_BF16, torch.float32: _lib.HSTU_DTYPE_FP32}
-MAX_D = 32768
+MAX_D = 16384
 
 
 def _rows2d(t: torch.Tensor) -> torch.Tensor:

@@ -24,9 +24,14 @@ import torch
 from . import _lib
 
 _TYPES = {torch.bfloat16: _lib.HSTU_DTYPE_BF16, torch.float32: _lib.HSTU_DTYPE_FP32}
-# Up to here the product's kernel quantizes its rows of x itself (one launch, the
-# work repeated for every 16 outputs); beyond, a kernel of its own does it once.
+# Up to here the product's kernel quantizes its rows of x itself, one launch and the
+# work and the reads of x repeated for every 16 or 32 outputs; beyond, a kernel of
+# its own does it once.  Measured (us on the device, one launch / two): 5 x 5632
+# (M x K) against 2048 outputs 6.9 / 7.7, 16 x 4096 against 4096 8.3 / 9.4, 8 x 8192
+# against 8192 13.0 / 14.4; 16 x 8192 against 8192 16.4 / 16.1, against 2048 13.2 /
+# 10.7.  A launch from Python is 8 us of the host's time more.
 ROWS_QUANT = 16
+VALUES_QUANT = 65536
 Packed = Tuple[torch.Tensor, torch.Tensor]
 
 
@@ -152,7 +157,7 @@ def mxfp4_linear(x: torch.Tensor, weight: Packed, bias: Optional[torch.Tensor] =
     if shape[-1] != K or x.device != wc.device:
         raise ValueError(f"x {tuple(shape)} on {x.device} against weight [{N}, {K}] on {wc.device}")
     M = x.numel() // K
-    if M > ROWS_QUANT:
+    if M > ROWS_QUANT or M * K > VALUES_QUANT:
         return mxfp4_mm(quantize_mxfp4(x), weight, bias, residual)
     shape = shape[:-1] + (N,)
     bias, r2 = _epilogue(bias, residual, shape, wc.device)
