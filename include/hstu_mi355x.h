@@ -707,7 +707,7 @@ int hstu_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, i
  * C[m][n] = sum_k A[m][k] W[n][k] [+ bias[n]] [+ residual[m][n]]: A [M, K] and W
  * [N, K] in the format above (ld of codes and scales in bytes, codes' rows
  * 16-byte and scales' rows 4-byte aligned), bias [N], residual and C bf16, fp32
- * accumulation.  N % 16 == 0, K % 128 == 0, any M.
+ * accumulation.  N % 16 == 0, K % 128 == 0, any M; rows less than 2^23 bytes apart.
  */
 int hstu_mxfp4_gemm(const void* A, int64_t lda, const void* a_scale, int64_t ldas, const void* W, int64_t ldw,
                     const void* w_scale, int64_t ldws, const void* bias, const void* residual, int64_t ldr, void* C,

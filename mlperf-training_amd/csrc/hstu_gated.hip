@@ -112,8 +112,8 @@ __device__ __forceinline__ void gated_store(const GatedParams& p, int m, int n, 
 }
 
 // ---------------------------------------------------------------- row form
-// Few rows: the weights' bytes are the time.  A workgroup owns 16 columns and 16 MB
-// rows; its WAVES waves take one contiguous piece of the contraction each, with the
+// Few rows: the weights' bytes are the time.  A workgroup owns 16 columns of all
+// (at most 16 MB) rows; its WAVES waves take one contiguous piece of the contraction each, with the
 // operands going from memory to registers as the MFMA takes them (lane (li, q): bytes
 // 32 q .. 32 q + 31 of each 128 of row li, so both of its loads hit one line), and
 // meet in LDS: wave b sums row block b over the waves in order.
@@ -125,7 +125,8 @@ __global__ void __launch_bounds__(64 * WAVES) gated_rows_kernel(GatedParams p) {
   constexpr int STEP = 128, LB = STEP / 4;  // bytes of a row, and of a lane
   __shared__ f32x4 part[WAVES][2 * MB][64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, q = lane >> 4;
-  const int nt = p.F / 16, mt = blockIdx.x / nt, n0 = (blockIdx.x - mt * nt) * 16, m0 = mt * 16 * MB;
+  constexpr int m0 = 0;  // all rows
+  const int n0 = blockIdx.x * 16;
   const uint8_t* gp = p.wg + (int64_t)(n0 + li) * p.ldwg + LB * q;
   const uint8_t* up = p.wu + (int64_t)(n0 + li) * p.ldwu + LB * q;
   const uint8_t* xp[MB];
@@ -179,6 +180,119 @@ __global__ void __launch_bounds__(64 * WAVES) gated_rows_kernel(GatedParams p) {
     }
   }
   gated_store<BWD, 4>(p, m, n, g, u);
+}
+
+// ---------------------------------------------------------------- middle form
+// Some hundred rows: 128 x 128 tiles leave most CUs idle and one tile's serial
+// k-steps are the time.  This form takes 64 rows x 32 columns of h (64 x 64 of
+// products, 4 waves of 32 rows x 16 columns, two workgroups per CU) through a ring of
+// four 16 KiB stages, three k-steps' loads in flight, one barrier a step.  W rows of a
+// wave in LDS: 16 gate rows, then the 16 up rows of the same columns, permuted so
+// that a lane holds both products of eight (bf16) or four (e4m3) columns.
+constexpr int kFewStages = 4, kFewStage = 2 * 64 * 128;
+
+template <bool F8, bool BWD>
+__global__ void __launch_bounds__(kThreads, 2) gated_few_kernel(GatedParams p) {
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[kFewStages][kFewStage];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  // an XCD runs a contiguous range of column panels: its L2 holds its share of the weights and all of x
+  const int tiles_m = (p.M + 63) / 64, total = tiles_m * (p.F / 32), per_xcd = (total + 7) / 8;
+  const int t = ((int)blockIdx.x & 7) * per_xcd + ((int)blockIdx.x >> 3);
+  if (t >= min((((int)blockIdx.x & 7) + 1) * per_xcd, total)) return;
+  const int nt = t / tiles_m, mt = t - nt * tiles_m;
+  const int m0 = mt * 64, n0 = nt * 32, mrows = min(64, p.M - m0);
+  const int wm = 32 * (wave >> 1), wn = wave & 1;
+  const int nk = p.K >> 7;
+  const int li = lane & 15, q = lane >> 4, lr = lane & 31, h = lane >> 5;
+
+  // wave w fills rows 16 w .. 16 w + 15 of both operands' stages: W rows of one matrix
+  uint32_t av[2], wv[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int s = 64 * (2 * wave + j) + lane, r = s >> 3, i = r & 15;
+    const uint32_t pos = (uint32_t)(((s & 7) ^ wide_swz(r)) * 16);
+    const int col = 16 * (wave >> 1) + (F8 ? i : 8 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3));
+    av[j] = (uint32_t)r * (uint32_t)p.ldx + pos;
+    wv[j] = (uint32_t)col * (uint32_t)(wave & 1 ? p.ldwu : p.ldwg) + pos;
+  }
+  const i32x4 ars = rsrc_sgprs(p.x + (int64_t)m0 * p.ldx, (uint32_t)((mrows - 1) * p.ldx + p.K));
+  const int64_t ldw = wave & 1 ? p.ldwu : p.ldwg;
+  const i32x4 wrs = rsrc_sgprs((wave & 1 ? p.wu : p.wg) + (int64_t)n0 * ldw, (uint32_t)(31 * ldw + p.K));
+  const uint32_t ring0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)&ring[0][0];
+  auto issue = [&](int s) {  // four loads of this wave
+    const uint32_t dst = __builtin_amdgcn_readfirstlane(ring0 + (uint32_t)((s % kFewStages) * kFewStage + 2048 * wave));
+#pragma unroll
+    for (int j = 0; j < 2; ++j) dma_to_lds(dst + 1024 * j, av[j], ars, (uint32_t)(128 * s));
+#pragma unroll
+    for (int j = 0; j < 2; ++j) dma_to_lds(dst + kFewStage / 2 + 1024 * j, wv[j], wrs, (uint32_t)(128 * s));
+  };
+  for (int s = 0; s < min(kFewStages - 1, nk); ++s) issue(s);
+
+  f32x4 acc4[2][2];  // e4m3: [row block][gate, up]
+  f32x16 acc16;      // bf16: gate, then up
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc4[i >> 1][i & 1] = zero4();
+#pragma unroll
+  for (int r = 0; r < 16; ++r) acc16[r] = 0.f;
+  auto kstep = [&](int s, auto vm_c) {
+    // step s has landed when only the later steps' loads are outstanding; the barrier
+    // also frees step s - 1's stage for step s + 3
+    dma_barrier<decltype(vm_c)::value>();
+    if (s + kFewStages - 1 < nk) issue(s + kFewStages - 1);
+    const uint8_t* sa = ring[s % kFewStages] + wm * 128;
+    const uint8_t* sw = ring[s % kFewStages] + kFewStage / 2 + wn * 32 * 128;
+    if constexpr (!F8) {
+      u32x4 a[4], w[4];
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        a[kk] = lds_ld128(sa + lr * 128 + (((2 * kk + h) ^ wide_swz(wm + lr)) * 16));
+        w[kk] = lds_ld128(sw + lr * 128 + (((2 * kk + h) ^ wide_swz(32 * wn + lr)) * 16));
+      }
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) acc16 = mfma32_bf16(w[kk], a[kk], acc16);
+    } else {
+      i32x8 a[2], w[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = 16 * i + li;
+        a[i] = cat8(lds_ld128(sa + r * 128 + ((q ^ wide_swz(wm + r)) * 16)),
+                    lds_ld128(sa + r * 128 + (((q + 4) ^ wide_swz(wm + r)) * 16)));
+        w[i] = cat8(lds_ld128(sw + r * 128 + ((q ^ wide_swz(32 * wn + r)) * 16)),
+                    lds_ld128(sw + r * 128 + (((q + 4) ^ wide_swz(32 * wn + r)) * 16)));
+      }
+#pragma unroll
+      for (int ms = 0; ms < 2; ++ms)
+#pragma unroll
+        for (int ns = 0; ns < 2; ++ns) acc4[ms][ns] = mfma_fp8(w[ns], a[ms], acc4[ms][ns]);
+    }
+  };
+  for (int s = 0; s < nk - 2; ++s) kstep(s, std::integral_constant<int, 8>{});
+  if (nk >= 2) kstep(nk - 2, std::integral_constant<int, 4>{});
+  kstep(nk - 1, std::integral_constant<int, 0>{});
+
+  if constexpr (!F8) {
+    const int r = wm + lr;
+    if (r >= mrows) return;
+    float g[8], u[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) g[e] = acc16[e], u[e] = acc16[8 + e];
+    gated_store<BWD, 8>(p, m0 + r, n0 + 16 * wn + 8 * h, g, u);
+  } else {
+    const int n = n0 + 16 * wn + 4 * q;
+#pragma unroll
+    for (int ms = 0; ms < 2; ++ms) {
+      const int r = wm + 16 * ms + li;
+      if (r >= mrows) continue;
+      const float xs = p.xs[p.xs_row ? m0 + r : 0];
+      float g[4], u[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        g[e] = acc4[ms][0][e] * (xs * p.gs[p.gs_row ? n + e : 0]);
+        u[e] = acc4[ms][1][e] * (xs * p.us[p.us_row ? n + e : 0]);
+      }
+      gated_store<BWD, 4>(p, m0 + r, n, g, u);
+    }
+  }
 }
 
 // ---------------------------------------------------------------- tile form, bf16
@@ -472,24 +586,38 @@ __global__ void __launch_bounds__(256) gated_transpose_kernel(const uint16_t* wg
   }
 }
 
+// Which form.  Rows: 16 columns a workgroup, so F / 16 of them; few rows with at most
+// one a CU, or with many.  Between, 256 < F / 16 <= 512, half of the CUs have two
+// while the middle form's F / 32 tiles have a CU each (us, rows / middle, 8 rows:
+// D = 2 048, F = 4 096 7.3 / 10.5, 5 632 11.8 / 10.7, 8 192 13.3 / 12.2, 10 240 19.3 / 22.4;
+// D = 512, F = 2 048 4.0 / 4.9).  Its two row blocks serve narrow weights (D = 2 048, F =
+// 4 096, 24 rows 9.0 / 10.3, D = 512, F = 2 048, 64 rows 5.4 / 4.7).
+// Middle: up to 1.5 rounds of the chip's 512 places (us, middle / 128 x 128 tiles:
+// 704 tiles 23.3 / 29.7, 1 056 34.6 / 30.0, 1 280 86.7 / 72.8; e4m3 14.0 / 20.2, 21.3 /
+// 20.5), and e4m3 rows of one k-step.
+bool rows_form(int M, int F) { return F <= 4096 ? M <= 32 : F > 8192 && M <= 16; }
+constexpr int kFewMaxTiles = 768;
+
 template <bool F8, bool BWD>
 int launch_gated(GatedParams p, hipStream_t stream) {
-  p.tiles_m = (p.M + 127) / 128;
-  const int64_t big = (int64_t)p.tiles_m * (p.F / 128);
-  if (p.M > 64 && p.K >= 256 && big < (1 << 30)) {
-    const int per_xcd = (int)((big + 7) / 8);
-    if constexpr (F8) hipLaunchKernelGGL(gated_tile_fp8_kernel, dim3(8 * per_xcd), dim3(kDuoThreads), 0, stream, p, per_xcd);
-    else hipLaunchKernelGGL((gated_tile_kernel<BWD>), dim3(8 * per_xcd), dim3(kDuoThreads), 0, stream, p, per_xcd);
+  if (rows_form(p.M, p.F)) {
+    constexpr int W = 4;
+    const dim3 grid(p.F / 16), block(64 * W);
+    if (p.M <= 16) hipLaunchKernelGGL((gated_rows_kernel<F8, 1, W, BWD>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((gated_rows_kernel<F8, 2, W, BWD>), grid, block, 0, stream, p);
     return (int)hipGetLastError();
   }
-  const int mb = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
-  const int64_t tiles = ((int64_t)p.M + 16 * mb - 1) / (16 * mb) * (p.F / 16);
-  if (tiles >= ((int64_t)1 << 31)) return HSTU_E_UNSUPPORTED;
-  const dim3 grid((unsigned)tiles);
-  constexpr int W = 4;
-  if (mb == 1) hipLaunchKernelGGL((gated_rows_kernel<F8, 1, W, BWD>), grid, dim3(64 * W), 0, stream, p);
-  else if (mb == 2) hipLaunchKernelGGL((gated_rows_kernel<F8, 2, W, BWD>), grid, dim3(64 * W), 0, stream, p);
-  else hipLaunchKernelGGL((gated_rows_kernel<F8, 4, W, BWD>), grid, dim3(64 * W), 0, stream, p);
+  const int64_t few = ((int64_t)p.M + 63) / 64 * (p.F / 32), big = ((int64_t)p.M + 127) / 128 * (p.F / 128);
+  if (few <= kFewMaxTiles || p.K < 256) {
+    if (few >= (1 << 30)) return HSTU_E_UNSUPPORTED;
+    hipLaunchKernelGGL((gated_few_kernel<F8, BWD>), dim3((unsigned)((few + 7) / 8 * 8)), dim3(kThreads), 0, stream, p);
+    return (int)hipGetLastError();
+  }
+  if (big >= (1 << 30)) return HSTU_E_UNSUPPORTED;
+  p.tiles_m = (p.M + 127) / 128;
+  const int per_xcd = (int)((big + 7) / 8);
+  if constexpr (F8) hipLaunchKernelGGL(gated_tile_fp8_kernel, dim3(8 * per_xcd), dim3(kDuoThreads), 0, stream, p, per_xcd);
+  else hipLaunchKernelGGL((gated_tile_kernel<BWD>), dim3(8 * per_xcd), dim3(kDuoThreads), 0, stream, p, per_xcd);
   return (int)hipGetLastError();
 }
 

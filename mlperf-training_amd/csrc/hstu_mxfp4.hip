@@ -291,6 +291,116 @@ __global__ void __launch_bounds__(64 * WAVES) mx_rows_kernel(MxParams p) {
   mx_store4(p, m, n, t);
 }
 
+template <int BYTE>
+__device__ __forceinline__ f32x16 mfma32_mx4(u32x4 a, u32x4 b, f32x16 c, int sa, int sb) {
+  const u32x4 z = {0u, 0u, 0u, 0u};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(cat8(a, z), cat8(b, z), c, 4, 4, BYTE, sa, BYTE, sb);
+}
+
+// Middle form, for some hundred rows: 64 x 64 outputs a workgroup of 4 waves (32 x 32
+// each), two workgroups per CU, a ring of four 16 KiB steps (256 values of k) with
+// three steps' loads in flight and one barrier a step; scales of two steps at a time
+// in a ring of four.  Fragments, scale bytes and the last half step as in the tile
+// form below.
+constexpr int kMxFewStages = 4, kMxFewStage = 2 * 64 * 128, kMxFewScales = 4 * 1024;
+__global__ void __launch_bounds__(kThreads, 2) mx_few_kernel(MxParams p) {
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[kMxFewStages][kMxFewStage];
+  __shared__ __attribute__((aligned(1024))) uint8_t sring[4][kMxFewScales];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int tiles_m = (p.M + 63) / 64, total = tiles_m * ((p.N + 63) / 64), per_xcd = (total + 7) / 8;
+  const int t = ((int)blockIdx.x & 7) * per_xcd + ((int)blockIdx.x >> 3);
+  if (t >= min((((int)blockIdx.x & 7) + 1) * per_xcd, total)) return;
+  const int nt = t / tiles_m, mt = t - nt * tiles_m;
+  const int m0 = mt * 64, n0 = nt * 64, mrows = min(64, p.M - m0), ncols = min(64, p.N - n0);
+  const int wm = 32 * (wave >> 1), wn = 32 * (wave & 1);
+  const int S = (p.K + 255) >> 8;
+  const int lr = lane & 31, h = lane >> 5;
+  auto column = [](int r) {  // output column (in the tile) of LDS row r of W
+    const int i = r & 31;
+    return (r & ~31) + duo32_col((i >> 2) & 1, 4 * (i >> 3) + (i & 3));
+  };
+  // wave w fills rows 16 w .. 16 w + 15 of both operands, and the scales of 32 rows:
+  // A's (waves 0, 1) or W's (2, 3), each twice in its KiB
+  uint32_t av[2], wv[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int s = 64 * (2 * wave + j) + lane, r = s >> 3;
+    const uint32_t pos = (uint32_t)(((s & 7) ^ ((r >> 1) & 7)) * 16);
+    av[j] = (uint32_t)r * (uint32_t)p.lda + pos;
+    wv[j] = (uint32_t)column(r) * (uint32_t)p.ldw + pos;
+  }
+  const bool sw_wave = wave >= 2;
+  const int sr = 32 * (wave & 1) + lr;
+  const uint32_t sv = sw_wave ? (uint32_t)column(sr) * (uint32_t)p.ldws : (uint32_t)sr * (uint32_t)p.ldas;
+  // rows past M and N read as zero (code 0, scale byte 0)
+  const i32x4 ars = rsrc_sgprs(p.A + (int64_t)m0 * p.lda, (uint32_t)((mrows - 1) * p.lda + p.K / 2));
+  const i32x4 wrs = rsrc_sgprs(p.W + (int64_t)n0 * p.ldw, (uint32_t)((ncols - 1) * p.ldw + p.K / 2));
+  const i32x4 srs = rsrc_sgprs(sw_wave ? p.ws + (int64_t)n0 * p.ldws : p.as + (int64_t)m0 * p.ldas,
+                               sw_wave ? (uint32_t)((ncols - 1) * p.ldws + p.K / 32) : (uint32_t)((mrows - 1) * p.ldas + p.K / 32));
+  const uint32_t ring0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)&ring[0][0];
+  const uint32_t sring0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)&sring[0][0];
+  auto issue = [&](int s) {  // four loads of this wave, five in an even step
+    const uint32_t dst = __builtin_amdgcn_readfirstlane(ring0 + (uint32_t)((s % kMxFewStages) * kMxFewStage + 2048 * wave));
+    if ((s & 1) == 0)
+      dma_to_lds(__builtin_amdgcn_readfirstlane(sring0 + (uint32_t)(((s >> 1) & 3) * kMxFewScales + 1024 * wave)), sv, srs,
+                 (uint32_t)(8 * s));
+#pragma unroll
+    for (int j = 0; j < 2; ++j) dma_to_lds(dst + 1024 * j, av[j], ars, (uint32_t)(128 * s));
+#pragma unroll
+    for (int j = 0; j < 2; ++j) dma_to_lds(dst + kMxFewStage / 2 + 1024 * j, wv[j], wrs, (uint32_t)(128 * s));
+  };
+  for (int s = 0; s < min(kMxFewStages - 1, S); ++s) issue(s);
+
+  f32x16 acc;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+  const uint32_t rd = lr * 128 + (((4 * h) ^ ((lr >> 1) & 7)) * 16);  // chunk 4 h + kk at rd ^ 16 kk
+  auto kstep = [&](int s, auto vm_c, bool half) {
+    // Step s has landed when only the two later steps' loads are outstanding (nine);
+    // the barrier also frees step s - 1's place for step s + 3.
+    dma_barrier<decltype(vm_c)::value>();
+    if (s + kMxFewStages - 1 < S) issue(s + kMxFewStages - 1);
+    const uint8_t* sa = ring[s % kMxFewStages] + wm * 128;
+    const uint8_t* sw = ring[s % kMxFewStages] + kMxFewStage / 2 + wn * 128;
+    const uint8_t* sc = sring[(s >> 1) & 3] + 16 * lr + 8 * (s & 1) + 4 * h;
+    u32x4 a[4], w[4];
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      a[kk] = lds_ld128(sa + (rd ^ (16 * kk)));
+      w[kk] = lds_ld128(sw + (rd ^ (16 * kk)));
+    }
+    int as = *(const int*)(sc + 1024 * (wave >> 1)), ws = *(const int*)(sc + 2048 + 1024 * (wave & 1));
+    if (half && h == 1) {  // a last step of 128 values: half 1 has none
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) w[kk] = u32x4{0u, 0u, 0u, 0u};
+      as = ws = 0;
+    }
+    acc = mfma32_mx4<0>(w[0], a[0], acc, ws, as);
+    acc = mfma32_mx4<1>(w[1], a[1], acc, ws, as);
+    acc = mfma32_mx4<2>(w[2], a[2], acc, ws, as);
+    acc = mfma32_mx4<3>(w[3], a[3], acc, ws, as);
+  };
+  for (int s = 0; s < S - 2; ++s) kstep(s, std::integral_constant<int, 9>{}, false);
+  if (S >= 2) kstep(S - 2, std::integral_constant<int, 4>{}, false);
+  kstep(S - 1, std::integral_constant<int, 0>{}, (p.K & 255) != 0);
+
+  // lane: row m0 + wm + lr, columns n0 + wn + 16 run + 8 h + (0..7)
+  const int m = m0 + wm + lr;
+  if (m >= p.M) return;
+#pragma unroll
+  for (int run = 0; run < 2; ++run) {
+    const int c = n0 + wn + 16 * run + 8 * h;
+    if (c >= p.N) continue;
+    float o[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = acc[8 * run + e];
+    if (p.bias) add8(*(const u32x4*)(p.bias + c), o);
+    if (p.resid) add8(*(const u32x4*)(p.resid + (int64_t)m * p.ldr + c), o);
+    *(u32x4*)(p.C + (int64_t)m * p.ldc + c) =
+        u32x4{pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7])};
+  }
+}
+
 // Tile form: 256 x 256 outputs a workgroup of 8 waves (2 x 4 of 128 x 64, 4 x 2
 // accumulators of 32 x 32), v_mfma_scale_f32_32x32x64_f8f6f4.
 //  * A step is 256 values of k, 128 bytes of each row: 64 KiB, in a ring of two,
@@ -314,12 +424,6 @@ constexpr int kMxOperand = kMxTile * 128;    // 32 KiB
 constexpr int kMxStage = 2 * kMxOperand;     // A, W
 constexpr int kMxScales = 2 * kMxTile * 16;  // 16 bytes for each row of A and W: two steps
 constexpr int kMxLds = 2 * kMxStage + 2 * kMxScales;
-
-template <int BYTE>
-__device__ __forceinline__ f32x16 mfma32_mx4(u32x4 a, u32x4 b, f32x16 c, int sa, int sb) {
-  const u32x4 z = {0u, 0u, 0u, 0u};
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(cat8(a, z), cat8(b, z), c, 4, 4, BYTE, sa, BYTE, sb);
-}
 
 __global__ void __launch_bounds__(kMxThreads, 2) mx_tile_kernel(MxParams p, int tiles_m, int tiles_n, int per_xcd) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
@@ -541,6 +645,14 @@ extern "C" int hstu_mxfp4_dequantize(const void* codes, const void* scales, int6
 }
 
 namespace {
+// Rows: up to 16, and up to 32 for narrow outputs, where a middle tile's serial steps
+// would be the time on a few CUs (us, rows / middle, M x K x N: 32 x 8 192 x 1 024 9.9 /
+// 12.0, 32 x 5 632 x 2 048 7.0 / 9.0, 16 x 5 632 x 2 048 5.2 / 8.9; 32 x 2 048 x 5 632 6.3 /
+// 4.9, 32 x 8 192 x 8 192 18.9 / 12.0).  Middle: up to three rounds of the chip's 512
+// places (us, middle / 256 x 256 tiles: 1 024 tiles 36.9 / 52.7, 1 408 16.7 / 18.3, 2 048
+// 23.8 / 19.9 and 78.2 / 59.0).
+bool mx_rows_form(int M, int N) { return M <= 16 || (M <= 32 && N <= 2048); }
+constexpr int kMxFewTiles = 1536;
 int check_product(const MxParams& p, bool quant) {
   if (p.M < 0 || p.N <= 0 || p.K <= 0 || p.ldw < p.K / 2 || p.ldws < p.K / 32 || p.ldc < p.N || (p.resid && p.ldr < p.N) ||
       (quant ? p.lda < 2 * (int64_t)p.K : p.lda < p.K / 2 || p.ldas < p.K / 32))
@@ -551,6 +663,8 @@ int check_product(const MxParams& p, bool quant) {
       (p.lda | p.ldw) % 16 || ((uintptr_t)p.as | (uintptr_t)p.ws) % 4 || (p.ldas | p.ldws) % 4 || p.ldc % 8 ||
       (p.resid && p.ldr % 8))
     return HSTU_E_UNSUPPORTED;
+  // 32-bit offsets of a tile's rows
+  if ((p.lda | p.ldw | p.ldas | p.ldws) >> 23) return HSTU_E_UNSUPPORTED;
   return 0;
 }
 template <int MB, int NB, bool QUANT>
@@ -571,16 +685,20 @@ extern "C" int hstu_mxfp4_gemm(const void* A, int64_t lda, const void* a_scale, 
              ldws, (const uint16_t*)bias, (const uint16_t*)residual, (uint16_t*)C, ldr, ldc, M, N, K};
   const int st = check_product(p, false);
   if (st != 0 || M == 0) return st;
+  if (mx_rows_form(M, N)) return M <= 16 ? launch_rows<1, 1, false>(p, stream) : launch_rows<2, 1, false>(p, stream);
+  const int64_t few = ((int64_t)M + 63) / 64 * ((N + 63) / 64);
   const int64_t tiles_m = ((int64_t)M + kMxTile - 1) / kMxTile, tiles_n = (N + kMxTile - 1) / kMxTile;
-  if (M > 64 && tiles_m * tiles_n < (1 << 30) && (int64_t)kMxTile * std::max(lda, ldw) < ((int64_t)1 << 31)) {
-    hipError_t e = set_mx_lds((const void*)mx_tile_kernel);
-    if (e != hipSuccess) return (int)e;
-    const int per_xcd = (int)((tiles_m * tiles_n + 7) / 8);
-    hipLaunchKernelGGL(mx_tile_kernel, dim3(8 * per_xcd), dim3(kMxThreads), kMxLds, stream, p, (int)tiles_m,
-                       (int)tiles_n, per_xcd);
+  if (few <= kMxFewTiles) {
+    hipLaunchKernelGGL(mx_few_kernel, dim3((unsigned)((few + 7) / 8 * 8)), dim3(kThreads), 0, stream, p);
     return (int)hipGetLastError();
   }
-  return M <= 16 ? launch_rows<1, 1, false>(p, stream) : M <= 32 ? launch_rows<2, 1, false>(p, stream) : launch_rows<4, 2, false>(p, stream);
+  if (tiles_m * tiles_n >= (1 << 30)) return HSTU_E_UNSUPPORTED;
+  hipError_t e = set_mx_lds((const void*)mx_tile_kernel);
+  if (e != hipSuccess) return (int)e;
+  const int per_xcd = (int)((tiles_m * tiles_n + 7) / 8);
+  hipLaunchKernelGGL(mx_tile_kernel, dim3(8 * per_xcd), dim3(kMxThreads), kMxLds, stream, p, (int)tiles_m, (int)tiles_n,
+                     per_xcd);
+  return (int)hipGetLastError();
 }
 
 extern "C" int hstu_mxfp4_linear_rows(const void* x, int64_t ldx, const void* W, int64_t ldw, const void* w_scale,

@@ -48,7 +48,8 @@ def h_bound(x, wg, wu, name):
 
 
 SHAPES = [(1, 256, 128), (3, 256, 128), (16, 512, 256), (17, 512, 384), (33, 256, 640), (64, 512, 128), (65, 768, 128),
-          (127, 512, 256), (129, 512, 256), (300, 1024, 384), (1027, 512, 2048), (2050, 256, 512), (4100, 512, 640)]
+          (127, 512, 256), (129, 512, 256), (300, 1024, 384), (9, 256, 5632), (1027, 512, 2048), (2050, 256, 512),
+          (4100, 512, 640), (2100, 256, 1024), (1700, 768, 1152)]
 
 
 @gpu
@@ -96,7 +97,8 @@ def test_backward(hip_lib, M, D, F, name):
 @gpu
 @pytest.mark.parametrize("modes", [(0, 0), (1, 1), (1, 0), (0, 1)])
 @pytest.mark.parametrize("M,D,F", [(1, 128, 128), (5, 384, 128), (17, 512, 256), (65, 256, 384), (129, 1024, 128),
-                                   (300, 640, 256), (1027, 512, 1024), (4100, 256, 512)])
+                                   (300, 640, 256), (1027, 512, 1024), (9, 128, 5632), (4100, 256, 512), (2100, 384, 1024),
+                                   (1700, 640, 1152)])
 def test_e4m3(hip_lib, M, D, F, modes):
     import hstu_amd
 
@@ -236,9 +238,9 @@ def test_rows_past_the_last_are_left(hip_lib):
     """The C entry writes M rows and F columns of a larger buffer, nothing else."""
     import hstu_amd._lib as lib
 
-    D, F = 256, 128
+    D, F = 256, 640
     wg, wu = weights(F, D)
-    for M in (1, 17, 130, 4100):
+    for M in (1, 17, 130, 4100):  # every form
         x = rnd((M, D), 13).to(DEV)
         out = torch.full((M + 140, F + 8), 7.0, dtype=torch.bfloat16, device=DEV)
         st = lib.fn("hstu_gated_fwd")(x.data_ptr(), D, wg.data_ptr(), D, wu.data_ptr(), D, M, F, D, 0, out.data_ptr(),

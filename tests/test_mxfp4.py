@@ -121,7 +121,9 @@ def test_quantize_strides_and_shapes(hip_lib):
 @pytest.mark.parametrize("bias", [False, True])
 @pytest.mark.parametrize("M,N,K", [(1, 16, 128), (3, 48, 256), (16, 64, 384), (17, 80, 128), (33, 272, 640),
                                    (64, 128, 512), (65, 256, 256), (130, 272, 1152), (257, 512, 1024), (300, 1040, 384),
-                                   (1027, 528, 2048), (2050, 768, 256), (515, 2064, 896)])
+                                   (1027, 528, 2048), (2050, 768, 256), (515, 2064, 896),
+                                   (2600, 2576, 128), (2600, 2576, 256), (2600, 2576, 384), (2600, 2576, 512),
+                                   (2600, 2576, 640), (2600, 2576, 768), (2600, 2576, 1024), (2600, 2576, 1152)])
 def test_product(hip_lib, M, N, K, bias, residual):
     import hstu_amd
 
@@ -150,7 +152,7 @@ def test_product_special_values(hip_lib):
     """NaN blocks make their rows (columns) NaN and no others; zero blocks and far scales are exact."""
     import hstu_amd
 
-    for M in (4, 40, 300):
+    for M in (4, 40, 300, 20000):  # every form
         K, N = 256, 272
         x, w = rnd((M, K), 8).to(DEV), rnd((N, K), 9).to(DEV)
         x[1, 64:96] = 0
@@ -174,7 +176,7 @@ def test_each_scale_and_block_has_its_place(hip_lib):
     """One value in each block in turn, every block with a scale of its own."""
     import hstu_amd
 
-    for M, N, K in ((5, 32, 512), (40, 48, 512), (260, 272, 1024)):
+    for M, N, K in ((5, 32, 512), (40, 48, 512), (260, 272, 1024), (6300, 1040, 1024)):
         blocks = K // 32
         x = torch.zeros((M, K), device=DEV)
         w = torch.zeros((N, K), device=DEV)
@@ -194,7 +196,7 @@ def test_rows_past_the_last_are_left_and_strides(hip_lib):
     import hstu_amd._lib as lib
 
     N, K = 272, 256
-    for M in (1, 17, 130, 1030):
+    for M in (1, 17, 130, 20000):  # every form
         a, w = hstu_amd.quantize_mxfp4(rnd((M, K), 10).to(DEV)), hstu_amd.quantize_mxfp4(rnd((N, K), 11).to(DEV))
         want = hstu_amd.mxfp4_mm(a, w)
         out = torch.full((M + 260, N + 8), 7.0, dtype=torch.bfloat16, device=DEV)
