@@ -25,8 +25,6 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .fp8 import bf16_gemm
-from .wgrad import wgrad
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "sigmoid": 2}
 E4M3 = torch.float8_e4m3fn
@@ -114,14 +112,23 @@ def gated_linear_bwd(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_
         _lib.launch("hstu_gated_bwd", x, d2.data_ptr(), _ld(d2), x2.data_ptr(), _ld(x2), g.data_ptr(), _ld(g),
                     u.data_ptr(), _ld(u), M, F, D, act, dgu.data_ptr(), 2 * F)
     dx = dg = du = None
-    with torch.cuda.device(device):
-        if need_dx:  # the contraction runs over both halves of dgu: the weights side by side, transposed
-            wt = torch.empty((D, 2 * F), dtype=torch.bfloat16, device=device)
-            _lib.launch("hstu_gated_transpose", x, g.data_ptr(), _ld(g), u.data_ptr(), _ld(u), F, D, wt.data_ptr(), 2 * F)
-            dx = bf16_gemm(dgu, wt).view(x.shape)
-        if need_dw:
-            dw = wgrad(dgu, x2, split=_wgrad_split(M, 2 * F, D))
-            dg, du = dw[:F], dw[F:]
+    bf16 = _lib.HSTU_DTYPE_BF16
+    if need_dx:  # the contraction runs over both halves of dgu: the weights side by side, transposed
+        wt = torch.empty((D, 2 * F), dtype=torch.bfloat16, device=device)
+        dx = torch.empty(x.shape, dtype=torch.bfloat16, device=device)
+        _lib.launch("hstu_gated_transpose", x, g.data_ptr(), _ld(g), u.data_ptr(), _ld(u), F, D, wt.data_ptr(), 2 * F)
+        _lib.launch("hstu_bf16_gemm", x, dgu.data_ptr(), 2 * F, wt.data_ptr(), 2 * F, None, None, 0, dx.data_ptr(), D, M,
+                    D, 2 * F, 0, 0)
+    if need_dw:
+        split = _wgrad_split(M, max(2 * F, _ld(x2)))
+        if split < 0:  # rows too far apart for its offsets
+            x2, split = x2.contiguous(), _wgrad_split(M, 2 * F)
+        nbytes = _lib.fn("hstu_wgrad_workspace_bytes")(M, 2 * F, D, split)
+        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
+        dw = torch.empty((2 * F, D), dtype=torch.bfloat16, device=device)
+        _lib.launch("hstu_wgrad", x, bf16, dgu.data_ptr(), 2 * F, bf16, x2.data_ptr(), _ld(x2), M, 2 * F, D, None, None,
+                    dw.data_ptr(), D, bf16, None, split, ws.data_ptr(), nbytes)
+        dg, du = dw[:F], dw[F:]
     return dx, dg, du
 
 
@@ -131,11 +138,11 @@ def gated_linear_bwd(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_
 RECOMPUTE_BELOW = 1024
 
 
-def _wgrad_split(T: int, n1: int, n2: int) -> Optional[int]:
-    """Token ranges for the weight gradient: the kernel's own choice, more where
-    a range's rows would pass its 32-bit offsets."""
-    most = (2 ** 31) // (2 * max(n1, n2)) - 256
-    return None if T <= most else -(-T // most)
+def _wgrad_split(T: int, ld: int) -> int:
+    """Token ranges for the weight gradient: the kernel's own choice (0), more where
+    a range's rows would pass its 32-bit offsets; -1 where none would do."""
+    most = (2 ** 31) // (2 * ld) - 256
+    return -1 if most < 256 else 0 if T <= most else -(-T // most)
 
 
 class GatedLinearFunction(torch.autograd.Function):

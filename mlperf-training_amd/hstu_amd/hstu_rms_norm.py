@@ -135,23 +135,41 @@ def rms_norm_bwd(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, rstd: 
 
 class RMSNormFunction(torch.autograd.Function):
     """Autograd of the norm: (y, h) from (x, residual, weight).  A gradient
-    that nothing asks for is None and costs nothing."""
+    that nothing asks for is None and costs nothing.  What the backward needs
+    besides tensors is settled in the forward: the engine runs it on a thread of
+    its own, where every Python operation costs more."""
 
     @staticmethod
     def forward(ctx, x, weight, eps, residual):
         ctx.set_materialize_grads(False)
         y, h, rstd, _ = rms_norm_fwd(x, weight, eps, residual)
         ctx.save_for_backward(h, weight, rstd)
-        ctx.has_residual = residual is not None
-        return (y, h) if ctx.has_residual else y
+        D = h.shape[-1]
+        rows = rstd.shape[0]
+        ctx.plan = (_TYPES[h.dtype], _TYPES[weight.dtype], rows, D,
+                    _lib.fn("hstu_rms_norm_bwd_workspace_bytes")(rows, D), h.shape, h.dtype, h.device,
+                    residual is not None)
+        return (y, h) if residual is not None else y
 
     @staticmethod
     def backward(ctx, dy, dh=None):
-        h, weight, rstd = ctx.saved_tensors
         if dy is None:  # only h was used
             return dh, None, None, dh
-        dx, dw = rms_norm_bwd(dy, h, weight, rstd, dh)
-        return dx, dw if ctx.needs_input_grad[1] else None, None, dx if ctx.has_residual else None
+        h, weight, rstd = ctx.saved_tensors
+        code, wcode, rows, D, nbytes, shape, dtype, device, has_residual = ctx.plan
+        h2, dy2 = _rows2d(h), _rows2d(dy)
+        d_ptr = d_ld = 0
+        if dh is not None:
+            d2 = _rows2d(dh)
+            d_ptr, d_ld = d2.data_ptr(), _ld(d2)
+        w = weight if weight.stride(0) == 1 else weight.contiguous()
+        dx = torch.empty(shape, dtype=dtype, device=device)
+        dw = torch.empty(D, dtype=weight.dtype, device=device)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        _lib.launch("hstu_rms_norm_bwd", h, code, dy2.data_ptr(), _ld(dy2), h2.data_ptr(), _ld(h2), d_ptr, d_ld,
+                    w.data_ptr(), wcode, rstd.data_ptr(), rows, D, dx.data_ptr(), D, dw.data_ptr(), wcode,
+                    ws.data_ptr(), nbytes)
+        return dx, dw, None, dx if has_residual else None
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None):
