@@ -975,14 +975,26 @@ __global__ void __launch_bounds__(kDuoThreads, 2) fp8_gemm_duo_kernel(GemmParams
 // rows 124 -> 102, 80 -> 70, 96 -> 83 us.  With few rows the tiles no longer
 // cover the chip and a tile's serial k-steps (0.87 us each) are the time; those
 // calls take gemm_few_rows_kernel, or the tile kernel in between (hstu_bf16_gemm).
+// Tile order: up to 8 column tiles (N <= 2 048) one row panel's tiles run together;
+// with more, an XCD's 64 running tiles would share one or two panels of A and read
+// all of W, so they go in groups of 8 row panels (us, panel by panel / in groups:
+// 8 192 x 8 192 x 8 192 1 168 / 856, 8 192 x 4 096 (N) x 20 480 1 153 / 1 128; at N = 512 and
+// 2 048 the same or 3 % slower).
+constexpr int kPanelTiles = 8;
+
 template <bool RESID>
 __global__ void __launch_bounds__(kDuoThreads, 2) bf16_gemm_duo_kernel(GemmParams p, int per_xcd) {
   __shared__ __attribute__((aligned(1024))) uint8_t ring[kDuoSlots][kDuoItem];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int xcd = (int)blockIdx.x & 7;
-  const int t = xcd * per_xcd + ((int)blockIdx.x >> 3);
-  if (t >= min((xcd + 1) * per_xcd, p.tiles_m * p.tiles_n)) return;
-  const int mt = t / p.tiles_n, nt = t - mt * p.tiles_n;
+  int mt, nt;
+  if (p.tiles_n <= kPanelTiles) {  // row panel by row panel
+    const int xcd = (int)blockIdx.x & 7, t = xcd * per_xcd + ((int)blockIdx.x >> 3);
+    if (t >= min((xcd + 1) * per_xcd, p.tiles_m * p.tiles_n)) return;
+    mt = t / p.tiles_n;
+    nt = t - mt * p.tiles_n;
+  } else if (!tile_of(p.tiles_m, p.tiles_n, per_xcd, mt, nt)) {
+    return;
+  }
   const int m0 = mt * kBM, n0 = nt * kWideBN, mrows = min(kBM, p.M - m0);
   const int nk = p.K >> 7;  // K in bytes
 
