@@ -296,6 +296,36 @@ def launch(name: str, t, *args) -> None:
         check(status, name)
 
 
+def guard_graph(ctx, t) -> None:
+    """Called in an autograd function's forward: refuses a graph capture while a
+    graph built outside it on the default stream holds one of the same leaves.
+    The leaf's accumulation belongs to the stream it was first used on, and a
+    captured backward that crosses to the default stream ends the process; so
+    eager uses mark the leaf's accumulation node, which lives as long as such a
+    graph does, and a capture looks for the mark."""
+    if stream(t) == 0:
+        for node, _ in ctx.next_functions:
+            if node is not None and not node.next_functions:
+                node.metadata["hstu_default_stream"] = True
+        return
+    import torch
+
+    if torch.cuda.is_current_stream_capturing():
+        for node, _ in ctx.next_functions:
+            if node is not None and not node.next_functions and "hstu_default_stream" in node.metadata:
+                raise HstuKernelError("graph capture of a function of a leaf that a graph outside the capture, built on "
+                                      "the default stream, still holds: let go of that graph's outputs first, or warm "
+                                      "up on a side stream")
+
+
+def refuse_second_derivatives() -> None:
+    """Called in an autograd function's backward, which runs with gradients enabled only under create_graph."""
+    import torch
+
+    if torch.is_grad_enabled():
+        raise NotImplementedError("second derivatives (create_graph=True)")
+
+
 def ptr(t) -> Optional[int]:
     """Device address of a tensor (None for None)."""
     return None if t is None else t.data_ptr()

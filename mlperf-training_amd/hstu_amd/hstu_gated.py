@@ -133,9 +133,12 @@ def gated_linear_bwd(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_
 
 
 # Keeping g and u costs 16 bytes of memory traffic a value (written and read in
-# fp32), computing them again 4 D operations: equal near D = 900 at this card's
-# rates.  Measured (us a training step, kept / computed again): KEPT_FIGURES
-RECOMPUTE_BELOW = 1024
+# fp32), computing them again 4 D operations: equal near D = 1200 at the rates that
+# these kernels reach.  Measured (us on the device a training step, computed again /
+# kept): 37 429 rows x 512 -> 2048 714 / 838, 16 384 x 768 -> 3584 745 / 809, 16 384 x
+# 1024 -> 4096 1030 / 1107, 16 384 x 1280 -> 5120 1628 / 1594, 16 384 x 2048 -> 5632
+# 2721 / 2440, 8192 x 4096 -> 10240 4588 / 3755, 512 x 2048 -> 5632 176 / 154.
+RECOMPUTE_BELOW = 1280
 
 
 def _wgrad_split(T: int, ld: int) -> int:
@@ -150,16 +153,16 @@ class GatedLinearFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w_gate, w_up, activation, keep):
+        h = gated_linear_fwd(x, w_gate, w_up, activation, keep)
+        h, gu = h if keep else (h, None)
+        _lib.guard_graph(ctx, x)
         ctx.activation = activation
-        if not keep:
-            ctx.save_for_backward(x, w_gate, w_up, None)
-            return gated_linear_fwd(x, w_gate, w_up, activation)
-        h, gu = gated_linear_fwd(x, w_gate, w_up, activation, keep=True)
         ctx.save_for_backward(x, w_gate, w_up, gu)
         return h
 
     @staticmethod
     def backward(ctx, dh):
+        _lib.refuse_second_derivatives()
         x, w_gate, w_up, gu = ctx.saved_tensors
         need_x, need_g, need_u = ctx.needs_input_grad[:3]
         dx, dg, du = gated_linear_bwd(dh, x, w_gate, w_up, ctx.activation, need_x, need_g or need_u, gu)
@@ -171,8 +174,8 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, acti
     """a(x @ w_gate^T) * (x @ w_up^T): x [.., D], weights [F, D], h [.., F], bf16.
     Differentiable in x and both weights.  ``recompute``: the backward computes g
     and u again (nothing but x and the weights is kept) instead of keeping them
-    in fp32, 8 bytes a value of h; None: where that is the faster way (D < 1024).
-    The gradients are the same bytes."""
+    in fp32, 8 bytes a value of h; None: where that is the faster way (D < 1280).
+    The gradients are the same bytes.  Not differentiable a second time."""
     if not (torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad)):
         return gated_linear_fwd(x, w_gate, w_up, activation)
     if recompute is None:
@@ -191,7 +194,8 @@ def _scale(name: str, s: torch.Tensor, n: int, x: torch.Tensor) -> Tuple[torch.T
 def gated_linear_fp8(x8: torch.Tensor, x_scale: torch.Tensor, gate: Scaled, up: Scaled, activation: str = "silu"
                      ) -> torch.Tensor:
     """The forward from e4m3: x8 [.., D] with one fp32 scale or one a row, and
-    ``gate``, ``up`` as pairs (e4m3 [F, D], scale: one or [F]).  h [.., F] in bf16."""
+    ``gate``, ``up`` as pairs (e4m3 [F, D], scale: one or [F]).  h [.., F] in bf16,
+    which carries no gradient."""
     act = _act(activation)
     (g8, gs), (u8, us) = gate, up
     F, D = _check(x8, g8, u8, E4M3, 128)

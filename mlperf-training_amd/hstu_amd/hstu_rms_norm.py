@@ -143,6 +143,7 @@ class RMSNormFunction(torch.autograd.Function):
     def forward(ctx, x, weight, eps, residual):
         ctx.set_materialize_grads(False)
         y, h, rstd, _ = rms_norm_fwd(x, weight, eps, residual)
+        _lib.guard_graph(ctx, x)
         ctx.save_for_backward(h, weight, rstd)
         D = h.shape[-1]
         rows = rstd.shape[0]
@@ -153,6 +154,7 @@ class RMSNormFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, dh=None):
+        _lib.refuse_second_derivatives()
         if dy is None:  # only h was used
             return dh, None, None, dh
         h, weight, rstd = ctx.saved_tensors
@@ -175,7 +177,7 @@ class RMSNormFunction(torch.autograd.Function):
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None):
     """``y``, or ``(y, h)`` with a residual: h = x + residual is the new residual
     stream and y its norm times ``weight``.  Differentiable in x, residual and
-    weight, through y and h."""
+    weight, through y and h; not a second time."""
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
                                     or (residual is not None and residual.requires_grad)):
         return RMSNormFunction.apply(x, weight, eps, residual)
@@ -187,6 +189,6 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
                  scale: Optional[torch.Tensor] = None):
     """``(y8, scale)`` or, with a residual, ``(y8, scale, h)``: the norm in e4m3,
     y = y8 * scale with one fp32 scale a row ([rows], max|y| / 448) or the given
-    one (returned as [1])."""
+    one (returned as [1]).  Forward only: nothing returned carries a gradient."""
     y8, h, _, s = rms_norm_fwd(x, weight, eps, residual, output_fp8=True, scale=scale, want_rstd=False)
     return (y8, s) if residual is None else (y8, s, h)

@@ -149,7 +149,8 @@ def mxfp4_mm(a: Packed, weight: Packed, bias: Optional[torch.Tensor] = None,
 
 def mxfp4_linear(x: torch.Tensor, weight: Packed, bias: Optional[torch.Tensor] = None,
                  residual: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """quantize(x) @ weight^T (+ bias) (+ residual) in bf16, for bf16 x [.., K]."""
+    """quantize(x) @ weight^T (+ bias) (+ residual) in bf16, for bf16 x [.., K].
+    Forward only: the result carries no gradient."""
     if x.dtype != torch.bfloat16:
         raise NotImplementedError(f"x: bf16 (got {x.dtype})")
     wc, ws, N, K = _weight(weight)
