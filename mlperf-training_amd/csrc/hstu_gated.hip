@@ -30,19 +30,22 @@ constexpr float kGelu1 = 1.5957691216057308f;  // 2 sqrt(2 / pi)
 constexpr float kGelu3 = 0.044715f;
 
 // a(g), and a'(g) with DERIV.  1 - s(z) is taken as e^-z s(z), which keeps the
-// digits that a subtraction from 1 would lose; e^-z is held below 2^126, so
-// that s stays a normal number.
+// digits that a subtraction from 1 would lose.  Where e^-z passes 2^126, s is 0
+// (its value is under 2^-126, and g may be anything); gelu's cubic is taken at 64
+// at the most, where s is 0 or 1 in fp32 and the cube still a number.
 template <bool DERIV>
 __device__ __forceinline__ void act(int kind, float g, float& a, float& da) {
   float z = g, dz = 1.f;
   if (kind == kGelu) {
-    const float q = kGelu3 * g * g;
-    z = kGelu1 * __builtin_fmaf(q, g, g);
+    const float c = __builtin_fabsf(g) > 64.f ? __builtin_copysignf(64.f, g) : g;  // NaN stays
+    const float q = kGelu3 * c * c;
+    z = kGelu1 * __builtin_fmaf(q, c, c);
     dz = kGelu1 * __builtin_fmaf(3.f, q, 1.f);
   }
-  float t = -kLog2e * z;
-  t = t > 126.f ? 126.f : t;  // NaN stays
-  const float e = __builtin_amdgcn_exp2f(t), s = __builtin_amdgcn_rcpf(1.f + e);
+  const float t = -kLog2e * z;
+  const float e = __builtin_amdgcn_exp2f(t > 126.f ? 126.f : t);
+  float s = __builtin_amdgcn_rcpf(1.f + e);
+  s = t > 126.f ? 0.f : s;
   a = kind == kSigmoid ? s : g * s;
   if constexpr (DERIV) {
     const float d = e * s * s;  // s (1 - s)

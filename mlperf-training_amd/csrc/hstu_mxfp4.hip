@@ -15,9 +15,8 @@
 #include <stdint.h>
 
 #include <algorithm>
-#include <mutex>
+#include <atomic>
 #include <type_traits>
-#include <vector>
 
 #include "hstu_common.h"
 #include "hstu_mi355x.h"
@@ -594,14 +593,15 @@ __global__ void __launch_bounds__(kMxThreads, 2) mx_tile_kernel(MxParams p, int 
     }
 }
 
-hipError_t set_mx_lds(const void* fn) {
-  static std::mutex mu;
-  static std::vector<const void*> done;
-  std::lock_guard<std::mutex> lock(mu);
-  for (const void* d : done)
-    if (d == fn) return hipSuccess;
-  const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, kMxLds);
-  if (e == hipSuccess) done.push_back(fn);
+// the tile form's LDS limit, once a device
+hipError_t set_mx_lds() {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  const uint64_t bit = dev >= 0 && dev < 64 ? (uint64_t)1 << dev : 0;
+  if (e != hipSuccess || (done.load() & bit)) return e;
+  e = hipFuncSetAttribute((const void*)mx_tile_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kMxLds);
+  if (e == hipSuccess) done.fetch_or(bit);
   return e;
 }
 
@@ -693,7 +693,7 @@ extern "C" int hstu_mxfp4_gemm(const void* A, int64_t lda, const void* a_scale, 
     return (int)hipGetLastError();
   }
   if (tiles_m * tiles_n >= (1 << 30)) return HSTU_E_UNSUPPORTED;
-  hipError_t e = set_mx_lds((const void*)mx_tile_kernel);
+  hipError_t e = set_mx_lds();
   if (e != hipSuccess) return (int)e;
   const int per_xcd = (int)((tiles_m * tiles_n + 7) / 8);
   hipLaunchKernelGGL(mx_tile_kernel, dim3(8 * per_xcd), dim3(kMxThreads), kMxLds, stream, p, (int)tiles_m, (int)tiles_n,

@@ -214,12 +214,13 @@ __global__ void __launch_bounds__(BLOCK) rms_fwd_kernel(FwdArgs a) {
     if (!live) continue;
     const float rstd = __builtin_amdgcn_rsqf(ss * a.inv_d + a.eps);
     if (a.rstd && tg == 0) a.rstd[row] = rstd;
-    float s = 1.f, is = 1.f;
+    float s = 1.f, is = 1.f, up = 1.f;
     if constexpr (OUT8) {
       // max|y| as max|h w| rstd: one reduction for both statistics
       top *= rstd;
       s = a.scale_in ? given : top > 0.f ? top / 448.f : top == 0.f ? 1.f / 448.f : top;  // NaN stays
-      is = 1.f / s;
+      up = __builtin_fabsf(s) < 0x1p-100f ? 0x1p64f : 1.f;  // 1 / s would overflow: y 2^64 over s 2^64
+      is = 1.f / (s * up);
       if (!a.scale_in && tg == 0) a.scale_out[row] = s;
     }
 #pragma unroll
@@ -230,7 +231,7 @@ __global__ void __launch_bounds__(BLOCK) rms_fwd_kernel(FwdArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         y[e] = h[i][e] * rstd * w[i][e];
-        if constexpr (OUT8) y[e] = sat_e4m3(div_by(y[e], s, is));
+        if constexpr (OUT8) y[e] = sat_e4m3(div_by(y[e] * up, s * up, is));
       }
       if constexpr (OUT8) store8_e4m3<VEC>(a.y + row * a.ldy, c0, a.D, y);
       else store8<F32, VEC>(a.y + row * a.ldy, c0, a.D, y);

@@ -158,6 +158,35 @@ def test_large_arguments(hip_lib):
 
 
 @gpu
+@pytest.mark.parametrize("M", [26, 200, 1100])
+@pytest.mark.parametrize("name", ACTS)
+def test_every_size_of_the_gate(hip_lib, name, M):
+    """g = v and u = 1 exactly: a(v) and a'(v) from 0 to bf16's largest.  Far on the
+    negative side they are products with an s below 2^-126, at most 88 of it; a'
+    changes sign, so what its argument is off counts by itself."""
+    import hstu_amd
+
+    v = torch.tensor([0, 1e-30, 1e-3, 0.3, 1, 1.28, 5, 30, 60, 86, 1e3, 1e20, 3e38], dtype=torch.bfloat16)
+    v = torch.cat((v, -v)).repeat(-(-M // 26))[:M]
+    F = 1024
+    x = torch.zeros((M, 256), dtype=torch.bfloat16)
+    x[:, 0], x[:, 1] = v, 1
+    wg, wu, dh = torch.zeros((F, 256)), torch.zeros((F, 256)), torch.zeros((M, F))
+    wg[5, 0] = wu[5, 1] = 1
+    dh[:, 5] = 1
+    x, wg, wu, dh = (t.to(torch.bfloat16).to(DEV) for t in (x, wg, wu, dh))
+    h = hstu_amd.gated_linear(x, wg, wu, name)
+    kept, gu = hstu_amd.gated_linear_fwd(x, wg, wu, name, keep=True)
+    assert torch.equal(kept, h)
+    a, da = orc.activation_ref(name, v.to(DEV).double())
+    within(h[:, 5], a, a.abs() * (HALF + ARG) + 2.0 ** -110, "h")
+    for keep in (None, gu):
+        dx = hstu_amd.gated_linear_bwd(dh, x, wg, wu, name, gu=keep)[0]
+        within(dx[:, 1], a, a.abs() * (HALF + ARG) + 2.0 ** -110, "du")
+        within(dx[:, 0], da, da.abs() * HALF + 2 * ARG, "dg")
+
+
+@gpu
 def test_gradient_against_differences(hip_lib):
     """The kernels' gradient along a direction against a difference quotient of the float64 formula."""
     import hstu_amd

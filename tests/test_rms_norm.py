@@ -108,6 +108,26 @@ def test_e4m3_output(hip_lib, rows, D, dtype, residual):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_e4m3_of_the_smallest_rows(hip_lib, dtype):
+    """Scales below 2^-126, whose reciprocal no fp32 value holds.  They and y are
+    multiples of 2^-149: half of one more for each, 448 of them for the scale's."""
+    import hstu_amd
+
+    x = make(6, 520, dtype, 5, 3e-39).to(DEV)
+    x[:, ::7] = 0
+    w = make_weight(520, torch.float32).to(DEV)
+    for eps in (1e-6, 1e-2):
+        y8, s = hstu_amd.rms_norm_fp8(x, w, eps)
+        yr, _ = orc.rms_norm_ref(x, w, eps)
+        sr = yr.abs().amax(-1) / 448.0
+        assert float(sr.max()) < 2.0 ** -120
+        within(s, sr, sr * 2 * FP32 + 2.0 ** -149, "scale")
+        sd = s.double()[:, None]
+        within(y8.float().double() * sd, yr, yr.abs() * (2.0 ** -4 + 4 * FP32) + sd * 2.0 ** -10 + 450 * 2.0 ** -150, "y8")
+
+
+@gpu
 def test_non_finite_rows_stay_in_their_row(hip_lib):
     import hstu_amd
 
