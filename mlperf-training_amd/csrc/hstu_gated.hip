@@ -299,12 +299,17 @@ __global__ void __launch_bounds__(kThreads, 2) gated_few_kernel(GatedParams p) {
 }
 
 // ---------------------------------------------------------------- tile form, bf16
-// 128 rows x 128 columns of h a workgroup, so 128 x 256 of products: the
-// projection GEMM's two-workgroup form (ring of five 16 KiB slots, exact waits on
+// Bound by the matrix cores.  128 rows x 128 columns of h a workgroup, so 128 x 256 of
+// products: the projection GEMM's two-workgroup form (ring of five 16 KiB slots, exact waits on
 // inline LDS DMAs) with W0 the tile's gate rows and W1 its up rows.  Wave w owns all
 // 128 rows and columns 32 w .. 32 w + 31 of both products, so a lane's
 // accumulators of one output pair up in registers and the epilogue is local.
 // W rows are permuted in LDS so that a lane holds runs of eight columns.
+// Measured (M x D -> F): 8 192 x 4 096 -> 10 240 1 080-1 180 us (1.16-1.27 PFLOP/s; a large
+// library product 1.42), with g and u kept 1 220-1 310; 37 429 x 512 -> 2 048 159-172 (0.91-
+// 0.99, eight k-steps a tile), the backward's computation 223-250.  The clock is at
+// 1.6-1.75 GHz under it, the card's power limit: tiles of 256 rows with a quarter
+// less LDS traffic were 2-5 % faster at D = 4 096 and up to 27 % slower at D <= 1 024.
 template <bool BWD>
 __global__ void __launch_bounds__(kDuoThreads, 2) gated_tile_kernel(GatedParams p, int per_xcd) {
   __shared__ __attribute__((aligned(1024))) uint8_t ring[kDuoSlots][kDuoItem];
@@ -410,7 +415,8 @@ __global__ void __launch_bounds__(kDuoThreads, 2) gated_tile_kernel(GatedParams 
 // ---------------------------------------------------------------- tile form, e4m3
 // The same tile, ring and items on rows of e4m3 (a k-step is 128 elements) with
 // v_mfma_f32_16x16x128_f8f6f4: 16-row blocks 0, 1 of a wave's weights are gate
-// rows, 2, 3 up rows.
+// rows, 2, 3 up rows.  Measured: 37 429 x 1 024 -> 4 096 310-336 us, 1.9-2.0 PFLOP/s, in eight
+// k-steps a tile (a large library product 2.63).
 __global__ void __launch_bounds__(kDuoThreads, 2) gated_tile_fp8_kernel(GatedParams p, int per_xcd) {
   __shared__ __attribute__((aligned(1024))) uint8_t ring[kDuoSlots][kDuoItem];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -522,7 +528,7 @@ __global__ void __launch_bounds__(kDuoThreads, 2) gated_tile_fp8_kernel(GatedPar
 
 // ---------------------------------------------------------------- backward from kept g and u
 // Memory alone bounds it: 10 bytes in and 4 out a value.  A thread takes eight
-// consecutive columns.
+// consecutive columns.  8 192 x 10 240 (1.17 GB) 247-253 us, 4.7 TB/s.
 struct KeptArgs {
   const uint16_t* dh;
   const float* keep;
@@ -561,7 +567,8 @@ __global__ void __launch_bounds__(256) gated_kept_kernel(KeptArgs a) {
 // The weights side by side with the contraction index of dx = [dg | du] [Wg; Wu]
 // contiguous: out[d][f] = Wg[f][d], out[d][F + f] = Wu[f][d].  64 x 64 tiles through
 // LDS (pitch 66 elements: both the row and the column accesses spread over the
-// banks), 16-byte loads and stores; bound by memory.
+// banks), 16-byte loads and stores; bound by memory: two of 10 240 x 4 096 (336 MB)
+// 57-60 us, 5.7 TB/s.
 __global__ void __launch_bounds__(256) gated_transpose_kernel(const uint16_t* wg, const uint16_t* wu, int64_t ldg,
                                                               int64_t ldu, int F, uint16_t* out, int64_t ldo) {
   __shared__ uint16_t tile[64 * 66];

@@ -154,7 +154,9 @@ struct FwdArgs {
 
 // A block of BLOCK threads is BLOCK / G row groups; every group walks the same
 // number of rows, so that the barriers of a group of several waves are the
-// block's.
+// block's.  Measured: 162 251 x 512 bf16 with residual to e4m3 (581 MB) 108 us, 5.4 TB/s;
+// 37 429 x 512 bf16 with residual (153 MB) 26-30 us; 4 099 x 5 120 fp32 (168 MB) 33-39 us;
+// a large copy runs at 5.1 TB/s.  One row of 2 048 2.6 us, a launch's own time.
 template <bool F32, bool VEC, int G, int NV, int BLOCK, bool OUT8>
 __global__ void __launch_bounds__(BLOCK) rms_fwd_kernel(FwdArgs a) {
   constexpr int GROUPS = BLOCK / G, WPG = G / 64;
@@ -253,6 +255,11 @@ struct BwdArgs {
   float inv_d;
 };
 
+// The same groups, over at most as many blocks as the chip holds at a time: each
+// keeps its columns' share of dw in registers over all of its rows and writes it
+// once, so that dw costs blocks x D x 8 bytes and no second pass over the rows.
+// Measured: 37 429 x 512 bf16 with dh (153 MB) 27-29 us, 5.3-5.7 TB/s; 4 099 x 5 120 fp32
+// (252 MB) 44-45 us, 5.6 TB/s; rms_dw_kernel 4 us more.
 template <bool F32, bool VEC, int G, int NV, int BLOCK>
 __global__ void __launch_bounds__(BLOCK) rms_bwd_kernel(BwdArgs a) {
   constexpr int GROUPS = BLOCK / G, WPG = G / 64;

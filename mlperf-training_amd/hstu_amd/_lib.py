@@ -265,14 +265,16 @@ def check(status: int, what: str) -> None:
         raise HstuKernelError(f"{what} failed: {msg}")
 
 
-def stream(t) -> int:
-    """The current stream of the tensor's device."""
+_raw = None
+
+
+def _bind_raw():
+    global _raw
     import torch
 
-    return torch.cuda.current_stream(t.device).cuda_stream
-
-
-_raw = None
+    _raw = (torch.cuda.current_device, torch._C._cuda_getCurrentRawStream, torch.cuda.device,
+            torch.cuda.is_current_stream_capturing)
+    return _raw
 
 
 def launch(name: str, t, *args) -> None:
@@ -280,18 +282,14 @@ def launch(name: str, t, *args) -> None:
     tensor's device as the last argument, with that device current (a launch on
     its stream needs it); raise on a status.  One call costs the host as little
     as it can: a decoding step is made of such calls."""
-    global _raw
-    if _raw is None:
-        import torch
-
-        _raw = (torch.cuda.current_device, torch._C._cuda_getCurrentRawStream, torch.cuda.device)
+    raw = _raw or _bind_raw()
     f = _bound.get(name) or fn(name)
     index = t.device.index
-    if index == _raw[0]():
-        status = f(*args, _raw[1](index))
+    if index == raw[0]():
+        status = f(*args, raw[1](index))
     else:
-        with _raw[2](index):
-            status = f(*args, _raw[1](index))
+        with raw[2](index):
+            status = f(*args, raw[1](index))
     if status != 0:
         check(status, name)
 
@@ -303,27 +301,18 @@ def guard_graph(ctx, t) -> None:
     captured backward that crosses to the default stream ends the process; so
     eager uses mark the leaf's accumulation node, which lives as long as such a
     graph does, and a capture looks for the mark."""
-    if stream(t) == 0:
+    raw = _raw or _bind_raw()
+    if raw[1](t.device.index) == 0:
         for node, _ in ctx.next_functions:
             if node is not None and not node.next_functions:
                 node.metadata["hstu_default_stream"] = True
         return
-    import torch
-
-    if torch.cuda.is_current_stream_capturing():
+    if raw[3]():
         for node, _ in ctx.next_functions:
             if node is not None and not node.next_functions and "hstu_default_stream" in node.metadata:
                 raise HstuKernelError("graph capture of a function of a leaf that a graph outside the capture, built on "
                                       "the default stream, still holds: let go of that graph's outputs first, or warm "
                                       "up on a side stream")
-
-
-def refuse_second_derivatives() -> None:
-    """Called in an autograd function's backward, which runs with gradients enabled only under create_graph."""
-    import torch
-
-    if torch.is_grad_enabled():
-        raise NotImplementedError("second derivatives (create_graph=True)")
 
 
 def ptr(t) -> Optional[int]:

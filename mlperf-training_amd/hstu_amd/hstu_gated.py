@@ -162,7 +162,8 @@ class GatedLinearFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dh):
-        _lib.refuse_second_derivatives()
+        if torch.is_grad_enabled():  # only under create_graph
+            raise NotImplementedError("second derivatives (create_graph=True)")
         x, w_gate, w_up, gu = ctx.saved_tensors
         need_x, need_g, need_u = ctx.needs_input_grad[:3]
         dx, dg, du = gated_linear_bwd(dh, x, w_gate, w_up, ctx.activation, need_x, need_g or need_u, gu)
