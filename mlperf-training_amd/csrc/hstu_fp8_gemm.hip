@@ -959,16 +959,16 @@ __global__ void __launch_bounds__(kDuoThreads, 2) fp8_gemm_duo_kernel(GemmParams
 // ring, item protocol and two workgroups per CU as above, on rows of bf16 (a
 // k-step of 128 bytes is 64 elements).
 //
-// What bounds it: the matrix cores at long K (busy 61 % of the time at K = 2048;
-// per k-step and wave 1 M MAC against 24 KiB of LDS reads, 0.3 of the LDS rate),
-// at K = 512 (40 %) the output and its epilogue beside them.  So the MFMA is
-// v_mfma_f32_32x32x16_bf16, whose measured rate is 1.62 PFLOP/s against 1.23 for
-// 16x16x32 (whole chip, register operands).  Wave w owns all 128 rows and columns [64 w, 64 w + 64)
-// as 4 x 2 accumulators of 32 x 32 (128 registers); a lane reads chunk
-// 2 kk + lane / 32 of row lane % 32 for the step's MFMA kk, which is conflict
-// free under the same swizzle (16 lanes read 16 consecutive rows).  The W rows
-// are permuted in LDS so that a lane's 16 accumulators of one 32 x 32 block
-// are two runs of eight output columns: 16-byte stores.
+// What bounds it: the card's power at long K (the clock falls to 1.6-1.75 GHz under
+// it), at K = 512 the output and its epilogue too.  So the MFMA is
+// v_mfma_f32_16x16x32_bf16: with random register operands it runs at 1.91 PFLOP/s
+// and 32x32x16 at 1.73, with zeros both at 2.45, and their sums are the same bytes (M x N x K, us,
+// 32x32x16 / 16x16x32: 162 251 x 2 048 x 512 443 / 415, 162 251 x 512 x 1 536 316 / 301, 8 192^3
+// 864 / 805, 8 192 x 4 096 x 20 480 1 148 / 1 086).  Wave w owns all 128 rows and columns
+// [64 w, 64 w + 64) as 8 x 4 accumulators of 16 x 16 (128 registers); a lane reads
+// chunk 4 kk + lane / 16 of row lane % 16 for the step's MFMA kk, which is conflict
+// free under the same swizzle.  The W rows are permuted in LDS so that a lane's
+// accumulators of two blocks are eight consecutive output columns: 16-byte stores.
 // Measured against the 128 x 128 tile kernel (event-timed, back to back):
 // 162 251 x 512 x 2048 (M, K, N) 542 -> 420 us, K = 1536, N = 512 with a
 // residual 389 -> 300, K = 2048, N = 512 421 -> 326 us (1.04 PFLOP/s); 37 429
@@ -978,8 +978,8 @@ __global__ void __launch_bounds__(kDuoThreads, 2) fp8_gemm_duo_kernel(GemmParams
 // Tile order: up to 8 column tiles (N <= 2 048) one row panel's tiles run together;
 // with more, an XCD's 64 running tiles would share one or two panels of A and read
 // all of W, so they go in groups of 8 row panels (us, panel by panel / in groups:
-// 8 192 x 8 192 x 8 192 1 168 / 856, 8 192 x 4 096 (N) x 20 480 1 153 / 1 128; at N = 512 and
-// 2 048 the same or 3 % slower).
+// 8 192 x 8 192 x 8 192 1 168 / 856, 8 192 x 4 096 (N) x 20 480 1 153 / 1 128, both on
+// 32x32x16; at N = 512 and 2 048 the same or 3 % slower).
 constexpr int kPanelTiles = 8;
 
 template <bool RESID>
@@ -1004,8 +1004,8 @@ __global__ void __launch_bounds__(kDuoThreads, 2) bf16_gemm_duo_kernel(GemmParam
     const int q = 64 * (4 * wave + j) + lane, r = q >> 3;
     const uint32_t pos = (uint32_t)(((q & 7) ^ wide_swz(r)) * 16);
     av[j] = (uint32_t)r * (uint32_t)p.lda + pos;
-    const int i = r & 31;  // MFMA row of this LDS row: accumulator 4 (i / 8) + i % 4 of half (i / 4) % 2
-    const int col = (r & ~31) + duo32_col((i >> 2) & 1, 4 * (i >> 3) + (i & 3));
+    const int i = r & 31;  // MFMA row i % 16 of block i / 16: accumulator i % 4 of lane quarter (i % 16) / 4
+    const int col = (r & ~31) + 8 * ((i & 15) >> 2) + 4 * (i >> 4) + (i & 3);
     wv[0][j] = (uint32_t)col * (uint32_t)p.ldw + pos;
     wv[1][j] = (uint32_t)(128 + col) * (uint32_t)p.ldw + pos;
   }
@@ -1021,40 +1021,36 @@ __global__ void __launch_bounds__(kDuoThreads, 2) bf16_gemm_duo_kernel(GemmParam
   };
   for (int it = 0; it < min(5, nitems); ++it) issue(it);
 
-  const int lr = lane & 31, h = lane >> 5;
-  // chunk 2 kk + h of row lr of an even 32-row block; in odd blocks the
-  // swizzle flips bit 2, i.e. kk and kk ^ 2 trade places
-  uint32_t rd[4];
+  const int li = lane & 15, q = lane >> 4;
+  // chunk 4 kk + q of row li of an even 32-row block; in odd blocks the swizzle
+  // flips bit 2, i.e. the two kk trade places
+  uint32_t rd[2];
 #pragma unroll
-  for (int kk = 0; kk < 4; ++kk) rd[kk] = lr * 128 + (((2 * kk + h) ^ wide_swz(lr)) * 16);
+  for (int kk = 0; kk < 2; ++kk) rd[kk] = li * 128 + (((4 * kk + q) ^ wide_swz(li)) * 16);
   const uint32_t w_off = 64 * (wave & 1) * 128;
 
-  // the lane's bias runs: columns 64 wave + 32 nb + 16 run + 8 h + (0..7)
-  const int cl = n0 + 64 * wave + 8 * h;
-  u32x4 bv[2][2];
+  // the lane's bias runs: columns 64 wave + 32 run + 8 q + (0..7)
+  const int cl = n0 + 64 * wave + 8 * q;
+  u32x4 bv[2];
   auto load_consts = [&]() {
     const BufRsrc bsr = make_rsrc(p.bias, p.bias ? (uint32_t)p.N * 2u : 0u);  // no bias: zeros
 #pragma unroll
-    for (int nb = 0; nb < 2; ++nb)
-#pragma unroll
-      for (int run = 0; run < 2; ++run) bv[nb][run] = buf_ld128(bsr, (uint32_t)(cl + 32 * nb + 16 * run) * 2u, 0);
+    for (int run = 0; run < 2; ++run) bv[run] = buf_ld128(bsr, (uint32_t)(cl + 32 * run) * 2u, 0);
   };
 
-  f32x16 acc[4][2];
+  f32x4 acc[8][4];
 #pragma unroll
-  for (int mb = 0; mb < 4; ++mb)
+  for (int m = 0; m < 8; ++m)
 #pragma unroll
-    for (int nb = 0; nb < 2; ++nb)
+    for (int nb = 0; nb < 4; ++nb) acc[m][nb] = zero4();
+  auto read_block = [&](const uint8_t* st, int blk, u32x4 (&x)[2]) {  // 16 rows
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[mb][nb][r] = 0.f;
-  auto read_block = [&](const uint8_t* st, int blk, u32x4 (&x)[4]) {
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk) x[kk] = lds_ld128(st + 4096 * blk + rd[blk & 1 ? kk ^ 2 : kk]);
+    for (int kk = 0; kk < 2; ++kk) x[kk] = lds_ld128(st + 2048 * blk + rd[blk & 2 ? kk ^ 1 : kk]);
   };
   // one k-step; ITEMS: how many items are left to issue (3; 1 at step nk - 2;
   // 0 at the last, which loads the epilogue constants instead).  All operands
   // go to registers first, which frees the step's slots before its MFMAs; the
-  // DMAs are spread one per two MFMAs, because a wave that issues its twelve
+  // DMAs are spread one per four MFMAs, because a wave that issues its twelve
   // in a row waits at the texture address unit for the other waves' (48 KiB
   // of loads) before its next MFMA.
   auto kstep = [&](int s, auto items_c) {
@@ -1063,11 +1059,11 @@ __global__ void __launch_bounds__(kDuoThreads, 2) bf16_gemm_duo_kernel(GemmParam
     else dma_barrier<8>();
     const uint8_t* sa_ = ring[(3 * s) % kDuoSlots];
     const uint8_t* sw_ = ring[(3 * s + 1 + (wave >> 1)) % kDuoSlots] + w_off;
-    u32x4 w[2][4], a[4][4];
-    read_block(sw_, 0, w[0]);
-    read_block(sw_, 1, w[1]);
+    u32x4 w[4][2], a[8][2];
 #pragma unroll
-    for (int mb = 0; mb < 4; ++mb) read_block(sa_, mb, a[mb]);
+    for (int nb = 0; nb < 4; ++nb) read_block(sw_, nb, w[nb]);
+#pragma unroll
+    for (int m = 0; m < 8; ++m) read_block(sa_, m, a[m]);
     pc_barrier_lds();  // every wave has read step s: its three slots are free
     if constexpr (ITEMS == 0) load_consts();
     const uint32_t ka = (uint32_t)(128 * (s + 2)), kw1 = (uint32_t)(128 * (s + 1));
@@ -1075,11 +1071,11 @@ __global__ void __launch_bounds__(kDuoThreads, 2) bf16_gemm_duo_kernel(GemmParam
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k)
       dst[k] = __builtin_amdgcn_readfirstlane(ring0 + (uint32_t)(((3 * s + 5 + k) % kDuoSlots) * kDuoItem + 4096 * wave));
-    static_for<32>([&](auto nc) {
-      constexpr int n = decltype(nc)::value, mb = n >> 3, kk = (n >> 1) & 3, nb = n & 1;
-      acc[mb][nb] = mfma32_bf16(w[nb][kk], a[mb][kk], acc[mb][nb]);
-      if constexpr ((n & 1) == 1 && (n >> 1) < 4 * ITEMS) {  // items 3 s + 5 (W1), 3 s + 6 (A), 3 s + 7 (W0)
-        constexpr int k = n >> 3, j = (n >> 1) & 3;
+    static_for<64>([&](auto nc) {
+      constexpr int n = decltype(nc)::value, kk = n >> 5, m = (n >> 2) & 7, nb = n & 3;
+      acc[m][nb] = mfma_bf16(w[nb][kk], a[m][kk], acc[m][nb]);
+      if constexpr (nb == 3 && (n >> 2) < 4 * ITEMS) {  // items 3 s + 5 (W1), 3 s + 6 (A), 3 s + 7 (W0)
+        constexpr int k = n >> 4, j = (n >> 2) & 3;
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (k == 0) dma_to_lds(dst[0] + 1024 * j, wv[1][j], wrs, kw1);
         else if constexpr (k == 1) dma_to_lds(dst[1] + 1024 * j, av[j], ars, ka);
@@ -1092,7 +1088,7 @@ __global__ void __launch_bounds__(kDuoThreads, 2) bf16_gemm_duo_kernel(GemmParam
   kstep(nk - 2, std::integral_constant<int, 1>{});
   kstep(nk - 1, std::integral_constant<int, 0>{});
 
-  // epilogue: lane holds C[m0 + 32 mb + lr][cl + 32 nb + 16 run + (0..7)];
+  // epilogue: lane holds C[m0 + 16 m + li][cl + 32 run + (0..7)];
   // rows past M are dropped (stores) or read as zero (residual) by the range
   // check of the buffer resources
   const BufRsrc crs = make_rsrc((uint8_t*)p.C + (int64_t)m0 * p.ldc * 2, (uint32_t)(mrows * p.ldc * 2));
@@ -1101,36 +1097,34 @@ __global__ void __launch_bounds__(kDuoThreads, 2) bf16_gemm_duo_kernel(GemmParam
   const int wc0 = n0 + 64 * wave;
   const bool silu = wc0 >= p.silu_begin && wc0 < p.silu_end;
 #pragma unroll
-  for (int mb = 0; mb < 4; ++mb) {
-    const int r = 32 * mb + lr;
+  for (int m = 0; m < 8; ++m) {
+    const int r = 16 * m + li;
 #pragma unroll
-    for (int nb = 0; nb < 2; ++nb)
+    for (int run = 0; run < 2; ++run) {
+      const int c = cl + 32 * run;
+      float o[8];
 #pragma unroll
-      for (int run = 0; run < 2; ++run) {
-        const int c = cl + 32 * nb + 16 * run;
-        float o[8];
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t b = bv[run][j];
+        o[2 * j] = acc[m][2 * run + (j >> 1)][2 * (j & 1)] + bf16_to_f32((uint16_t)(b & 0xffff));
+        o[2 * j + 1] = acc[m][2 * run + (j >> 1)][2 * (j & 1) + 1] + bf16_to_f32((uint16_t)(b >> 16));
+      }
+      if (silu) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = o[e] * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * o[e]));
+      }
+      if constexpr (RESID) {
+        const u32x4 rv = buf_ld128(rrs, (uint32_t)(r * p.ldr + c) * 2, 0);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t b = bv[nb][run][j];
-          o[2 * j] = acc[mb][nb][8 * run + 2 * j] + bf16_to_f32((uint16_t)(b & 0xffff));
-          o[2 * j + 1] = acc[mb][nb][8 * run + 2 * j + 1] + bf16_to_f32((uint16_t)(b >> 16));
+          o[2 * j] += bf16_to_f32(rv[j] & 0xffff);
+          o[2 * j + 1] += bf16_to_f32(rv[j] >> 16);
         }
-        if (silu) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] = o[e] * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * o[e]));
-        }
-        if constexpr (RESID) {
-          const u32x4 rv = buf_ld128(rrs, (uint32_t)(r * p.ldr + c) * 2, 0);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            o[2 * j] += bf16_to_f32(rv[j] & 0xffff);
-            o[2 * j + 1] += bf16_to_f32(rv[j] >> 16);
-          }
-        }
-        __builtin_amdgcn_raw_buffer_store_b128(
-            u32x4{pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7])}, crs,
-            (uint32_t)(r * p.ldc + c) * 2, 0, 0);
       }
+      __builtin_amdgcn_raw_buffer_store_b128(
+          u32x4{pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7])}, crs,
+          (uint32_t)(r * p.ldc + c) * 2, 0, 0);
+    }
   }
 }
 
@@ -1142,8 +1136,8 @@ __global__ void __launch_bounds__(kDuoThreads, 2) bf16_gemm_duo_kernel(GemmParam
 // and a step costs its LDS reads and MFMAs, not a memory round trip.  One
 // barrier per step: it publishes step s and frees step s - 1's stage, which
 // the loads of step s + 3 then take.  Every element is the same chain of the
-// same MFMAs over k as in the other forms (fp8: 16x16x128; bf16: 32x32x16 as
-// in bf16_gemm_duo_kernel), so the bytes are the same.
+// same MFMAs over k as in the other forms (fp8: 16x16x128; bf16: 32x32x16, of
+// which two round as one 16x16x32 of bf16_gemm_duo_kernel), so the bytes are the same.
 // W rows are permuted in LDS so that a lane's accumulators of one row are
 // runs of eight output columns.
 // Measured (us, wide form before): 1 027 rows, e4m3 K = 1536, N = 512 with a

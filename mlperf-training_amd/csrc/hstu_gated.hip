@@ -305,11 +305,13 @@ __global__ void __launch_bounds__(kThreads, 2) gated_few_kernel(GatedParams p) {
 // 128 rows and columns 32 w .. 32 w + 31 of both products, so a lane's
 // accumulators of one output pair up in registers and the epilogue is local.
 // W rows are permuted in LDS so that a lane holds runs of eight columns.
-// Measured (M x D -> F): 8 192 x 4 096 -> 10 240 1 080-1 180 us (1.16-1.27 PFLOP/s; a large
-// library product 1.42), with g and u kept 1 220-1 310; 37 429 x 512 -> 2 048 159-172 (0.91-
-// 0.99, eight k-steps a tile), the backward's computation 223-250.  The clock is at
-// 1.6-1.75 GHz under it, the card's power limit: tiles of 256 rows with a quarter
-// less LDS traffic were 2-5 % faster at D = 4 096 and up to 27 % slower at D <= 1 024.
+// The MFMA is v_mfma_f32_16x16x32_bf16, which takes less power than 32x32x16 for the same
+// bytes (M x D -> F, us, 32x32x16 / 16x16x32: 8 192 x 4 096 -> 10 240 1 091 / 1 037, 37 429 x
+// 1 024 -> 4 096 558 / 540, 37 429 x 512 -> 2 048 161 / 165): 1.32, 1.16 and 0.95 PFLOP/s, where a
+// large library product reaches 1.42.  With g and u kept 8 192 x 4 096 -> 10 240 takes 1 125-1 240,
+// the backward's computation of 37 429 x 512 -> 2 048 223-253.
+// Tiles of 256 rows in one workgroup, with a third less to load, were 4 % faster at D =
+// 4 096 and 7 % slower at D = 1 024.
 template <bool BWD>
 __global__ void __launch_bounds__(kDuoThreads, 2) gated_tile_kernel(GatedParams p, int per_xcd) {
   __shared__ __attribute__((aligned(1024))) uint8_t ring[kDuoSlots][kDuoItem];
@@ -326,7 +328,7 @@ __global__ void __launch_bounds__(kDuoThreads, 2) gated_tile_kernel(GatedParams 
     av[j] = (uint32_t)r * (uint32_t)p.ldx + (uint32_t)(((q & 7) ^ wide_swz(r)) * 16);
     // W blocks of 32 rows all in one swizzle (a wave reads one block of each product)
     const uint32_t pos = (uint32_t)(((q & 7) ^ wide_swz(i)) * 16);
-    const int col = (r & ~31) + duo32_col((i >> 2) & 1, 4 * (i >> 3) + (i & 3));
+    const int col = (r & ~31) + 8 * ((i & 15) >> 2) + 4 * (i >> 4) + (i & 3);  // a lane: 8 consecutive columns
     wv[0][j] = (uint32_t)col * (uint32_t)p.ldwg + pos;
     wv[1][j] = (uint32_t)col * (uint32_t)p.ldwu + pos;
   }
@@ -344,46 +346,45 @@ __global__ void __launch_bounds__(kDuoThreads, 2) gated_tile_kernel(GatedParams 
   };
   for (int it = 0; it < 5; ++it) issue(it);  // D % 256: at least four k-steps
 
-  const int lr = lane & 31, h = lane >> 5;
-  uint32_t rd[4];  // chunk 2 kk + h of row lr; in odd 32-row blocks of x, kk and kk ^ 2 trade places
+  const int li = lane & 15, q = lane >> 4;
+  // chunks q and q + 4 of row li; in odd 32-row blocks of x the two trade places
+  uint32_t rd[2];
 #pragma unroll
-  for (int kk = 0; kk < 4; ++kk) rd[kk] = lr * 128 + (((2 * kk + h) ^ wide_swz(lr)) * 16);
+  for (int kk = 0; kk < 2; ++kk) rd[kk] = li * 128 + (((4 * kk + q) ^ wide_swz(li)) * 16);
   const uint32_t w_off = 4096 * wave;
 
-  f32x16 acc[4][2];
+  f32x4 acc[8][4];
 #pragma unroll
-  for (int mb = 0; mb < 4; ++mb)
+  for (int m = 0; m < 8; ++m)
 #pragma unroll
-    for (int nb = 0; nb < 2; ++nb)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[mb][nb][r] = 0.f;
+    for (int nb = 0; nb < 4; ++nb) acc[m][nb] = zero4();
   auto kstep = [&](int s, auto items_c) {
     constexpr int ITEMS = decltype(items_c)::value;
     if constexpr (ITEMS == 0) dma_barrier<0>();
     else dma_barrier<8>();
     const uint8_t* sa = ring[(3 * s) % kDuoSlots];
-    u32x4 w[2][4], a[4][4];
+    u32x4 w[4][2], a[8][2];
 #pragma unroll
-    for (int nb = 0; nb < 2; ++nb) {
-      const uint8_t* sw = ring[(3 * s + 1 + nb) % kDuoSlots] + w_off;
+    for (int nb = 0; nb < 4; ++nb) {
+      const uint8_t* sw = ring[(3 * s + 1 + (nb >> 1)) % kDuoSlots] + w_off + 2048 * (nb & 1);
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) w[nb][kk] = lds_ld128(sw + rd[kk]);
+      for (int kk = 0; kk < 2; ++kk) w[nb][kk] = lds_ld128(sw + rd[kk]);
     }
 #pragma unroll
-    for (int mb = 0; mb < 4; ++mb)
+    for (int m = 0; m < 8; ++m)
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) a[mb][kk] = lds_ld128(sa + 4096 * mb + rd[mb & 1 ? kk ^ 2 : kk]);
+      for (int kk = 0; kk < 2; ++kk) a[m][kk] = lds_ld128(sa + 2048 * m + rd[m & 2 ? kk ^ 1 : kk]);
     pc_barrier_lds();  // every wave has read step s: its three slots are free
     const uint32_t ka = (uint32_t)(128 * (s + 2)), kw1 = (uint32_t)(128 * (s + 1));
     uint32_t dst[3];
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k)
       dst[k] = __builtin_amdgcn_readfirstlane(ring0 + (uint32_t)(((3 * s + 5 + k) % kDuoSlots) * kDuoItem + 4096 * wave));
-    static_for<32>([&](auto nc) {
-      constexpr int n = decltype(nc)::value, mb = n >> 3, kk = (n >> 1) & 3, nb = n & 1;
-      acc[mb][nb] = mfma32_bf16(w[nb][kk], a[mb][kk], acc[mb][nb]);
-      if constexpr ((n & 1) == 1 && (n >> 1) < 4 * ITEMS) {  // items 3 s + 5 (up), 3 s + 6 (x), 3 s + 7 (gate)
-        constexpr int k = n >> 3, j = (n >> 1) & 3;
+    static_for<64>([&](auto nc) {
+      constexpr int n = decltype(nc)::value, kk = n >> 5, m = (n >> 2) & 7, nb = n & 3;
+      acc[m][nb] = mfma_bf16(w[nb][kk], a[m][kk], acc[m][nb]);
+      if constexpr (n % 4 == 3 && n / 4 < 4 * ITEMS) {  // items 3 s + 5 (up), 3 s + 6 (x), 3 s + 7 (gate)
+        constexpr int i = n / 4, k = i >> 2, j = i & 3;
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (k == 0) dma_to_lds(dst[0] + 1024 * j, wv[1][j], urs, kw1);
         else if constexpr (k == 1) dma_to_lds(dst[1] + 1024 * j, av[j], ars, ka);
@@ -396,19 +397,16 @@ __global__ void __launch_bounds__(kDuoThreads, 2) gated_tile_kernel(GatedParams 
   kstep(nk - 2, std::integral_constant<int, 1>{});
   kstep(nk - 1, std::integral_constant<int, 0>{});
 
-  // lane: rows m0 + 32 mb + lr, columns n0 + 32 wave + 16 run + 8 h + (0..7) of both products
-  const int cl = n0 + 32 * wave + 8 * h;
+  // lane: rows m0 + 16 mb + li, columns n0 + 32 wave + 8 q + (0..7) of both products
+  const int cl = n0 + 32 * wave + 8 * q;
 #pragma unroll
-  for (int mb = 0; mb < 4; ++mb) {
-    const int r = 32 * mb + lr;
+  for (int mb = 0; mb < 8; ++mb) {
+    const int r = 16 * mb + li;
     if (r >= mrows) continue;
+    float g[8], u[8];
 #pragma unroll
-    for (int run = 0; run < 2; ++run) {
-      float g[8], u[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) g[e] = acc[mb][0][8 * run + e], u[e] = acc[mb][1][8 * run + e];
-      gated_store<BWD, 8>(p, m0 + r, cl + 16 * run, g, u);
-    }
+    for (int e = 0; e < 8; ++e) g[e] = acc[mb][e >> 2][e & 3], u[e] = acc[mb][2 + (e >> 2)][e & 3];
+    gated_store<BWD, 8>(p, m0 + r, cl, g, u);
   }
 }
 

@@ -265,6 +265,13 @@ def check(status: int, what: str) -> None:
         raise HstuKernelError(f"{what} failed: {msg}")
 
 
+def stream(t) -> int:
+    """The current stream of the tensor's device."""
+    import torch
+
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
 _raw = None
 
 
