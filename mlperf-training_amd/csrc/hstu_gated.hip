@@ -33,10 +33,10 @@ constexpr float kGelu3 = 0.044715f;
 // digits that a subtraction from 1 would lose.  Where e^-z passes 2^126, s is 0
 // (its value is under 2^-126, and g may be anything); gelu's cubic is taken at 64
 // at the most, where s is 0 or 1 in fp32 and the cube still a number.
-template <bool DERIV>
-__device__ __forceinline__ void act(int kind, float g, float& a, float& da) {
+template <int KIND, bool DERIV>
+__device__ __forceinline__ void act(float g, float& a, float& da) {
   float z = g, dz = 1.f;
-  if (kind == kGelu) {
+  if constexpr (KIND == kGelu) {
     const float c = __builtin_fabsf(g) > 64.f ? __builtin_copysignf(64.f, g) : g;  // NaN stays
     const float q = kGelu3 * c * c;
     z = kGelu1 * __builtin_fmaf(q, c, c);
@@ -46,11 +46,19 @@ __device__ __forceinline__ void act(int kind, float g, float& a, float& da) {
   const float e = __builtin_amdgcn_exp2f(t > 126.f ? 126.f : t);
   float s = __builtin_amdgcn_rcpf(1.f + e);
   s = t > 126.f ? 0.f : s;
-  a = kind == kSigmoid ? s : g * s;
+  a = KIND == kSigmoid ? s : g * s;
   if constexpr (DERIV) {
     const float d = e * s * s;  // s (1 - s)
-    da = kind == kSigmoid ? d : __builtin_fmaf(g * d, dz, s);
+    da = KIND == kSigmoid ? d : KIND == kSilu ? __builtin_fmaf(g, d, s) : __builtin_fmaf(g * d, dz, s);
   }
+}
+// f with the activation as a constant: a branch in every value would keep their
+// chains of exponential and reciprocal from overlapping
+template <typename F>
+__device__ __forceinline__ void by_act(int kind, F&& f) {
+  if (kind == kSilu) f(std::integral_constant<int, kSilu>{});
+  else if (kind == kGelu) f(std::integral_constant<int, kGelu>{});
+  else f(std::integral_constant<int, kSigmoid>{});
 }
 
 struct GatedParams {
@@ -74,18 +82,25 @@ struct GatedParams {
 
 __device__ __forceinline__ float bf16f(uint32_t b16) { return __builtin_bit_cast(float, b16 << 16); }
 
-// N (4 or 8) consecutive outputs from column n of row m on, from their products.
-template <bool BWD, int N>
+template <int N>
+using Bf16s = typename std::conditional<N == 8, u32x4, u32x2>::type;
+// N (4 or 8) consecutive values of dh from column n of row m on
+template <int N>
+__device__ __forceinline__ Bf16s<N> load_dh(const GatedParams& p, int m, int n) {
+  return *(const Bf16s<N>*)(p.dh + (int64_t)m * p.lddh + n);
+}
+// N consecutive outputs from column n of row m on, from their products (and d, their dh).
+template <int KIND, bool BWD, int N>
 __device__ __forceinline__ void gated_store(const GatedParams& p, int m, int n, const float (&g)[N],
-                                            const float (&u)[N]) {
-  using Vec = typename std::conditional<N == 8, u32x4, u32x2>::type;
+                                            const float (&u)[N], Bf16s<N> d) {
+  using Vec = Bf16s<N>;
   Vec o0, o1;
   if constexpr (!BWD) {
 #pragma unroll
     for (int j = 0; j < N / 2; ++j) {
       float a0, a1, unused;
-      act<false>(p.act, g[2 * j], a0, unused);
-      act<false>(p.act, g[2 * j + 1], a1, unused);
+      act<KIND, false>(g[2 * j], a0, unused);
+      act<KIND, false>(g[2 * j + 1], a1, unused);
       o0[j] = pack_bf16(a0 * u[2 * j], a1 * u[2 * j + 1]);
     }
     *(Vec*)(p.out + (int64_t)m * p.ldo + n) = o0;
@@ -98,13 +113,12 @@ __device__ __forceinline__ void gated_store(const GatedParams& p, int m, int n, 
       }
     }
   } else {
-    const Vec d = *(const Vec*)(p.dh + (int64_t)m * p.lddh + n);
 #pragma unroll
     for (int j = 0; j < N / 2; ++j) {
       const float d0 = bf16f(d[j] & 0xffffu), d1 = __builtin_bit_cast(float, d[j] & 0xffff0000u);
       float a0, a1, b0, b1;
-      act<true>(p.act, g[2 * j], a0, b0);
-      act<true>(p.act, g[2 * j + 1], a1, b1);
+      act<KIND, true>(g[2 * j], a0, b0);
+      act<KIND, true>(g[2 * j + 1], a1, b1);
       o0[j] = pack_bf16(d0 * u[2 * j] * b0, d1 * u[2 * j + 1] * b1);
       o1[j] = pack_bf16(d0 * a0, d1 * a1);
     }
@@ -182,7 +196,7 @@ __global__ void __launch_bounds__(64 * WAVES) gated_rows_kernel(GatedParams p) {
       u[e] *= xs * p.us[p.us_row ? n + e : 0];
     }
   }
-  gated_store<BWD, 4>(p, m, n, g, u);
+  by_act(p.act, [&](auto k) { gated_store<decltype(k)::value, BWD, 4>(p, m, n, g, u, BWD ? load_dh<4>(p, m, n) : u32x2{}); });
 }
 
 // ---------------------------------------------------------------- middle form
@@ -279,7 +293,8 @@ __global__ void __launch_bounds__(kThreads, 2) gated_few_kernel(GatedParams p) {
     float g[8], u[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) g[e] = acc16[e], u[e] = acc16[8 + e];
-    gated_store<BWD, 8>(p, m0 + r, n0 + 16 * wn + 8 * h, g, u);
+    const int n = n0 + 16 * wn + 8 * h;
+    by_act(p.act, [&](auto k) { gated_store<decltype(k)::value, BWD, 8>(p, m0 + r, n, g, u, BWD ? load_dh<8>(p, m0 + r, n) : u32x4{}); });
   } else {
     const int n = n0 + 16 * wn + 4 * q;
 #pragma unroll
@@ -293,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_few_kernel(GatedParams p) {
         g[e] = acc4[ms][0][e] * (xs * p.gs[p.gs_row ? n + e : 0]);
         u[e] = acc4[ms][1][e] * (xs * p.us[p.us_row ? n + e : 0]);
       }
-      gated_store<BWD, 4>(p, m0 + r, n, g, u);
+      by_act(p.act, [&](auto k) { gated_store<decltype(k)::value, BWD, 4>(p, m0 + r, n, g, u, BWD ? load_dh<4>(p, m0 + r, n) : u32x2{}); });
     }
   }
 }
@@ -307,11 +322,14 @@ __global__ void __launch_bounds__(kThreads, 2) gated_few_kernel(GatedParams p) {
 // W rows are permuted in LDS so that a lane holds runs of eight columns.
 // The MFMA is v_mfma_f32_16x16x32_bf16, which takes less power than 32x32x16 for the same
 // bytes (M x D -> F, us, 32x32x16 / 16x16x32: 8 192 x 4 096 -> 10 240 1 091 / 1 037, 37 429 x
-// 1 024 -> 4 096 558 / 540, 37 429 x 512 -> 2 048 161 / 165): 1.32, 1.16 and 0.95 PFLOP/s, where a
-// large library product reaches 1.42.  With g and u kept 8 192 x 4 096 -> 10 240 takes 1 125-1 240,
-// the backward's computation of 37 429 x 512 -> 2 048 223-253.
+// 1 024 -> 4 096 558 / 540, 37 429 x 512 -> 2 048 161 / 165).  Now 1 025, 513 and 154-162: 1.34, 1.22
+// and 1.0 PFLOP/s, where a large library product reaches 1.42.  With g and u kept 8 192 x
+// 4 096 -> 10 240 takes 1 130-1 260; the backward's computation of 37 429 x 512 -> 2 048 197-215.
 // Tiles of 256 rows in one workgroup, with a third less to load, were 4 % faster at D =
 // 4 096 and 7 % slower at D = 1 024.
+// The epilogue has no branch on the activation inside, and the backward's has all of a
+// lane's dh in flight first (each row block waited for its own: 37 429 x 512 -> 2 048 253
+// -> 205-215 us, the forward 170 -> 162; e4m3 111 -> 99).
 template <bool BWD>
 __global__ void __launch_bounds__(kDuoThreads, 2) gated_tile_kernel(GatedParams p, int per_xcd) {
   __shared__ __attribute__((aligned(1024))) uint8_t ring[kDuoSlots][kDuoItem];
@@ -399,21 +417,30 @@ __global__ void __launch_bounds__(kDuoThreads, 2) gated_tile_kernel(GatedParams 
 
   // lane: rows m0 + 16 mb + li, columns n0 + 32 wave + 8 q + (0..7) of both products
   const int cl = n0 + 32 * wave + 8 * q;
+  u32x4 dh[8];
 #pragma unroll
-  for (int mb = 0; mb < 8; ++mb) {
-    const int r = 16 * mb + li;
-    if (r >= mrows) continue;
-    float g[8], u[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) g[e] = acc[mb][e >> 2][e & 3], u[e] = acc[mb][2 + (e >> 2)][e & 3];
-    gated_store<BWD, 8>(p, m0 + r, cl, g, u);
+  for (int mb = 0; mb < 8; ++mb) {  // all in flight before the first is used
+    dh[mb] = u32x4{};
+    if constexpr (BWD) dh[mb] = load_dh<8>(p, m0 + min(16 * mb + li, mrows - 1), cl);
   }
+  __builtin_amdgcn_sched_barrier(0);
+  by_act(p.act, [&](auto k) {
+#pragma unroll
+    for (int mb = 0; mb < 8; ++mb) {
+      const int r = 16 * mb + li;
+      if (r >= mrows) continue;
+      float g[8], u[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) g[e] = acc[mb][e >> 2][e & 3], u[e] = acc[mb][2 + (e >> 2)][e & 3];
+      gated_store<decltype(k)::value, BWD, 8>(p, m0 + r, cl, g, u, dh[mb]);
+    }
+  });
 }
 
 // ---------------------------------------------------------------- tile form, e4m3
 // The same tile, ring and items on rows of e4m3 (a k-step is 128 elements) with
 // v_mfma_f32_16x16x128_f8f6f4: 16-row blocks 0, 1 of a wave's weights are gate
-// rows, 2, 3 up rows.  Measured: 37 429 x 1 024 -> 4 096 310-336 us, 1.9-2.0 PFLOP/s, in eight
+// rows, 2, 3 up rows.  Measured: 37 429 x 1 024 -> 4 096 306-314 us, 2.0 PFLOP/s, in eight
 // k-steps a tile (a large library product 2.63).
 __global__ void __launch_bounds__(kDuoThreads, 2) gated_tile_fp8_kernel(GatedParams p, int per_xcd) {
   __shared__ __attribute__((aligned(1024))) uint8_t ring[kDuoSlots][kDuoItem];
@@ -510,18 +537,20 @@ __global__ void __launch_bounds__(kDuoThreads, 2) gated_tile_fp8_kernel(GatedPar
   for (int s = 1; s < nk - 1; ++s) kstep(s, std::false_type{}, std::false_type{});
   kstep(nk - 1, std::false_type{}, std::true_type{});
 
+  by_act(p.act, [&](auto k) {
 #pragma unroll
-  for (int ms = 0; ms < 8; ++ms) {
-    const int r = 16 * ms + li;
-    if (r >= mrows) continue;
-    float g[8], u[8];
+    for (int ms = 0; ms < 8; ++ms) {
+      const int r = 16 * ms + li;
+      if (r >= mrows) continue;
+      float g[8], u[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      g[e] = acc[ms][e >> 2][e & 3] * (sav[ms] * gsv[e >> 2][e & 3]);
-      u[e] = acc[ms][2 + (e >> 2)][e & 3] * (sav[ms] * usv[e >> 2][e & 3]);
+      for (int e = 0; e < 8; ++e) {
+        g[e] = acc[ms][e >> 2][e & 3] * (sav[ms] * gsv[e >> 2][e & 3]);
+        u[e] = acc[ms][2 + (e >> 2)][e & 3] * (sav[ms] * usv[e >> 2][e & 3]);
+      }
+      gated_store<decltype(k)::value, false, 8>(p, m0 + r, cl, g, u, u32x4{});
     }
-    gated_store<false, 8>(p, m0 + r, cl, g, u);
-  }
+  });
 }
 
 // ---------------------------------------------------------------- backward from kept g and u
@@ -546,16 +575,19 @@ __global__ void __launch_bounds__(256) gated_kept_kernel(KeptArgs a) {
     const f32x4 gv[2] = {*(const f32x4*)k, *(const f32x4*)(k + 4)};
     const f32x4 uv[2] = {*(const f32x4*)(k + a.F), *(const f32x4*)(k + a.F + 4)};
     u32x4 o0, o1;
+    by_act(a.act, [&](auto kind) {
+      constexpr int K = decltype(kind)::value;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t w = d[j];
-      const float d0 = bf16f(w & 0xffffu), d1 = __builtin_bit_cast(float, w & 0xffff0000u);
-      float a0, a1, b0, b1;
-      act<true>(a.act, gv[j >> 1][2 * (j & 1)], a0, b0);
-      act<true>(a.act, gv[j >> 1][2 * (j & 1) + 1], a1, b1);
-      o0[j] = pack_bf16(d0 * uv[j >> 1][2 * (j & 1)] * b0, d1 * uv[j >> 1][2 * (j & 1) + 1] * b1);
-      o1[j] = pack_bf16(d0 * a0, d1 * a1);
-    }
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t w = d[j];
+        const float d0 = bf16f(w & 0xffffu), d1 = __builtin_bit_cast(float, w & 0xffff0000u);
+        float a0, a1, b0, b1;
+        act<K, true>(gv[j >> 1][2 * (j & 1)], a0, b0);
+        act<K, true>(gv[j >> 1][2 * (j & 1) + 1], a1, b1);
+        o0[j] = pack_bf16(d0 * uv[j >> 1][2 * (j & 1)] * b0, d1 * uv[j >> 1][2 * (j & 1) + 1] * b1);
+        o1[j] = pack_bf16(d0 * a0, d1 * a1);
+      }
+    });
     uint16_t* o = a.out + m * a.ldo + n;
     *(u32x4*)o = o0;
     *(u32x4*)(o + a.F) = o1;
