@@ -423,9 +423,10 @@ __global__ void __launch_bounds__(kThreads, 2) mx_few_kernel(MxParams p) {
 //  * Chunk c of LDS row r lies at c ^ ((r >> 1) & 7): 16 consecutive rows read one
 //    chunk each from 16 distinct bank groups.  W rows are permuted in LDS so that a
 //    lane holds runs of eight columns.
-// Measured: 8 192^3 293-342 us, 3.2-3.7 PFLOP/s (a large library product in e4m3 2.6;
-// the instruction alone 7.9 from registers).  Without its MFMAs 206 us, without its
-// loads 235, without its stores 253; a workgroup has the CU's LDS to itself, so nothing runs under its epilogue.
+// Measured: 8 192^3 282-330 us, 3.3-3.9 PFLOP/s (a large library product in e4m3 2.6;
+// the instruction alone 6.5 from registers of random codes, the power limit, 9.9 of
+// zeros).  Without its MFMAs 206 us, without its loads 235; a workgroup has the CU's LDS
+// to itself, so nothing runs under its epilogue.
 constexpr int kMxThreads = 512;
 constexpr int kMxTile = 256;
 constexpr int kMxOperand = kMxTile * 128;    // 32 KiB
@@ -578,28 +579,56 @@ __global__ void __launch_bounds__(kMxThreads, 2) mx_tile_kernel(MxParams p, int 
   }
   step(S - 1, No{}, No{}, No{});
 
-  // lane: rows m0 + 128 wm + 32 mb + lr, columns n0 + 64 wn + 32 nb + 16 run + 8 h + (0..7)
-  const int cl = n0 + 64 * wn + 8 * h;
+  // The lane's outputs, rows 32 mb + lr and columns 32 nb + 16 run + 8 h + (0..7) of the
+  // wave's 128 x 64, go through LDS (chunk c of row r at c ^ ((r >> 1) & 7) of the wave's
+  // 16 KiB), so that a store writes whole lines of 8 rows; the residual
+  // comes the same way.  Straight from the registers they are 32-byte pieces of 32 rows
+  // (us, pieces / lines: 8 192^3 290 / 282, with a residual 401 / 363, 37 429 x 2 048 x 512 (M x N
+  // x K) 74 / 56 and 158 / 113; 2 600 x 2 576 x 768 12.5 / 13.2).
+  dma_barrier<0>();  // every wave has read its last fragments
+  int le = lane;
+  asm volatile("" : "+v"(le));  // what follows is computed here, not kept in registers over the loop
+  const int r8 = le >> 3, wrow = m0 + 128 * wm, wcol = n0 + 64 * wn, c8 = wcol + 8 * (le & 7);
+  const uint32_t mine = 128 * 128 * wave;
+  // row 8 j + r8, chunk le % 8; and row 32 mb + le % 32, chunk 4 nb + 2 run + le / 32
+  auto line_at = [&](int j) { return (mine + 128 * r8 + (((le & 7) ^ (r8 >> 1)) * 16)) ^ (64 * (j & 1)); };
+  auto out_at = [&](int nb, int run) {
+    return (mine + 128 * (le & 31) + (((le >> 5) ^ ((le >> 1) & 7)) * 16)) ^ (64 * nb + 32 * run);
+  };
+  if (p.resid) {
+    const uint16_t* from = p.resid + min(c8, p.N - 8);
+#pragma unroll
+    for (int i = 0; i < 16; i += 8) {
+      u32x4 v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = *(const u32x4*)(from + (int64_t)min(wrow + 8 * (i + j) + r8, p.M - 1) * p.ldr);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) *(u32x4*)(smem + line_at(i + j) + 1024 * (i + j)) = v[j];
+    }
+  }
 #pragma unroll
   for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
     for (int run = 0; run < 2; ++run) {
-      const int c = cl + 32 * nb + 16 * run;
-      if (c >= p.N) continue;
+      const int c = wcol + 32 * nb + 16 * run + 8 * (le >> 5);
       float b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (p.bias) add8(*(const u32x4*)(p.bias + c), b);
+      if (p.bias && c < p.N) add8(*(const u32x4*)(p.bias + c), b);
 #pragma unroll
       for (int mb = 0; mb < 4; ++mb) {
-        const int m = m0 + 128 * wm + 32 * mb + lr;
-        if (m >= p.M) continue;
+        u32x4* at = (u32x4*)(smem + out_at(nb, run) + 4096 * mb);
         float o[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[e] = acc[mb][nb][8 * run + e] + b[e];
-        if (p.resid) add8(*(const u32x4*)(p.resid + (int64_t)m * p.ldr + c), o);
-        *(u32x4*)(p.C + (int64_t)m * p.ldc + c) =
-            u32x4{pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7])};
+        if (p.resid) add8(*at, o);
+        *at = u32x4{pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7])};
       }
     }
+  if (c8 >= p.N) return;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const int m = wrow + 8 * j + r8;
+    if (m < p.M) *(u32x4*)(p.C + (int64_t)m * p.ldc + c8) = *(const u32x4*)(smem + line_at(j) + 1024 * j);
+  }
 }
 
 // the tile form's LDS limit, once a device

@@ -135,9 +135,9 @@ def gated_linear_bwd(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_
 # Keeping g and u costs 16 bytes of memory traffic a value (written and read in
 # fp32), computing them again 4 D operations: equal near D = 1200 at the rates that
 # these kernels reach.  Measured (us on the device a training step, computed again /
-# kept): 37 429 rows x 512 -> 2048 714 / 838, 16 384 x 768 -> 3584 745 / 809, 16 384 x
-# 1024 -> 4096 1030 / 1107, 16 384 x 1280 -> 5120 1628 / 1594, 16 384 x 2048 -> 5632
-# 2721 / 2440, 8192 x 4096 -> 10240 4588 / 3755, 512 x 2048 -> 5632 176 / 154.
+# kept): 37 429 rows x 512 -> 2048 659 / 794, 16 384 x 768 -> 3584 698 / 770, 16 384 x
+# 1024 -> 4096 948 / 1013, 16 384 x 1280 -> 5120 1519 / 1493, 16 384 x 2048 -> 5632
+# 2585 / 2322, 8192 x 4096 -> 10240 4347 / 3584, 512 x 2048 -> 5632 177 / 156.
 RECOMPUTE_BELOW = 1280
 
 
