@@ -192,11 +192,6 @@ def _e4m3_rows(v):
     return (v / scale[:, None]).clamp(-E4M3_MAX, E4M3_MAX).to(E4M3), scale
 
 
-def _pow2(e):
-    """2^e in fp32, -126 <= e <= 127, from its bits (a device's pow and ldexp may be an ulp off)."""
-    return ((e.int() + 127) << 23).view(torch.float32)
-
-
 def _mx_scale_exponent(blocks):
     """E of each block of 32: floor(log2 amax) - 2, -127 at the least."""
     amax = blocks.abs().amax(-1)
@@ -205,10 +200,10 @@ def _mx_scale_exponent(blocks):
 
 
 def _mx_split(v):
-    """(e2m1 codes 0..15 [R, C], E [R, C / 32]) of fp32 rows; nearest, ties to the even code."""
+    """(e2m1 codes 0..15 [R, C], E [R, C / 32]) of fp32 or fp64 rows; nearest, ties to the even code."""
     blocks = v.reshape(v.shape[0], -1, 32)
     exponent = _mx_scale_exponent(blocks)
-    t = blocks.abs() * _pow2(-exponent)[..., None]
+    t = torch.ldexp(blocks.abs(), -exponent[..., None])
     code = ((t > 0.25).int() + (t >= 0.75) + (t > 1.25) + (t >= 1.75) + (t > 2.5) + (t >= 3.5) + (t > 5.0))
     code = code + 8 * torch.signbit(blocks)
     return code.reshape(v.shape), exponent
@@ -225,8 +220,7 @@ def _mx_values(code, exponent, dtype):
     table = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -3.0, -4.0, -6.0],
                          dtype=dtype, device=code.device)
     v = table[code.long()].reshape(code.shape[0], -1, 32)
-    half = torch.where(exponent < -126, 0.5, 1.0)[..., None]  # 2^-127 is below fp32's normal range
-    return (v * half * _pow2(exponent.clamp(min=-126))[..., None]).reshape(code.shape)
+    return torch.ldexp(v, exponent[..., None]).reshape(code.shape)
 
 
 def _mx_unpack(packed, dtype):
@@ -385,7 +379,7 @@ def _mx64(v):
     e = torch.where(torch.exp2(e) > top, e - 1, e)
     e = torch.where(torch.exp2(e + 1) <= top, e + 1, e)
     e = torch.where(top > 0, (e - 2).clamp(min=-127), torch.full_like(e, -127))
-    unit = ((e.long() + 1023) << 52).view(torch.float64)[..., None]
+    unit = torch.exp2(e)[..., None]
     t = (b.abs() / unit).clamp(max=6.0)
     # steps of 0.5 up to 2, 1 up to 4, 2 beyond; torch.round takes ties to even
     step = torch.where(t < 2, 0.5, torch.where(t < 4, 1.0, 2.0))
@@ -424,7 +418,7 @@ def exact(case, seed):
         codes, scales = s["weight"]
         nibbles = torch.stack((codes % 16, codes // 16), 2).flatten(1).long()
         size = torch.tensor(_E2M1, dtype=torch.float64, device=codes.device)[nibbles % 8]
-        unit = ((scales.long() + (1023 - 127)) << 52).view(torch.float64).repeat_interleave(32, 1)
+        unit = torch.exp2(scales.double() - 127).repeat_interleave(32, 1)
         w = torch.where(nibbles >= 8, -size, size) * unit
         out = _mx64(s["x"])[0] @ w.t() + s["bias"].double()
         return out if s["residual"] is None else out + s["residual"].double()
