@@ -348,6 +348,13 @@ __device__ __forceinline__ f32x16 mfma32_bf16(u32x4 a, u32x4 b, f32x16 c) {
                                                  0, 0);
 }
 
+// The LDS accesses of a wave's lanes before it come before those after it.  A wave's
+// LDS instructions execute in order, so this holds the compiler to it and emits nothing.
+__device__ __forceinline__ void wave_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 // every wave's LDS reads are done (no memory fence: nothing waits for stores)
 __device__ __forceinline__ void pc_barrier_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 

@@ -585,6 +585,7 @@ __global__ void __launch_bounds__(kMxThreads, 2) mx_tile_kernel(MxParams p, int 
   // comes the same way.  Straight from the registers they are 32-byte pieces of 32 rows
   // (us, pieces / lines: 8 192^3 290 / 282, with a residual 401 / 363, 37 429 x 2 048 x 512 (M x N
   // x K) 74 / 56 and 158 / 113; 2 600 x 2 576 x 768 12.5 / 13.2).
+  // A wave's lanes read what others of its lanes wrote: wave_lds_order() between the two.
   dma_barrier<0>();  // every wave has read its last fragments
   int le = lane;
   asm volatile("" : "+v"(le));  // what follows is computed here, not kept in registers over the loop
@@ -605,6 +606,7 @@ __global__ void __launch_bounds__(kMxThreads, 2) mx_tile_kernel(MxParams p, int 
 #pragma unroll
       for (int j = 0; j < 8; ++j) *(u32x4*)(smem + line_at(i + j) + 1024 * (i + j)) = v[j];
     }
+    wave_lds_order();
   }
 #pragma unroll
   for (int nb = 0; nb < 2; ++nb)
@@ -623,6 +625,7 @@ __global__ void __launch_bounds__(kMxThreads, 2) mx_tile_kernel(MxParams p, int 
         *at = u32x4{pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7])};
       }
     }
+  wave_lds_order();
   if (c8 >= p.N) return;
 #pragma unroll
   for (int j = 0; j < 16; ++j) {

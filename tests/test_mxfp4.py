@@ -263,6 +263,22 @@ def test_past_32_bit_offsets(hip_lib):
     assert not out[:-5].any()
 
 
+def test_tile_epilogue_orders_its_lanes():
+    """The tile form's outputs pass between the lanes of a wave through LDS, the residual before them: each
+    exchange has a wave-level order between the lanes' writes and the others' reads, in the source, since a
+    compiler that leaves the order alone hides a missing one."""
+    from pathlib import Path
+
+    src = (Path(__file__).parents[1] / "mlperf-training_amd" / "csrc" / "hstu_mxfp4.hip").read_text()
+    body = src[src.index("void __launch_bounds__(kMxThreads, 2) mx_tile_kernel"):]
+    body = body[body.index("auto line_at"):body.index("hipError_t set_mx_lds")]
+    resid_in = body.index("*(u32x4*)(smem + line_at(")          # rows in, lane = row and chunk of a line
+    meet = body.index("smem + out_at(nb, run)")                 # the accumulators' lanes
+    lines_out = body.rindex("*(const u32x4*)(smem + line_at(")  # whole lines again
+    assert resid_in < meet < lines_out
+    assert "wave_lds_order();" in body[resid_in:meet] and "wave_lds_order();" in body[meet:lines_out]
+
+
 # ---------------------------------------------------------------- refusals
 def test_oracle_packs_and_unpacks():
     x = rnd((5, 96), 1, 3.0)
