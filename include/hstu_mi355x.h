@@ -618,7 +618,9 @@ int hstu_dequantize_do_e4m3_blk(const void* dout_e4m3, const void* e8, int64_t T
  * scale_in NULL, the row's own s = max|y| / 448 (1 / 448 for a row of zeros),
  * written to scale_out [rows]; exactly one of the two is given.  NaN stays
  * NaN.  rstd: fp32 [rows] for the backward, or NULL.  Statistics are fp32.
- * h may be x or residual, and y may be x, in place (same pointer and stride).
+ * In place: h may be x or residual, and y of the input's type may be x or
+ * residual (same pointer and stride).  Any other overlap of an output with an
+ * input or with the other output, and every overlap of an e4m3 y, is refused.
  * No counterpart in the reference's HSTU path, which norms with LayerNorm
  * (ops/triton/triton_layer_norm.py:1668-1740).
  */

@@ -457,6 +457,16 @@ void by_type(bool f32, bool vec, int D, A... args) {
 bool aligned16(const void* p, int64_t ld_bytes) { return (uintptr_t)p % 16 == 0 && ld_bytes % 16 == 0; }
 // element alignment, which every access needs
 bool aligned_es(const void* p, int es) { return (uintptr_t)p % es == 0; }
+// Whether rows of `a` (wa bytes each, lda apart) and of `b` share a byte.  Rows of one
+// stride may interleave (columns of one wide buffer); of two strides their whole
+// ranges have to be apart.
+bool share(const void* pa, int64_t lda, int64_t wa, const void* pb, int64_t ldb, int64_t wb, int64_t rows) {
+  const int64_t a = (int64_t)(uintptr_t)pa, b = (int64_t)(uintptr_t)pb;
+  if (a + (rows - 1) * lda + wa <= b || b + (rows - 1) * ldb + wb <= a) return false;
+  if (lda != ldb || rows == 1) return true;
+  const int64_t d = ((b - a) % lda + lda) % lda;  // where b's rows begin within a's
+  return d < wa || d + wb > lda;
+}
 
 }  // namespace
 
@@ -494,6 +504,16 @@ extern "C" int hstu_rms_norm_fwd(int dtype, const void* x, int64_t ldx, const vo
   a.w_f32 = ws == 4;
   a.eps = eps;
   a.inv_d = 1.f / (float)D;
+  // Row groups run in any order, so an output may lie on an input only where each
+  // row lies on itself: the same address, stride and type.  e4m3 rows are shorter.
+  const int64_t in_w = (int64_t)D * es, y_w = out8 ? D : in_w;
+  auto clash = [&](const void* out, int64_t ldo, int64_t wo, const void* in, int64_t ldi) {
+    return share(out, ldo, wo, in, ldi, in_w, rows) && !(out == in && ldo == ldi && wo == in_w);
+  };
+  if (clash(y, a.ldy, y_w, x, a.ldx)) return HSTU_E_BAD_ARG;
+  if (residual && (clash(y, a.ldy, y_w, residual, a.ldr) || clash(h, a.ldh, in_w, x, a.ldx) ||
+                   clash(h, a.ldh, in_w, residual, a.ldr) || share(y, a.ldy, y_w, h, a.ldh, in_w, rows)))
+    return HSTU_E_BAD_ARG;
   const bool vec = D % 8 == 0 && aligned16(x, a.ldx) && aligned16(weight, 0) &&
                    (!residual || (aligned16(residual, a.ldr) && aligned16(h, a.ldh))) &&
                    (out8 ? (uintptr_t)y % 8 == 0 && a.ldy % 8 == 0 : aligned16(y, a.ldy));

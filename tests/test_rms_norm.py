@@ -288,7 +288,65 @@ def test_side_stream_and_graph(hip_lib):
             assert torch.equal(a.float(), b.float()), k
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,D", [(1, 512), (37, 512), (5, 513), (300, 5120)])
+def test_in_place(hip_lib, rows, D, dtype):
+    """The C entry with h on x or on the residual, and y on x or on the residual; columns of one buffer beside each other."""
+    import hstu_amd
+    import hstu_amd._lib as lib
+
+    f = lib.fn("hstu_rms_norm_fwd")
+    code = lib.HSTU_DTYPE_BF16 if dtype == torch.bfloat16 else lib.HSTU_DTYPE_FP32
+    x, r, w = make(rows, D, dtype, 1).to(DEV), make(rows, D, dtype, 2, 3.0).to(DEV), make_weight(D, torch.float32).to(DEV)
+    y0, h0, _, _ = hstu_amd.rms_norm_fwd(x, w, EPS, residual=r)
+    alone, _, _, _ = hstu_amd.rms_norm_fwd(x, w, EPS)
+
+    def call(x, ldx, r, ldr, h, ldh, y, ldy):
+        return f(code, x.data_ptr(), ldx, lib.ptr(r), ldr, w.data_ptr(), lib.HSTU_DTYPE_FP32, EPS, rows, D, lib.ptr(h), ldh,
+                 y.data_ptr(), ldy, code, None, None, None, lib.stream(x))
+
+    for on in ("h on x", "h on residual", "y on x", "y on residual"):
+        a, b, new = x.clone(), r.clone(), torch.empty_like(x)
+        h, y = {"h on x": (a, new), "h on residual": (b, new), "y on x": (new, a), "y on residual": (new, b)}[on]
+        assert call(a, D, b, D, h, D, y, D) == 0
+        assert torch.equal(h, h0) and torch.equal(y, y0), on
+    a = x.clone()
+    assert call(a, D, None, 0, None, 0, a, D) == 0 and torch.equal(a, alone)
+    wide = torch.full((rows, 4 * D), 7.0, dtype=dtype, device=DEV)
+    a, b, h, y = (wide[:, i * D:(i + 1) * D] for i in range(4))
+    a.copy_(x), b.copy_(r)
+    assert call(a, 4 * D, b, 4 * D, h, 4 * D, y, 4 * D) == 0
+    assert torch.equal(a, x) and torch.equal(b, r) and torch.equal(h, h0) and torch.equal(y, y0)
+
+
 # ---------------------------------------------------------------- refusals, without a GPU
+def test_c_entry_refuses_overlaps():
+    """An output that lies on rows which another row group has still to read, and an e4m3 y on anything."""
+    import hstu_amd._lib as lib
+
+    f = lib.fn("hstu_rms_norm_fwd")
+    BF, F32, F8 = lib.HSTU_DTYPE_BF16, lib.HSTU_DTYPE_FP32, lib.HSTU_DTYPE_FP8_E4M3
+    X, R, H, Y, D, rows = 1 << 20, 2 << 20, 3 << 20, 4 << 20, 64, 8  # stand-in addresses, never read
+
+    def fwd(dtype=BF, x=X, ldx=D, res=R, ldr=D, h=H, ldh=D, y=Y, ldy=D, od=None, rows=rows):
+        out8 = od == F8
+        return f(dtype, x, ldx, res, ldr, 64, F32, 1e-6, rows, D, h, ldh, y, ldy, dtype if od is None else od, None,
+                 64 if out8 else None, None, None)
+
+    for dtype, es in ((BF, 2), (F32, 4)):
+        span = rows * D * es
+        for rows_ in (1, rows):
+            for bad in (dict(od=F8, y=X), dict(od=F8, y=R), dict(od=F8, y=H), dict(od=F8, y=X, res=None, h=None),
+                        dict(od=F8, y=X, ldy=D * es)):
+                assert fwd(dtype, rows=rows_, **bad) == lib.HSTU_E_BAD_ARG, bad
+        for bad in (dict(od=F8, y=X + span - 16), dict(od=F8, y=X - D * rows + 16), dict(y=X + es), dict(y=X + span - es),
+                    dict(y=X - span + es), dict(h=X + es), dict(h=R - es), dict(y=R + es), dict(y=X, ldy=D + 8),
+                    dict(h=X, ldh=2 * D), dict(y=H), dict(y=X, h=X), dict(y=X, res=None, h=None, ldy=2 * D),
+                    dict(x=X, ldx=2 * D, y=X + es * (D - 8), ldy=2 * D), dict(x=X, ldx=2 * D, y=X + es * (D + 8), ldy=2 * D)):
+            assert fwd(dtype, **bad) == lib.HSTU_E_BAD_ARG, bad
+
+
 def test_refusals():
     import hstu_amd
     from hstu_amd.hstu_rms_norm import MAX_D
