@@ -322,6 +322,21 @@ def guard_graph(ctx, t) -> None:
                                       "up on a side stream")
 
 
+_forward_ad = None
+
+
+def no_tangent(name: str, *tensors) -> None:
+    """Refuses dual tensors of ``torch.autograd.forward_ad``, which do not require
+    grad: a kernel takes their values alone, and the tangent would be lost."""
+    global _forward_ad
+    if _forward_ad is None:
+        from torch.autograd import forward_ad as _forward_ad
+    if _forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{name}: forward-mode derivatives (an input has a tangent)")
+
+
 def ptr(t) -> Optional[int]:
     """Device address of a tensor (None for None)."""
     return None if t is None else t.data_ptr()

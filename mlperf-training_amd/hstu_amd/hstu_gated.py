@@ -164,6 +164,7 @@ class GatedLinearFunction(torch.autograd.Function):
     def backward(ctx, dh):
         if torch.is_grad_enabled():  # only under create_graph
             raise NotImplementedError("second derivatives (create_graph=True)")
+        _lib.no_tangent("the backward of gated_linear", dh)
         x, w_gate, w_up, gu = ctx.saved_tensors
         need_x, need_g, need_u = ctx.needs_input_grad[:3]
         dx, dg, du = gated_linear_bwd(dh, x, w_gate, w_up, ctx.activation, need_x, need_g or need_u, gu)
@@ -176,7 +177,9 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, acti
     Differentiable in x and both weights.  ``recompute``: the backward computes g
     and u again (nothing but x and the weights is kept) instead of keeping them
     in fp32, 8 bytes a value of h; None: where that is the faster way (D < 1280).
-    The gradients are the same bytes.  Not differentiable a second time."""
+    The gradients are the same bytes.  Not differentiable a second time, nor in
+    forward mode."""
+    _lib.no_tangent("gated_linear", x, w_gate, w_up)
     if not (torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad)):
         return gated_linear_fwd(x, w_gate, w_up, activation)
     if recompute is None:

@@ -156,6 +156,7 @@ class RMSNormFunction(torch.autograd.Function):
     def backward(ctx, dy, dh=None):
         if torch.is_grad_enabled():  # only under create_graph
             raise NotImplementedError("second derivatives (create_graph=True)")
+        _lib.no_tangent("the backward of rms_norm", dy, dh)
         if dy is None:  # only h was used
             return dh, None, None, dh
         h, weight, rstd = ctx.saved_tensors
@@ -178,7 +179,8 @@ class RMSNormFunction(torch.autograd.Function):
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None):
     """``y``, or ``(y, h)`` with a residual: h = x + residual is the new residual
     stream and y its norm times ``weight``.  Differentiable in x, residual and
-    weight, through y and h; not a second time."""
+    weight, through y and h; not a second time, nor in forward mode."""
+    _lib.no_tangent("rms_norm", x, weight, residual)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
                                     or (residual is not None and residual.requires_grad)):
         return RMSNormFunction.apply(x, weight, eps, residual)

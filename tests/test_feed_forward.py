@@ -189,3 +189,52 @@ def test_no_second_derivative(hip_lib):
     for y in (hstu_amd.rms_norm(x, w), hstu_amd.gated_linear(x, wg, wu)):
         with pytest.raises(NotImplementedError):
             torch.autograd.grad(y.float().sum(), x, create_graph=True)
+
+
+def test_no_forward_mode(monkeypatch):
+    """A dual tensor does not require grad, and its tangent is refused, not dropped; other tensors in a dual
+    level are served.  Checked without a device: nothing is launched."""
+    import torch.autograd.forward_ad as fwd
+    from hstu_amd import hstu_gated, hstu_rms_norm
+
+    served = []
+    monkeypatch.setattr(hstu_rms_norm, "rms_norm_fwd", lambda x, *a, **k: served.append(x) or (x, x, x, x))
+    monkeypatch.setattr(hstu_gated, "gated_linear_fwd", lambda x, *a, **k: served.append(x) or x)
+    x, w, wg = torch.ones(4, 256), torch.ones(256), torch.ones(128, 256)
+    with fwd.dual_level():
+        def dual(t):
+            return fwd.make_dual(t, torch.ones_like(t))
+
+        with torch.no_grad():  # forward mode goes on without grad mode
+            for args in ((dual(x), w), (x, dual(w)), (x, w, 1e-6, dual(x))):
+                with pytest.raises(NotImplementedError):
+                    hstu_rms_norm.rms_norm(*args)
+        for args in ((dual(x), wg, wg), (x, dual(wg), wg), (x, wg, dual(wg))):
+            with pytest.raises(NotImplementedError):
+                hstu_gated.gated_linear(*args)
+        assert not served
+        hstu_rms_norm.rms_norm(x, w)
+        hstu_gated.gated_linear(x, wg, wg)
+        assert len(served) == 2
+    for t in (x, w, wg):
+        t.requires_grad_(True)
+    with fwd.dual_level():  # reverse mode over dual inputs, too
+        with pytest.raises(NotImplementedError):
+            hstu_rms_norm.rms_norm(dual(x), w)
+        with pytest.raises(NotImplementedError):
+            hstu_gated.gated_linear(x, wg, dual(wg))
+
+
+@gpu
+def test_no_forward_mode_through_the_backward(hip_lib):
+    """Reverse mode with a dual gradient."""
+    import hstu_amd
+    import torch.autograd.forward_ad as fwd
+
+    x, w = rnd((4, 256), 1).requires_grad_(True), norm_weight(256, 2)
+    wg, wu = rnd((128, 256), 3, 0.1), rnd((128, 256), 4, 0.1)
+    for y in (hstu_amd.rms_norm(x, w), hstu_amd.gated_linear(x, wg, wu)):
+        g = torch.ones_like(y)
+        with fwd.dual_level():
+            with pytest.raises(NotImplementedError):
+                torch.autograd.grad(y, x, fwd.make_dual(g, g))
