@@ -337,6 +337,18 @@ def no_tangent(name: str, *tensors) -> None:
                 raise NotImplementedError(f"{name}: forward-mode derivatives (an input has a tangent)")
 
 
+def forward_only(name: str, *tensors) -> None:
+    """Refuses inputs whose derivative a function without a backward would cut off."""
+    import torch
+
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise NotImplementedError(f"{name} is forward only and an input requires grad: call it under "
+                                          "torch.no_grad(), or on detached inputs")
+    no_tangent(name, *tensors)
+
+
 def ptr(t) -> Optional[int]:
     """Device address of a tensor (None for None)."""
     return None if t is None else t.data_ptr()

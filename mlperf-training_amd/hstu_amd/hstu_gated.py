@@ -199,9 +199,10 @@ def gated_linear_fp8(x8: torch.Tensor, x_scale: torch.Tensor, gate: Scaled, up: 
                      ) -> torch.Tensor:
     """The forward from e4m3: x8 [.., D] with one fp32 scale or one a row, and
     ``gate``, ``up`` as pairs (e4m3 [F, D], scale: one or [F]).  h [.., F] in bf16,
-    which carries no gradient."""
+    which carries no gradient; inputs that require grad are refused while grad mode is on."""
     act = _act(activation)
     (g8, gs), (u8, us) = gate, up
+    _lib.forward_only("gated_linear_fp8", x8, x_scale, g8, gs, u8, us)
     F, D = _check(x8, g8, u8, E4M3, 128)
     x2, g2, u2 = _rows2d(x8), _rows2d(g8), _rows2d(u8)
     M = x2.shape[0]

@@ -192,6 +192,8 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
                  scale: Optional[torch.Tensor] = None):
     """``(y8, scale)`` or, with a residual, ``(y8, scale, h)``: the norm in e4m3,
     y = y8 * scale with one fp32 scale a row ([rows], max|y| / 448) or the given
-    one (returned as [1]).  Forward only: nothing returned carries a gradient."""
+    one (returned as [1]).  Forward only: nothing returned carries a gradient, and
+    inputs that require grad are refused while grad mode is on."""
+    _lib.forward_only("rms_norm_fp8", x, weight, residual, scale)
     y8, h, _, s = rms_norm_fwd(x, weight, eps, residual, output_fp8=True, scale=scale, want_rstd=False)
     return (y8, s) if residual is None else (y8, s, h)

@@ -127,7 +127,9 @@ def _weight(weight: Packed) -> Tuple[torch.Tensor, torch.Tensor, int, int]:
 def mxfp4_mm(a: Packed, weight: Packed, bias: Optional[torch.Tensor] = None,
              residual: Optional[torch.Tensor] = None) -> torch.Tensor:
     """a @ weight^T (+ bias [N]) (+ residual [.., N]) in bf16, fp32 accumulation:
-    a a pair of [.., K], weight a pair of [N, K]; N a multiple of 16, K of 128."""
+    a a pair of [.., K], weight a pair of [N, K]; N a multiple of 16, K of 128.
+    Forward only, as ``mxfp4_linear``."""
+    _lib.forward_only("mxfp4_mm", bias, residual)
     wc, ws, N, K = _weight(weight)
     ac, as_ = a
     _pair("a", ac, as_)
@@ -150,7 +152,9 @@ def mxfp4_mm(a: Packed, weight: Packed, bias: Optional[torch.Tensor] = None,
 def mxfp4_linear(x: torch.Tensor, weight: Packed, bias: Optional[torch.Tensor] = None,
                  residual: Optional[torch.Tensor] = None) -> torch.Tensor:
     """quantize(x) @ weight^T (+ bias) (+ residual) in bf16, for bf16 x [.., K].
-    Forward only: the result carries no gradient."""
+    Forward only: the result carries no gradient, and inputs that require grad are
+    refused while grad mode is on."""
+    _lib.forward_only("mxfp4_linear", x, bias, residual)
     if x.dtype != torch.bfloat16:
         raise NotImplementedError(f"x: bf16 (got {x.dtype})")
     wc, ws, N, K = _weight(weight)

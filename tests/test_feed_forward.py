@@ -238,3 +238,48 @@ def test_no_forward_mode_through_the_backward(hip_lib):
         with fwd.dual_level():
             with pytest.raises(NotImplementedError):
                 torch.autograd.grad(y, x, fwd.make_dual(g, g))
+
+
+def forward_only_calls(dev):
+    """Each forward-only entry point with the names of its inputs that could carry a derivative."""
+    import hstu_amd
+
+    def z(*shape, dtype=torch.bfloat16):
+        return torch.zeros(shape, dtype=dtype, device=dev)
+
+    f8, f32, u8 = torch.float8_e4m3fn, torch.float32, torch.uint8
+    packed = (z(16, 64, dtype=u8), z(16, 4, dtype=u8))
+    return (
+        (dict(x=z(2, 128), w=z(128), r=z(2, 128), s=z(1, dtype=f32)),
+         lambda x, w, r, s: hstu_amd.rms_norm_fp8(x, w, EPS, residual=r, scale=s)),
+        (dict(x=z(2, 128).to(f8), xs=z(2, dtype=f32), gs=z(128, dtype=f32), us=z(1, dtype=f32)),
+         lambda x, xs, gs, us: hstu_amd.gated_linear_fp8(x, xs, (z(128, 128).to(f8), gs), (z(128, 128).to(f8), us))),
+        (dict(x=z(2, 128), b=z(16), r=z(2, 16)), lambda x, b, r: hstu_amd.mxfp4_linear(x, packed, bias=b, residual=r)),
+        (dict(b=z(16), r=z(16, 16)), lambda b, r: hstu_amd.mxfp4_mm(packed, packed, bias=b, residual=r)),
+    )
+
+
+def test_forward_only_refuses_derivatives():
+    """An input that requires grad would be cut off from the result without a word.  Refused before any look at
+    the device, so this runs without one."""
+    import torch.autograd.forward_ad as fwd
+
+    for inputs, call in forward_only_calls("cpu"):
+        for name, t in inputs.items():
+            with pytest.raises(NotImplementedError, match="forward only"):
+                call(**{**inputs, name: t.clone().requires_grad_(True)})
+            if t.dtype == torch.float8_e4m3fn:
+                continue
+            with fwd.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+                call(**{**inputs, name: fwd.make_dual(t, torch.ones_like(t))})
+
+
+@gpu
+def test_forward_only_without_grad_mode(hip_lib):
+    for inputs, call in forward_only_calls(DEV):
+        leaves = {name: t.clone().requires_grad_(True) for name, t in inputs.items()}
+        with torch.no_grad():
+            out = call(**leaves)
+        for t in out if isinstance(out, tuple) else (out,):
+            assert not t.requires_grad
+        call(**inputs)  # nor anything refused where nothing requires grad
