@@ -37,12 +37,17 @@ def _act(activation: str) -> int:
     return ACTIVATIONS[activation]
 
 
-def _rows2d(t: torch.Tensor) -> torch.Tensor:
-    """[rows, width] with unit column stride and 16-byte aligned rows."""
+FAR = 2 ** 24  # bytes between rows from which on the kernels' 32-bit offsets do not reach over a tile
+
+
+def _rows2d(t: torch.Tensor, far: int = FAR) -> torch.Tensor:
+    """[rows, width] with unit column stride and 16-byte aligned rows less than ``far`` bytes apart (a view
+    such as one position of every sequence is copied where they are further)."""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
     s0, s1 = t.stride()
-    if s1 == 1 and t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or (s0 >= t.shape[1] and s0 * t.element_size() % 16 == 0)):
+    apart = s0 * t.element_size()
+    if s1 == 1 and t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or (s0 >= t.shape[1] and apart % 16 == 0 and apart < far)):
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
@@ -97,7 +102,7 @@ def gated_linear_bwd(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_
     device = x.device
     if dh.shape != x.shape[:-1] + (F,) or dh.dtype != torch.bfloat16 or dh.device != device:
         raise ValueError(f"dh {tuple(dh.shape)} {dh.dtype}; expected {tuple(x.shape[:-1] + (F,))} bf16 on {device}")
-    x2, g, u, d2 = _rows2d(x), _rows2d(w_gate), _rows2d(w_up), _rows2d(dh)
+    x2, g, u, d2 = _rows2d(x), _rows2d(w_gate), _rows2d(w_up), _rows2d(dh, 2 ** 63)  # dh: 64-bit offsets
     M = x2.shape[0]
     if gu is not None and (gu.shape != (M, 2 * F) or gu.dtype != torch.float32 or not gu.is_contiguous()
                            or gu.device != device):

@@ -83,12 +83,17 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dty
     return out
 
 
-def _aligned(t: torch.Tensor, n: int) -> torch.Tensor:
-    """A 2-D operand with unit column stride and rows at multiples of n bytes."""
+FAR = 2 ** 23  # bytes between rows from which on the product's 32-bit offsets do not reach over a tile
+
+
+def _aligned(t: torch.Tensor, n: int, far: int = FAR) -> torch.Tensor:
+    """A 2-D operand with unit column stride and rows at multiples of n bytes, less than ``far`` bytes apart (a
+    view such as one position of every sequence is copied where they are further)."""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
     s0, s1 = t.stride()
-    if s1 == 1 and t.data_ptr() % n == 0 and (t.shape[0] <= 1 or (s0 >= t.shape[1] and s0 * t.element_size() % n == 0)):
+    apart = s0 * t.element_size()
+    if s1 == 1 and t.data_ptr() % n == 0 and (t.shape[0] <= 1 or (s0 >= t.shape[1] and apart % n == 0 and apart < far)):
         return t
     t = t.contiguous()
     return t if t.data_ptr() % n == 0 else t.clone()
@@ -109,7 +114,7 @@ def _epilogue(bias: Optional[torch.Tensor], residual: Optional[torch.Tensor], sh
         if residual.shape != shape or residual.device != device or residual.dtype != torch.bfloat16:
             raise ValueError(f"residual {tuple(residual.shape)} {residual.dtype} on {residual.device}; expected "
                              f"{tuple(shape)} bf16 on {device}")
-        residual = _aligned(residual, 16)
+        residual = _aligned(residual, 16, 2 ** 63)  # 64-bit offsets
     return bias, residual
 
 

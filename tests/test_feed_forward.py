@@ -283,3 +283,55 @@ def test_forward_only_without_grad_mode(hip_lib):
         for t in out if isinstance(out, tuple) else (out,):
             assert not t.requires_grad
         call(**inputs)  # nor anything refused where nothing requires grad
+
+
+@pytest.mark.parametrize("name,limit,es", [("hstu_gated", 2 ** 24, 2), ("mxfp4", 2 ** 23, 2), ("mxfp4", 2 ** 23, 1)])
+def test_rows_far_apart_are_copied(name, limit, es):
+    """Views whose rows are too far apart for the kernels' 32-bit offsets, as the last position of every
+    sequence: copied; the farthest that the kernels take stay in place.  The memory is never touched whole."""
+    import importlib
+
+    mod = importlib.import_module("hstu_amd." + name)
+    fit = mod._rows2d if name == "hstu_gated" else lambda t: mod._aligned(t, 16)
+    dtype = torch.bfloat16 if es == 2 else torch.uint8
+    for apart, copied in ((limit - 16, False), (limit, True), (4 * limit, True)):
+        base = torch.empty(3 * apart // es + 64, dtype=dtype)
+        view = base.as_strided((3, 32), (apart // es, 1))
+        view.copy_(torch.arange(96).reshape(3, 32))
+        got = fit(view)
+        assert torch.equal(got, view) and (got.data_ptr() != view.data_ptr()) == copied
+        assert mod._ld(got) * es < limit
+        one = view[1:2]  # a single row has no distance
+        assert fit(one).data_ptr() == one.data_ptr() and mod._ld(fit(one)) == 32
+
+
+@gpu
+def test_last_position_of_every_sequence(hip_lib):
+    """hidden[:, -1] of long sequences: rows of activations, of dh and of the residual 16 MiB apart and more."""
+    import hstu_amd
+    from hstu_amd.fp8 import quantize_e4m3_rows
+
+    for seqs, D in ((8, 512), (40, 256)):
+        F = 256
+        hidden = torch.zeros((seqs, 2 ** 24 // D, D), dtype=torch.bfloat16, device=DEV)  # 32 MiB a sequence
+        x = hidden[:, -1]
+        x.copy_(rnd((seqs, D), 1))
+        wg, wu, w = rnd((F, D), 2, D ** -0.5), rnd((F, D), 3, D ** -0.5), norm_weight(D, 4)
+        pair = hstu_amd.quantize_mxfp4(rnd((D, D), 5, D ** -0.5))
+        (g8, gs), (u8, us) = quantize_e4m3_rows(wg), quantize_e4m3_rows(wu)
+        x8 = x.to(torch.float8_e4m3fn)
+        far8 = torch.zeros((seqs, 2 ** 24), dtype=torch.float8_e4m3fn, device=DEV)[:, :D]
+        far8.copy_(x8)
+        s = torch.ones(seqs, device=DEV)
+
+        def all_of(x, x8):
+            leaf = x.detach().requires_grad_(True)
+            h = hstu_amd.gated_linear(leaf, wg, wu)
+            dh = x[:, :F]
+            return ((h.detach(),) + hstu_amd.gated_linear_bwd(dh, x, wg, wu) + torch.autograd.grad(h, leaf, dh)
+                    + (hstu_amd.gated_linear_fp8(x8, s, (g8, gs.reshape(-1)), (u8, us.reshape(-1))),
+                       hstu_amd.mxfp4_linear(x, pair), hstu_amd.mxfp4_linear(x.contiguous(), pair, residual=x),
+                       hstu_amd.rms_norm(x, w)))
+
+        for got, want in zip(all_of(x, far8), all_of(x.contiguous(), x8)):
+            assert torch.equal(got, want)
