@@ -714,6 +714,10 @@ int hstu_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, i
 int hstu_mxfp4_gemm(const void* A, int64_t lda, const void* a_scale, int64_t ldas, const void* W, int64_t ldw,
                     const void* w_scale, int64_t ldws, const void* bias, const void* residual, int64_t ldr, void* C,
                     int64_t ldc, int M, int N, int K, hipStream_t stream);
+/* The same with bias [N] in fp32 (16-byte aligned), added to the fp32 sum as it is. */
+int hstu_mxfp4_gemm_bias_fp32(const void* A, int64_t lda, const void* a_scale, int64_t ldas, const void* W, int64_t ldw,
+                              const void* w_scale, int64_t ldws, const float* bias, const void* residual, int64_t ldr,
+                              void* C, int64_t ldc, int M, int N, int K, hipStream_t stream);
 
 /*
  * The same product from bf16 x [M, K] (ldx in elements, rows 16-byte aligned),
@@ -725,6 +729,10 @@ int hstu_mxfp4_gemm(const void* A, int64_t lda, const void* a_scale, int64_t lda
 int hstu_mxfp4_linear_rows(const void* x, int64_t ldx, const void* W, int64_t ldw, const void* w_scale, int64_t ldws,
                            const void* bias, const void* residual, int64_t ldr, void* C, int64_t ldc, int M, int N,
                            int K, hipStream_t stream);
+/* The same with bias [N] in fp32 (16-byte aligned). */
+int hstu_mxfp4_linear_rows_bias_fp32(const void* x, int64_t ldx, const void* W, int64_t ldw, const void* w_scale,
+                                     int64_t ldws, const float* bias, const void* residual, int64_t ldr, void* C,
+                                     int64_t ldc, int M, int N, int K, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -169,11 +169,12 @@ struct MxParams {
   const uint8_t* as;
   const uint8_t* ws;
   int64_t lda, ldw, ldas, ldws;  // bytes
-  const uint16_t* bias;          // bf16 [N] or null
+  const void* bias;              // [N], bf16 or fp32, or null
   const uint16_t* resid;         // bf16 or null
   uint16_t* C;
   int64_t ldr, ldc;  // elements
   int M, N, K;
+  int bias_f32;
 };
 
 // e2m1 x e2m1 (16x16x128) with E8M0 scales: lane (li, q) holds values 32 q .. 32 q
@@ -192,10 +193,23 @@ __device__ __forceinline__ void add8(u32x4 b, float (&v)[8]) {  // eight bf16
     v[2 * j + 1] += __builtin_bit_cast(float, x & 0xffff0000u);
   }
 }
+// The bias of eight columns from n on: added as it is, fp32 or bf16
+__device__ __forceinline__ void add_bias8(const MxParams& p, int n, float (&v)[8]) {
+  if (p.bias_f32) {
+    const f32x4* b = (const f32x4*)((const float*)p.bias + n);
+    const f32x4 b0 = b[0], b1 = b[1];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += b0[e], v[4 + e] += b1[e];
+  } else {
+    add8(*(const u32x4*)((const uint16_t*)p.bias + n), v);
+  }
+}
 // Four consecutive outputs of row m from column n on.
 __device__ __forceinline__ void mx_store4(const MxParams& p, int m, int n, f32x4 v) {
-  if (p.bias) {
-    const u32x2 b = *(const u32x2*)(p.bias + n);
+  if (p.bias && p.bias_f32) {
+    v += *(const f32x4*)((const float*)p.bias + n);
+  } else if (p.bias) {
+    const u32x2 b = *(const u32x2*)((const uint16_t*)p.bias + n);
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] += bf16f(e & 1 ? b[e >> 1] >> 16 : b[e >> 1] & 0xffffu);
   }
@@ -399,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 2) mx_few_kernel(MxParams p) {
     float o[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = acc[8 * run + e];
-    if (p.bias) add8(*(const u32x4*)(p.bias + c), o);
+    if (p.bias) add_bias8(p, c, o);
     if (p.resid) add8(*(const u32x4*)(p.resid + (int64_t)m * p.ldr + c), o);
     *(u32x4*)(p.C + (int64_t)m * p.ldc + c) =
         u32x4{pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7])};
@@ -614,7 +628,7 @@ __global__ void __launch_bounds__(kMxThreads, 2) mx_tile_kernel(MxParams p, int 
     for (int run = 0; run < 2; ++run) {
       const int c = wcol + 32 * nb + 16 * run + 8 * (le >> 5);
       float b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (p.bias && c < p.N) add8(*(const u32x4*)(p.bias + c), b);
+      if (p.bias && c < p.N) add_bias8(p, c, b);
 #pragma unroll
       for (int mb = 0; mb < 4; ++mb) {
         u32x4* at = (u32x4*)(smem + out_at(nb, run) + 4096 * mb);
@@ -719,16 +733,13 @@ int launch_rows(const MxParams& p, hipStream_t stream) {
 }
 }  // namespace
 
-extern "C" int hstu_mxfp4_gemm(const void* A, int64_t lda, const void* a_scale, int64_t ldas, const void* W,
-                               int64_t ldw, const void* w_scale, int64_t ldws, const void* bias, const void* residual,
-                               int64_t ldr, void* C, int64_t ldc, int M, int N, int K, hipStream_t stream) {
-  MxParams p{(const uint8_t*)A, (const uint8_t*)W, (const uint8_t*)a_scale, (const uint8_t*)w_scale, lda, ldw, ldas,
-             ldws, (const uint16_t*)bias, (const uint16_t*)residual, (uint16_t*)C, ldr, ldc, M, N, K};
+namespace {
+int gemm(const MxParams& p, hipStream_t stream) {
   const int st = check_product(p, false);
-  if (st != 0 || M == 0) return st;
-  if (mx_rows_form(M, N)) return M <= 16 ? launch_rows<1, 1, false>(p, stream) : launch_rows<2, 1, false>(p, stream);
-  const int64_t few = ((int64_t)M + 63) / 64 * ((N + 63) / 64);
-  const int64_t tiles_m = ((int64_t)M + kMxTile - 1) / kMxTile, tiles_n = (N + kMxTile - 1) / kMxTile;
+  if (st != 0 || p.M == 0) return st;
+  if (mx_rows_form(p.M, p.N)) return p.M <= 16 ? launch_rows<1, 1, false>(p, stream) : launch_rows<2, 1, false>(p, stream);
+  const int64_t few = ((int64_t)p.M + 63) / 64 * ((p.N + 63) / 64);
+  const int64_t tiles_m = ((int64_t)p.M + kMxTile - 1) / kMxTile, tiles_n = (p.N + kMxTile - 1) / kMxTile;
   if (few <= kMxFewTiles) {
     hipLaunchKernelGGL(mx_few_kernel, dim3((unsigned)((few + 7) / 8 * 8)), dim3(kThreads), 0, stream, p);
     return (int)hipGetLastError();
@@ -741,16 +752,44 @@ extern "C" int hstu_mxfp4_gemm(const void* A, int64_t lda, const void* a_scale, 
                      per_xcd);
   return (int)hipGetLastError();
 }
+int linear_rows(const MxParams& p, hipStream_t stream) {
+  const int st = check_product(p, true);
+  if (st != 0 || p.M == 0) return st;
+  // Two column blocks a workgroup where that still leaves one for every CU: half of
+  // the quantisation (us, one / two: 8 x 8 192 x 8 192 (M x K x N) 17.7 / 13.0, 16 x
+  // 2 048 x 8 192 8.2 / 6.6; 16 x 4 096 x 4 096 8.3 / 9.5, 5 x 5 632 x 2 048 6.9 / 8.2).
+  return p.N >= 8192 ? launch_rows<1, 2, true>(p, stream) : launch_rows<1, 1, true>(p, stream);
+}
+MxParams product(const void* A, int64_t lda, const void* a_scale, int64_t ldas, const void* W, int64_t ldw,
+                 const void* w_scale, int64_t ldws, const void* bias, int bias_f32, const void* residual, int64_t ldr,
+                 void* C, int64_t ldc, int M, int N, int K) {
+  return MxParams{(const uint8_t*)A, (const uint8_t*)W, (const uint8_t*)a_scale, (const uint8_t*)w_scale, lda, ldw, ldas,
+                  ldws, bias, (const uint16_t*)residual, (uint16_t*)C, ldr, ldc, M, N, K, bias_f32};
+}
+}  // namespace
+
+extern "C" int hstu_mxfp4_gemm(const void* A, int64_t lda, const void* a_scale, int64_t ldas, const void* W,
+                               int64_t ldw, const void* w_scale, int64_t ldws, const void* bias, const void* residual,
+                               int64_t ldr, void* C, int64_t ldc, int M, int N, int K, hipStream_t stream) {
+  return gemm(product(A, lda, a_scale, ldas, W, ldw, w_scale, ldws, bias, 0, residual, ldr, C, ldc, M, N, K), stream);
+}
+
+extern "C" int hstu_mxfp4_gemm_bias_fp32(const void* A, int64_t lda, const void* a_scale, int64_t ldas, const void* W,
+                               int64_t ldw, const void* w_scale, int64_t ldws, const float* bias, const void* residual,
+                               int64_t ldr, void* C, int64_t ldc, int M, int N, int K, hipStream_t stream) {
+  return gemm(product(A, lda, a_scale, ldas, W, ldw, w_scale, ldws, bias, 1, residual, ldr, C, ldc, M, N, K), stream);
+}
 
 extern "C" int hstu_mxfp4_linear_rows(const void* x, int64_t ldx, const void* W, int64_t ldw, const void* w_scale,
                                       int64_t ldws, const void* bias, const void* residual, int64_t ldr, void* C,
                                       int64_t ldc, int M, int N, int K, hipStream_t stream) {
-  MxParams p{(const uint8_t*)x, (const uint8_t*)W, nullptr, (const uint8_t*)w_scale, 2 * ldx, ldw, 0,
-             ldws, (const uint16_t*)bias, (const uint16_t*)residual, (uint16_t*)C, ldr, ldc, M, N, K};
-  const int st = check_product(p, true);
-  if (st != 0 || M == 0) return st;
-  // Two column blocks a workgroup where that still leaves one for every CU: half of
-  // the quantisation (us, one / two: 8 x 8 192 x 8 192 (M x K x N) 17.7 / 13.0, 16 x
-  // 2 048 x 8 192 8.2 / 6.6; 16 x 4 096 x 4 096 8.3 / 9.5, 5 x 5 632 x 2 048 6.9 / 8.2).
-  return N >= 8192 ? launch_rows<1, 2, true>(p, stream) : launch_rows<1, 1, true>(p, stream);
+  return linear_rows(product(x, 2 * ldx, nullptr, 0, W, ldw, w_scale, ldws, bias, 0, residual, ldr, C, ldc, M, N, K),
+                     stream);
+}
+
+extern "C" int hstu_mxfp4_linear_rows_bias_fp32(const void* x, int64_t ldx, const void* W, int64_t ldw, const void* w_scale,
+                                      int64_t ldws, const float* bias, const void* residual, int64_t ldr, void* C,
+                                      int64_t ldc, int M, int N, int K, hipStream_t stream) {
+  return linear_rows(product(x, 2 * ldx, nullptr, 0, W, ldw, w_scale, ldws, bias, 1, residual, ldr, C, ldc, M, N, K),
+                     stream);
 }

@@ -77,7 +77,9 @@ EXPORTED_SYMBOLS = (
     "hstu_mxfp4_quantize",
     "hstu_mxfp4_dequantize",
     "hstu_mxfp4_gemm",
+    "hstu_mxfp4_gemm_bias_fp32",
     "hstu_mxfp4_linear_rows",
+    "hstu_mxfp4_linear_rows_bias_fp32",
 )
 
 
@@ -217,6 +219,8 @@ _SIGNATURES = {
         _i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _vp],
     ),
 }
+for _name in ("hstu_mxfp4_gemm", "hstu_mxfp4_linear_rows"):
+    _SIGNATURES[_name + "_bias_fp32"] = _SIGNATURES[_name]
 
 
 def load_library(path: Optional[Path] = None) -> ctypes.CDLL:

@@ -104,18 +104,24 @@ def _ld(t: torch.Tensor) -> int:
 
 
 def _epilogue(bias: Optional[torch.Tensor], residual: Optional[torch.Tensor], shape, device):
+    """(bias in bf16 or fp32, residual, what an entry point's name ends in): a bias is added to the fp32 sum
+    with the bits it has (of fp64's, fp32's)."""
+    entry = ""
     if bias is not None:
         if bias.shape != shape[-1:] or bias.device != device:
             raise ValueError(f"bias {tuple(bias.shape)} on {bias.device}; expected [{shape[-1]}] on {device}")
-        if bias.dtype != torch.bfloat16 or bias.stride(0) != 1:
-            bias = bias.detach().to(torch.bfloat16).contiguous()
+        if not bias.is_floating_point():
+            raise NotImplementedError(f"bias: a floating type (got {bias.dtype})")
+        if bias.dtype != torch.bfloat16:
+            bias, entry = bias.detach().to(torch.float32), "_bias_fp32"
+        bias = bias if bias.stride(0) == 1 else bias.contiguous()
         bias = bias if bias.data_ptr() % 16 == 0 else bias.clone()
     if residual is not None:
         if residual.shape != shape or residual.device != device or residual.dtype != torch.bfloat16:
             raise ValueError(f"residual {tuple(residual.shape)} {residual.dtype} on {residual.device}; expected "
                              f"{tuple(shape)} bf16 on {device}")
         residual = _aligned(residual, 16, 2 ** 63)  # 64-bit offsets
-    return bias, residual
+    return bias, residual, entry
 
 
 def _weight(weight: Packed) -> Tuple[torch.Tensor, torch.Tensor, int, int]:
@@ -131,7 +137,7 @@ def _weight(weight: Packed) -> Tuple[torch.Tensor, torch.Tensor, int, int]:
 
 def mxfp4_mm(a: Packed, weight: Packed, bias: Optional[torch.Tensor] = None,
              residual: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """a @ weight^T (+ bias [N]) (+ residual [.., N]) in bf16, fp32 accumulation:
+    """a @ weight^T (+ bias [N], bf16 or fp32) (+ residual [.., N], bf16) in bf16, fp32 accumulation:
     a a pair of [.., K], weight a pair of [N, K]; N a multiple of 16, K of 128.
     Forward only, as ``mxfp4_linear``."""
     _lib.forward_only("mxfp4_mm", bias, residual)
@@ -141,14 +147,14 @@ def mxfp4_mm(a: Packed, weight: Packed, bias: Optional[torch.Tensor] = None,
     if ac.shape[-1] != K // 2 or ac.device != wc.device:
         raise ValueError(f"a codes {tuple(ac.shape)} on {ac.device} against weight [{N}, {K}] on {wc.device}")
     shape = ac.shape[:-1] + (N,)
-    bias, r2 = _epilogue(bias, residual, shape, wc.device)
+    bias, r2, entry = _epilogue(bias, residual, shape, wc.device)
     a2, s2 = _aligned(ac, 16), _aligned(as_, 4)
     M = a2.shape[0]
     if M >= 2 ** 31 - 256:
         raise NotImplementedError("a: fewer than 2^31 rows")
     out = torch.empty(shape, dtype=torch.bfloat16, device=wc.device)
     if M > 0:
-        _lib.launch("hstu_mxfp4_gemm", wc, a2.data_ptr(), _ld(a2), s2.data_ptr(), _ld(s2), wc.data_ptr(), _ld(wc),
+        _lib.launch("hstu_mxfp4_gemm" + entry, wc, a2.data_ptr(), _ld(a2), s2.data_ptr(), _ld(s2), wc.data_ptr(), _ld(wc),
                     ws.data_ptr(), _ld(ws), _lib.ptr(bias), _lib.ptr(r2), 0 if r2 is None else _ld(r2), out.data_ptr(),
                     N, M, N, K)
     return out
@@ -170,10 +176,10 @@ def mxfp4_linear(x: torch.Tensor, weight: Packed, bias: Optional[torch.Tensor] =
     if M > ROWS_QUANT or M * K > VALUES_QUANT:
         return mxfp4_mm(quantize_mxfp4(x), weight, bias, residual)
     shape = shape[:-1] + (N,)
-    bias, r2 = _epilogue(bias, residual, shape, wc.device)
+    bias, r2, entry = _epilogue(bias, residual, shape, wc.device)
     out = torch.empty(shape, dtype=torch.bfloat16, device=wc.device)
     if M > 0:
         x2 = _aligned(x, 16)
-        _lib.launch("hstu_mxfp4_linear_rows", wc, x2.data_ptr(), _ld(x2), wc.data_ptr(), _ld(wc), ws.data_ptr(), _ld(ws),
+        _lib.launch("hstu_mxfp4_linear_rows" + entry, wc, x2.data_ptr(), _ld(x2), wc.data_ptr(), _ld(wc), ws.data_ptr(), _ld(ws),
                     _lib.ptr(bias), _lib.ptr(r2), 0 if r2 is None else _ld(r2), out.data_ptr(), N, M, N, K)
     return out

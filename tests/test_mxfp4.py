@@ -263,6 +263,49 @@ def test_past_32_bit_offsets(hip_lib):
     assert not out[:-5].any()
 
 
+@gpu
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.float64])
+@pytest.mark.parametrize("M,N,K", [(5, 48, 384), (16, 8208, 128), (24, 272, 256), (300, 272, 640), (2600, 2576, 384)])
+def test_bias_keeps_its_bits(hip_lib, M, N, K, dtype, residual):
+    """A bias is not rounded to bf16 on the way to the fp32 sum.  Every code is 0, so the sum is exact: the bias
+    (fp32 at the most: 2^-24), plus the residual (one rounding, 2^-24 of the magnitudes), rounded to bf16 once.
+    Biases next to the middle of two bf16 values, which their own rounding would move to the other one."""
+    import hstu_amd
+
+    b = rnd((N,), 6, 1.0, torch.float32)
+    b = (b.bfloat16().float() * (1 + 2.0 ** -8 + 2.0 ** -10 * torch.rand(N, generator=torch.Generator().manual_seed(3)))).to(dtype).to(DEV)
+    r = rnd((M, N), 7, 2.0 ** -8).to(DEV) if residual else None
+    x, w = torch.zeros((M, K), dtype=torch.bfloat16, device=DEV), hstu_amd.quantize_mxfp4(torch.zeros((N, K), device=DEV))
+    want, mag = b.double().expand(M, N), b.double().abs().expand(M, N)
+    if residual:
+        want, mag = want + r.double(), mag + r.double().abs()
+    tol = want.abs() * HALF + mag * 2.0 ** -23
+    got = [hstu_amd.mxfp4_linear(x, w, bias=b, residual=r), hstu_amd.mxfp4_mm(hstu_amd.quantize_mxfp4(x), w, bias=b, residual=r)]
+    for out in got:
+        off = (out.double() - want).abs()
+        assert (off <= tol).all(), float((off / tol).max())
+        # half a step of bf16 at this value, not of the largest mantissa's: nearest, but for the ties of fp32
+        near = b.float().expand(M, N) + (r.float() if residual else 0)
+        assert torch.equal(out, near.bfloat16())
+    odd = torch.zeros(N + 1, dtype=dtype, device=DEV)[1:].copy_(b)  # not 16-byte aligned; every second of a longer one
+    for same in (odd, torch.stack((b, b), 1)[:, 0]):
+        assert torch.equal(hstu_amd.mxfp4_linear(x, w, bias=same, residual=r), got[0])
+    with pytest.raises(NotImplementedError):
+        hstu_amd.mxfp4_linear(x, w, bias=torch.zeros(N, dtype=torch.int32, device=DEV))
+
+
+def test_bias_type_goes_to_the_entry_point():
+    """No bias is cast to bf16 (no device is touched)."""
+    from hstu_amd import mxfp4
+
+    for dtype, kept, entry in ((torch.bfloat16, torch.bfloat16, ""), (torch.float32, torch.float32, "_bias_fp32"),
+                               (torch.float16, torch.float32, "_bias_fp32")):
+        b = rnd((48,), 6, 1.0, dtype)
+        got = mxfp4._epilogue(b, None, (2, 48), b.device)
+        assert got[0].dtype == kept and torch.equal(got[0], b.to(kept)) and got[2] == entry
+
+
 def test_tile_epilogue_orders_its_lanes():
     """The tile form's outputs pass between the lanes of a wave through LDS, the residual before them: each
     exchange has a wave-level order between the lanes' writes and the others' reads, in the source, since a
