@@ -30,7 +30,8 @@ template <int CTRL, int ROW_MASK = 0xf>
 __device__ __forceinline__ float dpp_move(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROW_MASK, 0xf, true));
 }
-// sum, and maximum of values >= 0 (lanes without a source read 0), over the wave
+// sum, and largest magnitude (as its bits, so that a NaN is the largest; lanes without
+// a source read 0), over the wave
 __device__ __forceinline__ float wave_sum(float v) {
   v += dpp_move<0x111>(v);
   v += dpp_move<0x112>(v);
@@ -40,14 +41,19 @@ __device__ __forceinline__ float wave_sum(float v) {
   v += dpp_move<0x143, 0xc>(v);
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
-__device__ __forceinline__ float wave_max0(float v) {
-  v = __builtin_fmaxf(v, dpp_move<0x111>(v));
-  v = __builtin_fmaxf(v, dpp_move<0x112>(v));
-  v = __builtin_fmaxf(v, dpp_move<0x114>(v));
-  v = __builtin_fmaxf(v, dpp_move<0x118>(v));
-  v = __builtin_fmaxf(v, dpp_move<0x142, 0xa>(v));
-  v = __builtin_fmaxf(v, dpp_move<0x143, 0xc>(v));
-  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+template <int CTRL, int ROW_MASK = 0xf>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROW_MASK, 0xf, true));
+}
+__device__ __forceinline__ uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t wave_top(uint32_t v) {
+  v = dpp_max<0x111>(v);
+  v = dpp_max<0x112>(v);
+  v = dpp_max<0x114>(v);
+  v = dpp_max<0x118>(v);
+  v = dpp_max<0x142, 0xa>(v);
+  v = dpp_max<0x143, 0xc>(v);
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 // Eight consecutive values of a row from element c0 on.  VEC: whole and 16-byte
@@ -179,7 +185,8 @@ __global__ void __launch_bounds__(BLOCK) rms_fwd_kernel(FwdArgs a) {
     const int64_t row = r0 + group;
     const bool live = row < a.rows;
     float h[NV][8];
-    float ss = 0.f, top = 0.f;
+    float ss = 0.f;
+    uint32_t top = 0;  // bits of max|h w|
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c0 = 8 * (tg + G * i);
@@ -200,29 +207,33 @@ __global__ void __launch_bounds__(BLOCK) rms_fwd_kernel(FwdArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         ss = __builtin_fmaf(h[i][e], h[i][e], ss);
-        if constexpr (OUT8) top = __builtin_fmaxf(top, __builtin_fabsf(h[i][e] * w[i][e]));
+        if constexpr (OUT8) top = max(top, magnitude(h[i][e] * w[i][e]));
       }
     }
     ss = wave_sum(ss);
-    if constexpr (OUT8) top = wave_max0(top);
+    if constexpr (OUT8) top = wave_top(top);
     if constexpr (WPG > 1) {
-      if ((tg & 63) == 0) red[par][group][wg][0] = ss, red[par][group][wg][1] = top;
+      if ((tg & 63) == 0) red[par][group][wg][0] = ss, red[par][group][wg][1] = __builtin_bit_cast(float, top);
       __syncthreads();  // two copies: the next row's sums do not meet this row's readers
       ss = 0.f;
-      top = 0.f;
+      top = 0;
 #pragma unroll
-      for (int k = 0; k < WPG; ++k) ss += red[par][group][k][0], top = __builtin_fmaxf(top, red[par][group][k][1]);
+      for (int k = 0; k < WPG; ++k) ss += red[par][group][k][0], top = max(top, magnitude(red[par][group][k][1]));
     }
     if (!live) continue;
     const float rstd = __builtin_amdgcn_rsqf(ss * a.inv_d + a.eps);
     if (a.rstd && tg == 0) a.rstd[row] = rstd;
-    float s = 1.f, is = 1.f, up = 1.f;
+    float s = 1.f, is = 1.f, up = 1.f, den = 1.f;
     if constexpr (OUT8) {
       // max|y| as max|h w| rstd: one reduction for both statistics
-      top *= rstd;
-      s = a.scale_in ? given : top > 0.f ? top / 448.f : top == 0.f ? 1.f / 448.f : top;  // NaN stays
-      up = __builtin_fabsf(s) < 0x1p-100f ? 0x1p64f : 1.f;  // 1 / s would overflow: y 2^64 over s 2^64
-      is = 1.f / (s * up);
+      const float m = __builtin_bit_cast(float, top) * rstd;
+      s = a.scale_in ? given : m > 0.f ? m / 448.f : m == 0.f ? 1.f / 448.f : m;  // NaN stays
+      // y / s as (y up) / den: 1 / s would overflow for a small s (2^64 in both), and an
+      // infinite one has no reciprocal to correct with (y 0: zeros, NaN for an infinite y)
+      const bool far = __builtin_fabsf(s) == __builtin_huge_valf();
+      up = __builtin_fabsf(s) < 0x1p-100f ? 0x1p64f : far ? 0.f : 1.f;
+      den = far ? 1.f : s * up;
+      is = 1.f / den;
       if (!a.scale_in && tg == 0) a.scale_out[row] = s;
     }
 #pragma unroll
@@ -233,7 +244,7 @@ __global__ void __launch_bounds__(BLOCK) rms_fwd_kernel(FwdArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         y[e] = h[i][e] * rstd * w[i][e];
-        if constexpr (OUT8) y[e] = sat_e4m3(div_by(y[e] * up, s * up, is));
+        if constexpr (OUT8) y[e] = sat_e4m3(div_by(y[e] * up, den, is));
       }
       if constexpr (OUT8) store8_e4m3<VEC>(a.y + row * a.ldy, c0, a.D, y);
       else store8<F32, VEC>(a.y + row * a.ldy, c0, a.D, y);

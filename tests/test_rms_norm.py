@@ -147,6 +147,34 @@ def test_non_finite_rows_stay_in_their_row(hip_lib):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [520, 513, 1032, 5120, 16384])
+def test_non_finite_weights_and_scales(hip_lib, D, dtype):
+    """max|y| of a row with a NaN is NaN, wherever the NaN comes from, and so are its scale and its row; an
+    infinite scale takes every finite y to zero."""
+    import hstu_amd
+
+    x, w = make(5, D, dtype, 6).to(DEV), make_weight(D, torch.float32).to(DEV)
+    x[3] = 0  # its y is 0, NaN where the weight is not finite
+    bad = w.clone()
+    bad[D // 2] = float("nan")
+    y8, s = hstu_amd.rms_norm_fp8(x, bad, EPS)
+    assert s.isnan().all() and y8.float().isnan().all()
+    y8, s = hstu_amd.rms_norm_fp8(x, bad, EPS, scale=torch.ones(1, device=DEV))  # a given scale: the column alone
+    assert y8[:, D // 2].float().isnan().all() and int(y8.float().isnan().sum()) == 5
+    bad[D // 2] = float("inf")
+    y8, s = hstu_amd.rms_norm_fp8(x, bad, EPS)
+    live = torch.tensor([0, 1, 2, 4], device=DEV)
+    assert s[live].isinf().all() and s[3].isnan() and y8[3].float().isnan().all()
+    assert y8[live, D // 2].float().isnan().all() and int(y8[live].float().isnan().sum()) == 4
+    assert not y8[live].float().nan_to_num(0).any()
+    y8, _ = hstu_amd.rms_norm_fp8(x, w, EPS, scale=torch.full((1,), float("inf"), device=DEV))
+    assert not y8.float().any()
+    y8, _ = hstu_amd.rms_norm_fp8(x, w, EPS, scale=torch.full((1,), float("nan"), device=DEV))
+    assert y8.float().isnan().all()
+
+
+@gpu
 @pytest.mark.parametrize("shape", [(0, 512), (2, 0, 512), (2, 3, 512), (512,)])
 def test_leading_dimensions_and_no_rows(hip_lib, shape):
     import hstu_amd
