@@ -418,3 +418,34 @@ def test_bf16_gemm_forms_same_bytes(hip_lib, N, K, resid, kind):
     wide = torch.empty(M, N + 4, dtype=torch.bfloat16, device=DEV)
     run(a, r, out=wide[:, :N])
     assert torch.equal(full, wide[:, :N].contiguous().view(torch.int16))
+
+
+@pytest.mark.parametrize("resid", [False, True])
+@pytest.mark.parametrize("M,N,K", [(128 * 19 + 37, 2304, 192), (128 * 16 + 1, 4096, 128), (128 * 9, 4352, 256),
+                                   (128 * 7 + 100, 8192, 128)])
+def test_bf16_gemm_tile_groups(hip_lib, M, N, K, resid):
+    """More than 2 048 columns: the tiles run in groups of eight row panels, the last group of fewer, the last
+    panel ragged.  Every tile is there once: the bytes are those of column ranges of at most 2 048, which run
+    panel by panel (or in the other forms), and nothing is written past the last row."""
+    fp8 = _fp8()
+    assert -(-M // 128) * (N // 128) > 256  # the two-workgroup form
+    g = torch.Generator().manual_seed(N + K)
+    a = torch.randn(M, K, generator=g).to(torch.bfloat16).to(DEV)
+    w = (torch.randn(N, K, generator=g) / K ** 0.5).to(torch.bfloat16).to(DEV)
+    b = (0.1 * torch.randn(N, generator=g)).to(torch.bfloat16).to(DEV)
+    r = torch.randn(M, N, generator=g).to(torch.bfloat16).to(DEV) if resid else None
+    out = torch.full((M + 130, N), 7.0, dtype=torch.bfloat16, device=DEV)
+    full = fp8.bf16_gemm(a, w, bias=b, residual=r, silu_cols=(256, 2048), out=out[:M]).view(torch.int16)
+    assert (out[M:] == 7).all()
+    for c in range(0, N, 2048):
+        part = slice(c, min(c + 2048, N))
+        silu = (256, 2048) if c == 0 else None
+        got = fp8.bf16_gemm(a, w[part], bias=b[part], residual=None if r is None else r[:, part], silu_cols=silu)
+        assert torch.equal(full[:, part], got.view(torch.int16)), c
+    want = a.double() @ w.double().t() + b.double()
+    want[:, 256:2048] *= torch.sigmoid(want[:, 256:2048])
+    mag = a.double().abs() @ w.double().abs().t() + b.double().abs() + 1  # +1: SiLU's own argument, twice a rounding
+    if resid:
+        want, mag = want + r.double(), mag + r.double().abs()
+    off = (full.view(torch.bfloat16).double() - want).abs()
+    assert (off <= want.abs() * 2.0 ** -8 + (K + 32) * 2.0 ** -23 * mag).all()

@@ -311,6 +311,86 @@ def test_side_stream_graph_and_same_bytes(hip_lib):
         assert all(torch.equal(a, b) for a, b in zip(captured, step())), k
 
 
+# ---------------------------------------------------------------- each form by name
+def form(M, F, k_bytes):
+    """The form that a call of M rows takes (the dispatch of csrc/hstu_gated.hip), so that a case below fails when
+    a changed threshold takes it to another one."""
+    if M <= 32 if F <= 4096 else F > 8192 and M <= 16:
+        return "rows"
+    return "middle" if -(-M // 64) * (F // 32) <= 768 or k_bytes < 256 else "tile"
+
+
+@gpu
+@pytest.mark.parametrize("name", ACTS)
+@pytest.mark.parametrize("M,D,F", [(2100, 256, 1024), (1700, 1280, 1152)])
+def test_tile_form_keeps_g_and_u(hip_lib, M, D, F, name):
+    assert form(M, F, 2 * D) == "tile"
+    test_kept_and_computed_again_give_the_same_bytes(hip_lib, M, D, F, name)
+
+
+@gpu
+@pytest.mark.parametrize("name", ACTS)
+def test_tile_form_at_every_size_of_the_gate(hip_lib, name):
+    assert form(2100, 1024, 512) == "tile"
+    test_every_size_of_the_gate(hip_lib, name, 2100)
+
+
+@gpu
+@pytest.mark.parametrize("name", ACTS)
+@pytest.mark.parametrize("M,D,F,which", [(5, 256, 8320, "rows"), (16, 256, 10240, "rows"), (17, 256, 8320, "middle"),
+                                         (1900, 2304, 640, "middle"), (1700, 1280, 1152, "tile")])
+def test_wide_blocks(hip_lib, M, D, F, which, name):
+    """The row form of many columns, and wide x, whose dx has more than eight column tiles (their grouped order)."""
+    assert form(M, F, 2 * D) == which
+    test_forward(hip_lib, M, D, F, name)
+    test_backward(hip_lib, M, D, F, name)
+
+
+@gpu
+@pytest.mark.parametrize("name", ACTS)
+@pytest.mark.parametrize("modes", [(0, 0, 1), (0, 1, 0), (1, 0, 1), (1, 1, 0), (1, 1, 1), (0, 0, 0)])
+@pytest.mark.parametrize("M,D,F,which", [(5, 384, 256, "rows"), (20, 128, 640, "rows"), (9, 256, 8320, "rows"),
+                                         (65, 256, 384, "middle"), (4100, 128, 512, "middle"), (2100, 384, 1024, "tile")])
+def test_e4m3_activations_and_scales(hip_lib, M, D, F, which, modes, name):
+    """Scales of x, gate and up by row or one, each by itself."""
+    import hstu_amd
+
+    def e4m3(v, by_row):
+        a = v.float().abs()
+        s = (a.amax(-1, keepdim=True) if by_row else a.max().reshape(1, 1)) / 448
+        return (v.float() / s).clamp(-448, 448).to(torch.float8_e4m3fn), s.reshape(-1)
+
+    assert form(M, F, D) == which
+    x, wg, wu = rnd((M, D), 3).to(DEV), *weights(F, D)
+    (x8, xs), (g8, gs), (u8, us) = (e4m3(t, m) for t, m in zip((x, wg, wu), modes))
+    h = hstu_amd.gated_linear_fp8(x8, xs, (g8, gs), (u8, us), name)
+    x, wg, wu = (q.double() * s.double().reshape(-1, 1) for q, s in ((x8, xs), (g8, gs), (u8, us)))
+    want, tol = h_bound(x, wg, wu, name)
+    within(h, want, tol, "h")
+
+
+@gpu
+@pytest.mark.parametrize("name", ACTS)
+@pytest.mark.parametrize("M,which", [(26, "rows"), (200, "middle"), (2100, "tile")])
+def test_e4m3_at_every_size_of_the_gate(hip_lib, name, M, which):
+    """g = +-v and u = v, exactly, by the row's scale: a(g) u from 0 to 1e36, an s below 2^-126 as 0."""
+    import hstu_amd
+
+    v = torch.tensor([0, 1e-30, 1e-3, 0.3, 1, 1.28, 5, 30, 60, 86, 100, 1e3, 1e18]).bfloat16().float()
+    v = torch.cat((v, v)).repeat(-(-M // 26))[:M].to(DEV)
+    sign = torch.cat((torch.ones(13), -torch.ones(13))).repeat(-(-M // 26))[:M].to(DEV)
+    F = 1024
+    assert form(M, F, 256) == which
+    x, wg, wu = torch.zeros((M, 256), device=DEV), torch.zeros((F, 256), device=DEV), torch.zeros((F, 256), device=DEV)
+    x[:, 0], x[:, 1], wg[5, 0], wu[5, 1] = sign, 1, 1, 1
+    x8, g8, u8 = (t.to(torch.float8_e4m3fn) for t in (x, wg, wu))
+    one = torch.ones(1, device=DEV)
+    h = hstu_amd.gated_linear_fp8(x8, v, (g8, one), (u8, one), name)
+    want = orc.activation_ref(name, (sign * v).double())[0] * v.double()
+    within(h[:, 5], want, want.abs() * (HALF + ARG) + 2.0 ** -100, "h")
+    assert not h[:, :5].any()
+
+
 # ---------------------------------------------------------------- refusals
 def test_refusals():
     import hstu_amd

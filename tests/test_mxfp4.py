@@ -148,6 +148,18 @@ def test_product(hip_lib, M, N, K, bias, residual):
 
 
 @gpu
+@pytest.mark.parametrize("bias,residual", [(False, False), (True, True)])
+@pytest.mark.parametrize("N", [8192, 8208])
+@pytest.mark.parametrize("M,K", [(1, 128), (7, 384), (16, 1024), (16, 4096), (3, 8192)])
+def test_few_rows_of_many_outputs(hip_lib, M, N, K, bias, residual):
+    """Two column blocks a workgroup where x is quantised on the way, the last one of 16 columns or of 32."""
+    from hstu_amd import mxfp4
+
+    assert M <= mxfp4.ROWS_QUANT and M * K <= mxfp4.VALUES_QUANT
+    test_product(hip_lib, M, N, K, bias, residual)
+
+
+@gpu
 def test_product_special_values(hip_lib):
     """NaN blocks make their rows (columns) NaN and no others; zero blocks and far scales are exact."""
     import hstu_amd

@@ -74,6 +74,19 @@ def test_forward_and_backward(hip_lib, rows, D, dtype, residual):
 @gpu
 @pytest.mark.parametrize("residual", [False, True])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,D,blocks", [(1700, 2048, 768), (1700, 4096, 768), (1600, 2050, 768), (600, 5120, 256),
+                                           (520, 8192, 256), (600, 4100, 256)])
+def test_blocks_of_several_rows(hip_lib, rows, D, dtype, residual, blocks):
+    """Twice as many rows as the backward has blocks: the loads ahead go round more than once, and end."""
+    import hstu_amd._lib as lib
+
+    assert lib.fn("hstu_rms_norm_bwd_workspace_bytes")(rows, D) == blocks * D * 4 and rows > 2 * blocks
+    test_forward_and_backward(hip_lib, rows, D, dtype, residual)
+
+
+@gpu
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("rows,D", [(1, 1), (3, 7), (33, 512), (5, 520), (4, 1000), (6, 2048), (3, 5120), (2, 16380)])
 def test_e4m3_output(hip_lib, rows, D, dtype, residual):
     import hstu_amd
