@@ -305,6 +305,21 @@ def launch(name: str, t, *args) -> None:
         check(status, name)
 
 
+def _leaves(ctx):
+    """The accumulation nodes of a function's inputs that are leaves, or views and casts of one."""
+    for node, _ in ctx.next_functions:
+        for _ in range(8):
+            if node is None:
+                break
+            above = [n for n, _ in node.next_functions if n is not None]
+            if not above:
+                yield node
+                break
+            if len(above) > 1:
+                break
+            node = above[0]
+
+
 def guard_graph(ctx, t) -> None:
     """Called in an autograd function's forward: refuses a graph capture while a
     graph built outside it on the default stream holds one of the same leaves.
@@ -314,13 +329,12 @@ def guard_graph(ctx, t) -> None:
     graph does, and a capture looks for the mark."""
     raw = _raw or _bind_raw()
     if raw[1](t.device.index) == 0:
-        for node, _ in ctx.next_functions:
-            if node is not None and not node.next_functions:
-                node.metadata["hstu_default_stream"] = True
+        for node in _leaves(ctx):
+            node.metadata["hstu_default_stream"] = True
         return
     if raw[3]():
-        for node, _ in ctx.next_functions:
-            if node is not None and not node.next_functions and "hstu_default_stream" in node.metadata:
+        for node in _leaves(ctx):
+            if "hstu_default_stream" in node.metadata:
                 raise HstuKernelError("graph capture of a function of a leaf that a graph outside the capture, built on "
                                       "the default stream, still holds: let go of that graph's outputs first, or warm "
                                       "up on a side stream")

@@ -335,3 +335,32 @@ def test_last_position_of_every_sequence(hip_lib):
 
         for got, want in zip(all_of(x, far8), all_of(x.contiguous(), x8)):
             assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("use", [lambda t: t, lambda t: t[:4], lambda t: t.t().t(), lambda t: t.float().bfloat16()[1:5]])
+def test_capture_guard_sees_leaves_through_views(monkeypatch, use):
+    """A leaf that an eager graph on the default stream holds is refused in a capture also where both use a part
+    of it, its transpose or a cast (gate and up of one parameter).  Without a device: the streams are stand-ins."""
+    from hstu_amd import HstuKernelError, _lib, hstu_gated, hstu_rms_norm
+
+    stream, capturing = [0], [False]
+    monkeypatch.setattr(_lib, "_raw", (lambda: 0, lambda index: stream[0], None, lambda: capturing[0]))
+    monkeypatch.setattr(hstu_gated, "gated_linear_fwd", lambda x, *a, **k: x.new_ones(2, 128))
+    monkeypatch.setattr(hstu_rms_norm, "rms_norm_fwd", lambda x, *a, **k: (torch.ones_like(x), x, x.new_ones(len(x)), None))
+    monkeypatch.setattr(_lib, "fn", lambda name: lambda *a: 4)
+    leaf = torch.ones(8, 8, dtype=torch.bfloat16, requires_grad=True)
+    other = torch.ones(8, 8, dtype=torch.bfloat16)
+
+    for call in (lambda t: hstu_gated.gated_linear(other, use(t), use(t), recompute=True), lambda t: hstu_rms_norm.rms_norm(use(t), other)):
+        def capture():
+            stream[0], capturing[0] = 7, True
+            try:
+                return call(leaf)
+            finally:
+                stream[0], capturing[0] = 0, False
+
+        alive = call(leaf)
+        with pytest.raises(HstuKernelError):
+            capture()
+        del alive
+        capture()  # let go of: served
