@@ -340,26 +340,31 @@ def guard_graph(ctx, t) -> None:
                                       "up on a side stream")
 
 
-_forward_ad = None
+_ad = None
+
+
+def _bind_ad():
+    global _ad
+    import torch
+    from torch.autograd import forward_ad
+
+    _ad = (torch.is_grad_enabled, forward_ad)
+    return _ad
 
 
 def no_tangent(name: str, *tensors) -> None:
     """Refuses dual tensors of ``torch.autograd.forward_ad``, which do not require
     grad: a kernel takes their values alone, and the tangent would be lost."""
-    global _forward_ad
-    if _forward_ad is None:
-        from torch.autograd import forward_ad as _forward_ad
-    if _forward_ad._current_level >= 0:
+    forward_ad = (_ad or _bind_ad())[1]
+    if forward_ad._current_level >= 0:
         for t in tensors:
-            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 raise NotImplementedError(f"{name}: forward-mode derivatives (an input has a tangent)")
 
 
 def forward_only(name: str, *tensors) -> None:
     """Refuses inputs whose derivative a function without a backward would cut off."""
-    import torch
-
-    if torch.is_grad_enabled():
+    if (_ad or _bind_ad())[0]():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise NotImplementedError(f"{name} is forward only and an input requires grad: call it under "
