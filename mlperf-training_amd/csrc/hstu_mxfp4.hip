@@ -222,7 +222,7 @@ __device__ __forceinline__ void mx_store4(const MxParams& p, int m, int n, f32x4
 }
 
 // Row form, for few rows, where the weights' bytes and the calls are the time (5 x 5 632
-// against 2 048 outputs, 6.1 MB of weights, 6.8-7.3 us with the quantisation): 16 NB
+// against 2 048 outputs, 6.1 MB of weights, 6.2-7.3 us with the quantisation): 16 NB
 // columns and 16 MB rows a workgroup, whose WAVES waves take one contiguous piece
 // of the contraction each, operands going from memory to registers as the MFMA takes
 // them, and meet in LDS, where the blocks are summed over the waves in order.
@@ -320,7 +320,9 @@ __device__ __forceinline__ f32x16 mfma32_mx4(u32x4 a, u32x4 b, f32x16 c, int sa,
 // each), two workgroups per CU, a ring of four 16 KiB steps (256 values of k) with
 // three steps' loads in flight and one barrier a step; scales of two steps at a time
 // in a ring of four.  Fragments, scale bytes and the last half step as in the tile
-// form below.
+// form below.  Bound by what its tiles read from L2, 16 KiB a step each (256 x 8 192 x 8 192:
+// 512 tiles, 268 MB).  Measured (us, rows at K = N = 8 192): 64 12.8, 256 21.6, 512 38.3, where
+// the weights' bytes are 7.0.
 constexpr int kMxFewStages = 4, kMxFewStage = 2 * 64 * 128, kMxFewScales = 4 * 1024;
 __global__ void __launch_bounds__(kThreads, 2) mx_few_kernel(MxParams p) {
   __shared__ __attribute__((aligned(1024))) uint8_t ring[kMxFewStages][kMxFewStage];
@@ -440,7 +442,8 @@ __global__ void __launch_bounds__(kThreads, 2) mx_few_kernel(MxParams p) {
 // Measured: 8 192^3 282-330 us, 3.3-3.9 PFLOP/s (a large library product in e4m3 2.6;
 // the instruction alone 6.5 from registers of random codes, the power limit, 9.9 of
 // zeros).  Without its MFMAs 206 us, without its loads 235; a workgroup has the CU's LDS
-// to itself, so nothing runs under its epilogue.
+// to itself, so nothing runs under its epilogue.  43 registers are spilled: four are read
+// back in the main loop's two steps, the rest around the epilogue.
 constexpr int kMxThreads = 512;
 constexpr int kMxTile = 256;
 constexpr int kMxOperand = kMxTile * 128;    // 32 KiB

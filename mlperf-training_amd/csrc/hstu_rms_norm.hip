@@ -163,6 +163,10 @@ struct FwdArgs {
 // block's.  Measured: 162 251 x 512 bf16 with residual to e4m3 (581 MB) 108 us, 5.4 TB/s;
 // 37 429 x 512 bf16 with residual (153 MB) 26-30 us; 4 099 x 5 120 fp32 (168 MB) 33-39 us;
 // a large copy runs at 5.1 TB/s.  One row of 2 048 2.6 us, a launch's own time.
+// Without VEC (rows not 16-byte aligned, D % 8) every lane makes eight accesses of one
+// element where it makes one of 16 bytes, and these requests bound it, forward and
+// backward (bf16 with residual; aligned / not): 37 429 x 512 / 513 23.5 / 78 us, its e4m3
+// 24 / 85, its backward 26 / 93; 162 251 x 512 / 509 117 / 407, backward 138 / 401.
 template <bool F32, bool VEC, int G, int NV, int BLOCK, bool OUT8>
 __global__ void __launch_bounds__(BLOCK) rms_fwd_kernel(FwdArgs a) {
   constexpr int GROUPS = BLOCK / G, WPG = G / 64;
